@@ -2,7 +2,8 @@
 
 The product is libccinfer_attn.so (built in-tree by ccinfer_amd.build). This package is the
 Python host side: a ctypes binding of the C ABI (`_lib`), torch-facing operators that mirror
-the reference's backend ops (`ops`), and seeded synthetic workloads (`workloads`).
+the reference's backend ops (`ops`), rotary positions (`rope`), pages of the cache (`pages`),
+and seeded synthetic workloads (`workloads`).
 """
 from .ops import (  # noqa: F401
     ITEM_DECODE,
@@ -24,6 +25,16 @@ from .ops import (  # noqa: F401
     write_kv_cache_fp8,
     fp8_scale_numel,
 )
+from .pages import (  # noqa: F401
+    KV_EXHAUSTED,
+    KV_INVALID_TABLE,
+    compact_kv_blocks,
+    compact_workspace_size,
+    copy_kv_blocks,
+    update_block_tables,
+    update_tables_workspace_size,
+)
+from .rope import build_rope_cache, qkv_norm_rope, rope_frequencies, rotary_embedding  # noqa: F401
 
 __all__ = [
     "ITEM_DECODE",
@@ -44,4 +55,15 @@ __all__ = [
     "write_kv_cache",
     "write_kv_cache_fp8",
     "fp8_scale_numel",
+    "KV_EXHAUSTED",
+    "KV_INVALID_TABLE",
+    "build_rope_cache",
+    "compact_kv_blocks",
+    "compact_workspace_size",
+    "copy_kv_blocks",
+    "qkv_norm_rope",
+    "rope_frequencies",
+    "rotary_embedding",
+    "update_block_tables",
+    "update_tables_workspace_size",
 ]

@@ -11,7 +11,9 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libccinfer_attn.so"
 
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
+_c_i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
+_doubles = ctypes.POINTER(ctypes.c_double)
 
 # name -> (restype, argtypes); must match include/ccinfer_attn.h.
 SIGNATURES = {
@@ -52,6 +54,34 @@ SIGNATURES = {
     ),
     "ccinfer_prefill_attention_fp8_overlap": (
         _c_int, [_vp] * 9 + [_c_int] * 7 + [_vp, _c_size, _vp, _vp, _vp, _vp]),
+    "ccinfer_rope_frequencies": (
+        _c_int, [_c_int, ctypes.c_double, _c_int, _doubles, _doubles, _doubles]),
+    "ccinfer_build_rope_cache": (
+        _c_int, [_doubles, _c_int, ctypes.c_double, _c_int, _c_int, _vp, _vp]),
+    "ccinfer_rotary_embedding": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64,
+         _c_i64] + [_c_int] * 8 + [_vp],
+    ),
+    "ccinfer_qkv_norm_rope": (
+        _c_int,
+        [_vp, _c_i64, _vp, _c_int, _vp, _c_int] + [_vp] * 8 + [_c_int] * 8
+        + [ctypes.c_float, ctypes.c_float, _vp],
+    ),
+    "ccinfer_copy_kv_blocks": (
+        _c_int, [_vp] * 6 + [_c_int] * 2 + [_c_i64] * 2 + [_c_int] * 4 + [_vp, _vp]),
+    "ccinfer_update_tables_workspace_size": (_c_size, [_c_int] * 3),
+    "ccinfer_update_block_tables": (
+        _c_int,
+        [_vp] * 6 + [_c_int] * 3 + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
+        + [_vp, _vp, _c_size, _vp],
+    ),
+    "ccinfer_compact_workspace_size": (_c_size, [_c_int]),
+    "ccinfer_compact_kv_blocks": (
+        _c_int,
+        [_vp, _vp, _c_int, _c_int] + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
+        + [_vp] * 5 + [_c_size, _vp],
+    ),
     "ccinfer_error_message": (ctypes.c_char_p, [_c_int]),
     "ccinfer_version": (ctypes.c_char_p, []),
 }

@@ -47,16 +47,24 @@ SOURCES = [
     CSRC / "batch_meta.hip",
     CSRC / "kv_fp8.hip",
     CSRC / "noalloc.hip",
+    CSRC / "rope_table.hip",
+    CSRC / "rotary.hip",
+    CSRC / "kv_pages.hip",
     CSRC / "capi.cpp",
     CSRC / "dropin" / "launchers.cpp",
     CSRC / "dropin" / "hip_backend.cpp",
 ]
 
+# Sources that do rely on NaN semantics: a NaN in a row reaches the fp8 cache as a NaN, and a
+# NaN parameter of the frequencies is refused.
+HONOR_NANS = {"rotary.hip", "rope_table.hip"}
+
 
 def _compile(src: Path) -> Path:
     obj = BUILD / (src.stem + src.suffix.replace(".", "_") + ".o")
     lang = ["-x", "hip"] if src.suffix == ".hip" else []
-    cmd = [HIPCC, *HIP_FLAGS, *lang, "-c", str(src), "-o", str(obj)]
+    nans = ["-fhonor-nans"] if src.name in HONOR_NANS else []
+    cmd = [HIPCC, *HIP_FLAGS, *nans, *lang, "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")

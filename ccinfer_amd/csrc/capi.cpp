@@ -250,6 +250,71 @@ int prefill_fp8_entry(const void* q, const void* k_cache, const void* v_cache,
         as_stream(stream), overlap));
 }
 
+// eps > 0 (backend.h:84); NaN and inf are tested on the bits, which stays correct when the
+// compiler is told that NaNs do not occur.
+bool finite_bits(float v) {
+    uint32_t bits;
+    std::memcpy(&bits, &v, sizeof bits);
+    return (bits & 0x7f800000u) != 0x7f800000u;
+}
+
+bool finite_bits(double v) {
+    uint64_t bits;
+    std::memcpy(&bits, &v, sizeof bits);
+    return (bits & 0x7ff0000000000000u) != 0x7ff0000000000000u;
+}
+
+bool rotary_shape_ok(int tokens, int heads, int head_dim, int rotary_dim, int rope_max) {
+    return tokens > 0 && heads > 0 && head_dim > 0 && head_dim % 2 == 0 &&
+           head_dim <= kRotaryMaxHeadDim && rotary_dim > 0 && rotary_dim % 2 == 0 &&
+           rotary_dim <= head_dim && rope_max > 0 &&
+           fits_int(static_cast<int64_t>(tokens) * heads);
+}
+
+// The caches of a page operator. Both or neither of the scale arrays; an fp8 cache's blocks
+// have 16 tokens (its scales lie [block][head][16]).
+bool kv_layers_of(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int num_layers,
+                  int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                  int n_kv_heads, int head_dim, int cache_block_size, KvLayers& kv) {
+    if (!k_cache || !v_cache || (k_scale == nullptr) != (v_scale == nullptr)) return false;
+    if (num_layers <= 0 || num_layers > 32767 || num_blocks <= 0 || n_kv_heads <= 0 ||
+        head_dim <= 0 || cache_block_size <= 0)
+        return false;
+    const bool fp8 = k_scale != nullptr;
+    if (fp8 && cache_block_size != kFp8Block) return false;
+    const int64_t token = static_cast<int64_t>(n_kv_heads) * head_dim * (fp8 ? 1 : 2);
+    if (!fits_int(token) || !fits_int(token * cache_block_size) ||
+        !fits_int(static_cast<int64_t>(num_blocks) * cache_block_size))
+        return false;
+    // layers one after the other: none begins inside another one
+    const int64_t layer = token * cache_block_size * num_blocks;
+    const int64_t scales = static_cast<int64_t>(num_blocks) * n_kv_heads * kFp8Block;
+    if (num_layers > 1 && (layer_stride < layer || (!fp8 && layer_stride % 2 != 0))) return false;
+    if (num_layers > 1 && fp8 && scale_layer_stride < scales) return false;
+    kv.k = static_cast<char*>(k_cache);
+    kv.v = static_cast<char*>(v_cache);
+    kv.k_scale = k_scale;
+    kv.v_scale = v_scale;
+    kv.layer_stride = num_layers > 1 ? layer_stride : 0;
+    kv.scale_layer_stride = num_layers > 1 ? scale_layer_stride : 0;
+    kv.layers = num_layers;
+    kv.blocks = num_blocks;
+    kv.heads = n_kv_heads;
+    kv.block_size = cache_block_size;
+    kv.token_bytes = token;
+    return true;
+}
+
+// Tables and counts alone, without the caches that they speak of.
+bool kv_pool_of(int num_blocks, int cache_block_size, KvLayers& kv) {
+    if (num_blocks <= 0 || cache_block_size <= 0 ||
+        !fits_int(static_cast<int64_t>(num_blocks) * cache_block_size))
+        return false;
+    kv.blocks = num_blocks;
+    kv.block_size = cache_block_size;
+    return true;
+}
+
 }  // namespace
 
 namespace ccinfer::hipk {
@@ -298,12 +363,7 @@ int ccinfer_qkv_prologue(const void* qkv, const void* q_norm_weight, const void*
         rope_cache_max_position <= 0)
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (head_dim <= 0 || head_dim % 2 != 0 || head_dim > 1024) return CCINFER_ERR_INVALID_ARGUMENT;
-    // eps > 0 (backend.h:84); NaN and inf are tested on the bits, which stays correct when
-    // the compiler is told that NaNs do not occur.
-    uint32_t eps_bits;
-    std::memcpy(&eps_bits, &eps, sizeof eps_bits);
-    if ((eps_bits & 0x7f800000u) == 0x7f800000u || !(eps > 0.0f))
-        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!finite_bits(eps) || !(eps > 0.0f)) return CCINFER_ERR_INVALID_ARGUMENT;
     const int64_t rows = static_cast<int64_t>(num_tokens) * (num_q_heads + num_kv_heads);
     if (!fits_int(rows) ||
         !fits_int(static_cast<int64_t>(num_q_heads + 2 * static_cast<int64_t>(num_kv_heads)) *
@@ -618,6 +678,228 @@ int ccinfer_prefill_attention_fp8_overlap(
                              cache_block_size, workspace, workspace_bytes, stream, &ov);
 }
 
+int ccinfer_rope_frequencies(int rotary_dim, double theta, int scaling, const double* params,
+                             double* frequencies, double* magnitude) {
+    if (!frequencies || !magnitude) return CCINFER_ERR_INVALID_ARGUMENT;
+    return rope_frequencies(rotary_dim, theta, scaling, params, frequencies, magnitude)
+               ? CCINFER_OK
+               : CCINFER_ERR_INVALID_ARGUMENT;
+}
+
+int ccinfer_build_rope_cache(const double* frequencies, int rotary_dim, double magnitude,
+                             int first_position, int num_positions, void* rope_cache,
+                             void* stream) {
+    if (!frequencies || !rope_cache) return CCINFER_ERR_INVALID_ARGUMENT;
+    if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim / 2 > kRopeMaxPairs ||
+        first_position < 0 || num_positions <= 0 ||
+        !fits_int(static_cast<int64_t>(first_position) + num_positions))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!finite_bits(static_cast<float>(magnitude))) return CCINFER_ERR_INVALID_ARGUMENT;
+    for (int p = 0; p < rotary_dim / 2; ++p)
+        if (!finite_bits(frequencies[p])) return CCINFER_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(rope_cache) % 8 != 0) return CCINFER_ERR_INVALID_ARGUMENT;
+    return map_hip_error(build_rope_cache(frequencies, rotary_dim / 2, magnitude, first_position,
+                                          num_positions, rope_cache, as_stream(stream)));
+}
+
+int ccinfer_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                             const int32_t* positions, const void* rope_cache, void* q_out,
+                             int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                             int64_t k_out_token_stride, int64_t k_out_head_stride,
+                             int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                             int rotary_dim, int rope_cache_max_position, int interleaved,
+                             int inverse, void* stream) {
+    if (!q || !q_out || !positions || !rope_cache || (k == nullptr) != (k_out == nullptr))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_q_heads <= 0 || num_kv_heads < 0 || (k == nullptr) != (num_kv_heads == 0))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    const int64_t heads = static_cast<int64_t>(num_q_heads) + num_kv_heads;
+    if (!fits_int(heads) || !rotary_shape_ok(num_tokens, static_cast<int>(heads), head_dim,
+                                             rotary_dim, rope_cache_max_position))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(rope_cache) % 8 != 0) return CCINFER_ERR_INVALID_ARGUMENT;
+    RotaryArgs a;
+    a.sec[0].src = static_cast<const __bf16*>(q);
+    a.sec[0].src_t = q_token_stride;
+    a.sec[0].src_h = q_head_stride;
+    a.sec[0].dst = q_out;
+    a.sec[0].dst_t = q_out_token_stride;
+    a.sec[0].dst_h = q_out_head_stride;
+    a.sec[0].heads = num_q_heads;
+    a.sec[0].rotate = true;
+    a.sec[1].src = static_cast<const __bf16*>(k);
+    a.sec[1].src_t = k_token_stride;
+    a.sec[1].src_h = k_head_stride;
+    a.sec[1].dst = k_out;
+    a.sec[1].dst_t = k_out_token_stride;
+    a.sec[1].dst_h = k_out_head_stride;
+    a.sec[1].heads = num_kv_heads;
+    a.sec[1].rotate = true;
+    a.positions = positions;
+    a.rope_cache = static_cast<const float2*>(rope_cache);
+    a.tokens = num_tokens;
+    a.head_dim = head_dim;
+    a.rotary_dim = rotary_dim;
+    a.rope_max = rope_cache_max_position;
+    a.sin_sign = inverse != 0 ? -1.0f : 1.0f;
+    return map_hip_error(rotary_rows(a, interleaved != 0, false, as_stream(stream)));
+}
+
+int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void* q_norm_weight,
+                          int q_norm_per_head, const void* k_norm_weight, int k_norm_per_head,
+                          const int32_t* positions, const void* rope_cache,
+                          const int32_t* slot_mapping, void* q_out, void* k_cache, void* v_cache,
+                          float* k_scale, float* v_scale, int num_tokens, int num_q_heads,
+                          int num_kv_heads, int head_dim, int rotary_dim,
+                          int rope_cache_max_position, int max_slots, int interleaved, float eps,
+                          float weight_offset, void* stream) {
+    if (!qkv || !positions || !rope_cache || !slot_mapping || !q_out || !k_cache || !v_cache ||
+        (k_scale == nullptr) != (v_scale == nullptr))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_q_heads <= 0 || num_kv_heads <= 0 || max_slots <= 0)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    const int64_t heads = num_q_heads + 2 * static_cast<int64_t>(num_kv_heads);
+    if (!fits_int(heads) ||
+        !rotary_shape_ok(num_tokens, static_cast<int>(heads), head_dim, rotary_dim,
+                         rope_cache_max_position) ||
+        !fits_int(heads * head_dim) || qkv_token_stride < heads * head_dim)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!finite_bits(eps) || !(eps > 0.0f) || !finite_bits(weight_offset))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(rope_cache) % 8 != 0) return CCINFER_ERR_INVALID_ARGUMENT;
+    const bool fp8 = k_scale != nullptr;
+    RotaryArgs a;
+    const int first[3] = {0, num_q_heads, num_q_heads + num_kv_heads};
+    for (int s = 0; s < 3; ++s) {
+        RotarySection& c = a.sec[s];
+        c.src = static_cast<const __bf16*>(qkv) + static_cast<int64_t>(first[s]) * head_dim;
+        c.src_t = qkv_token_stride;
+        c.src_h = head_dim;
+        c.heads = s == 0 ? num_q_heads : num_kv_heads;
+        c.dst = s == 0 ? q_out : (s == 1 ? k_cache : v_cache);
+        c.dst_t = static_cast<int64_t>(c.heads) * head_dim;
+        c.dst_h = head_dim;
+        c.rotate = s < 2;
+        c.to_cache = s > 0;
+        c.scale = s == 1 ? k_scale : (s == 2 ? v_scale : nullptr);
+        const void* w = s == 0 ? q_norm_weight : (s == 1 ? k_norm_weight : nullptr);
+        c.weight = static_cast<const __bf16*>(w);
+        c.weight_h = (s == 0 ? q_norm_per_head : k_norm_per_head) != 0 ? head_dim : 0;
+        c.norm = w != nullptr;
+    }
+    a.positions = positions;
+    a.rope_cache = static_cast<const float2*>(rope_cache);
+    a.slot_mapping = slot_mapping;
+    a.tokens = num_tokens;
+    a.head_dim = head_dim;
+    a.rotary_dim = rotary_dim;
+    a.rope_max = rope_cache_max_position;
+    a.max_slots = max_slots;
+    a.eps = eps;
+    a.weight_offset = weight_offset;
+    return map_hip_error(rotary_rows(a, interleaved != 0, fp8, as_stream(stream)));
+}
+
+int ccinfer_copy_kv_blocks(void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                           const int32_t* src_blocks, const int32_t* dst_blocks, int num_pairs,
+                           int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                           int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
+                           int32_t* status, void* stream) {
+    KvLayers kv;
+    if (!kv_layers_of(k_cache, v_cache, k_scale, v_scale, num_layers, layer_stride,
+                      scale_layer_stride, num_blocks, n_kv_heads, head_dim, cache_block_size, kv))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_pairs < 0 || (num_pairs > 0 && (!src_blocks || !dst_blocks)))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_pairs > kPagesMaxBlocks - 1) return CCINFER_ERR_UNSUPPORTED;
+    if (num_pairs == 0) return CCINFER_OK;
+    return map_hip_error(
+        copy_kv_blocks(kv, src_blocks, dst_blocks, num_pairs, status, as_stream(stream)));
+}
+
+size_t ccinfer_update_tables_workspace_size(int num_items, int max_blocks_per_req,
+                                            int num_blocks) {
+    if (num_items < 0 || max_blocks_per_req <= 0 || num_blocks <= 0 ||
+        num_blocks > kPagesMaxBlocks || num_items > kPagesMaxItems ||
+        !fits_int(static_cast<int64_t>(num_items) * max_blocks_per_req))
+        return 0;
+    return update_tables_workspace_bytes(num_items, max_blocks_per_req, num_blocks);
+}
+
+int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int32_t* ref_counts,
+                                const int32_t* dst_rows, const int32_t* src_rows,
+                                const int32_t* lengths, int num_items, int num_rows,
+                                int max_blocks_per_req, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, int num_layers,
+                                int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                                int n_kv_heads, int head_dim, int cache_block_size,
+                                int32_t* status, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+    KvLayers kv;
+    const bool bare = !k_cache && !v_cache && !k_scale && !v_scale && num_layers == 0;
+    if (!(bare ? kv_pool_of(num_blocks, cache_block_size, kv)
+               : kv_layers_of(k_cache, v_cache, k_scale, v_scale, num_layers, layer_stride,
+                              scale_layer_stride, num_blocks, n_kv_heads, head_dim,
+                              cache_block_size, kv)))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!block_table || !context_lens || !ref_counts || !status || num_items < 0 ||
+        num_rows <= 0 || max_blocks_per_req <= 0)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_items > 0 && !dst_rows) return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!fits_int(static_cast<int64_t>(num_rows) * max_blocks_per_req) ||
+        !fits_int(static_cast<int64_t>(num_items) * max_blocks_per_req) ||
+        !fits_int(static_cast<int64_t>(max_blocks_per_req) * cache_block_size))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_blocks > kPagesMaxBlocks || num_items > kPagesMaxItems)
+        return CCINFER_ERR_UNSUPPORTED;
+    const size_t need = update_tables_workspace_bytes(num_items, max_blocks_per_req, num_blocks);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    TableUpdate u;
+    u.table = block_table;
+    u.ctx = context_lens;
+    u.refs = ref_counts;
+    u.rows = num_rows;
+    u.width = max_blocks_per_req;
+    u.dst = dst_rows;
+    u.src = src_rows;
+    u.lengths = lengths;
+    u.items = num_items;
+    u.status = status;
+    return map_hip_error(update_block_tables(u, kv, workspace, as_stream(stream)));
+}
+
+size_t ccinfer_compact_workspace_size(int num_blocks) {
+    if (num_blocks <= 0 || num_blocks > kPagesMaxBlocks) return 0;
+    return compact_workspace_bytes(num_blocks);
+}
+
+int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_counts, int num_rows,
+                              int max_blocks_per_req, void* k_cache, void* v_cache,
+                              float* k_scale, float* v_scale, int num_layers,
+                              int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                              int n_kv_heads, int head_dim, int cache_block_size,
+                              int32_t* block_table_out, int32_t* ref_counts_out, int32_t* remap,
+                              int32_t* num_live, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    KvLayers kv;
+    if (!kv_layers_of(k_cache, v_cache, k_scale, v_scale, num_layers, layer_stride,
+                      scale_layer_stride, num_blocks, n_kv_heads, head_dim, cache_block_size, kv))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!ref_counts || !ref_counts_out || !remap || !num_live || num_rows < 0)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_rows > 0 && (!block_table || !block_table_out || max_blocks_per_req <= 0))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (num_blocks > kPagesMaxBlocks) return CCINFER_ERR_UNSUPPORTED;
+    const size_t need = compact_workspace_bytes(num_blocks);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    return map_hip_error(compact_kv_blocks(
+        block_table, ref_counts, static_cast<int64_t>(num_rows) * max_blocks_per_req, kv,
+        block_table_out, ref_counts_out, remap, num_live, workspace, as_stream(stream)));
+}
+
 const char* ccinfer_error_message(int code) {
     switch (code) {
         case CCINFER_OK: return "ok";
@@ -626,6 +908,8 @@ const char* ccinfer_error_message(int code) {
         case CCINFER_ERR_DEVICE_INVALID_VALUE: return "device invalid value";
         case CCINFER_ERR_DEVICE_RUNTIME: return "device runtime error";
         case CCINFER_ERR_INVALID_ARGUMENT: return "invalid argument";
+        case CCINFER_ERR_KV_EXHAUSTED: return "cache blocks exhausted";
+        case CCINFER_ERR_KV_INVALID_TABLE: return "invalid block table";
         case CCINFER_ERR_UNSUPPORTED: return "unsupported operation";
         case CCINFER_ERR_INTERNAL: return "internal error";
         default: return "unknown error";

@@ -229,4 +229,87 @@ hipError_t scatter_rows(const void* src, void* dst, int64_t elems, hipStream_t s
 hipError_t expand_block_table(const int32_t* block_table, int32_t* out, int rows,
                               int max_blocks_per_req, int k, hipStream_t stream);
 
+// ---- rotary positions ---------------------------------------------------------
+// Frequencies of the pairs of a table, scaled for long contexts (rope_table.hip).
+constexpr int kRopeMaxPairs = 256;
+enum RopeScaling { kRopeNone, kRopeLinear, kRopeNtk, kRopeYarn, kRopeBands, kRopeFactors };
+// Places in the parameters of a scaling; the pairs' own factors follow.
+enum RopeParam { kRopeFactor, kRopeOriginalMax, kRopeFast, kRopeSlow, kRopeMagnitude, kRopeParams };
+
+bool rope_frequencies(int rotary_dim, double theta, int scaling, const double* prm, double* freq,
+                      double* magnitude);
+
+hipError_t build_rope_cache(const double* freq, int pairs, double magnitude, int first, int count,
+                            void* out, hipStream_t stream);
+
+// Rows of one kind (q, k or v heads) of a rotary call. Strides in elements; a row for the
+// cache goes to the token's slot instead of its index.
+struct RotarySection {
+    const __bf16* src = nullptr;
+    int64_t src_t = 0, src_h = 0;
+    void* dst = nullptr;
+    int64_t dst_t = 0, dst_h = 0;
+    const __bf16* weight = nullptr;  // of head h at weight + h * weight_h
+    int64_t weight_h = 0;
+    float* scale = nullptr;  // fp8 cache: the row scales
+    int heads = 0;
+    bool norm = false, rotate = false, to_cache = false;
+};
+
+constexpr int kRotaryMaxHeadDim = 1024;
+
+struct RotaryArgs {
+    RotarySection sec[3];
+    const int32_t* positions = nullptr;
+    const float2* rope_cache = nullptr;
+    const int32_t* slot_mapping = nullptr;
+    int tokens = 0, head_dim = 0, rotary_dim = 0, rope_max = 0, max_slots = 0;
+    float eps = 0.f, weight_offset = 0.f, sin_sign = 1.f;
+};
+
+hipError_t rotary_rows(const RotaryArgs& a, bool interleaved, bool fp8, hipStream_t stream);
+
+// ---- pages of the cache -------------------------------------------------------
+// All layers' K and V blocks, strides in bytes (scales in floats; NULL for a bf16 cache).
+struct KvLayers {
+    char* k = nullptr;
+    char* v = nullptr;
+    float* k_scale = nullptr;
+    float* v_scale = nullptr;
+    int64_t layer_stride = 0, scale_layer_stride = 0;
+    int layers = 0, blocks = 0, heads = 0, block_size = 0;
+    int64_t token_bytes = 0;  // of one token's heads
+    int64_t block_bytes() const { return token_bytes * block_size; }
+};
+
+// Blocks that the bitmap of free blocks covers at most (and one more than a copy's pairs).
+constexpr int kPagesMaxBlocks = 1 << 24;
+// Items of a table update at most (a workgroup each; a launch holds 2^32 work-items).
+constexpr int kPagesMaxItems = 1 << 20;
+
+hipError_t copy_kv_blocks(const KvLayers& kv, const int32_t* src, const int32_t* dst, int pairs,
+                          int32_t* status, hipStream_t stream);
+
+struct TableUpdate {
+    int32_t* table = nullptr;
+    int32_t* ctx = nullptr;
+    int32_t* refs = nullptr;
+    int rows = 0, width = 0;
+    const int32_t* dst = nullptr;
+    const int32_t* src = nullptr;
+    const int32_t* lengths = nullptr;
+    int items = 0;
+    int32_t* status = nullptr;
+};
+
+size_t update_tables_workspace_bytes(int items, int width, int blocks);
+hipError_t update_block_tables(const TableUpdate& u, const KvLayers& kv, void* workspace,
+                               hipStream_t stream);
+
+size_t compact_workspace_bytes(int blocks);
+hipError_t compact_kv_blocks(const int32_t* table, const int32_t* refs, int64_t entries,
+                             const KvLayers& kv, int32_t* table_out, int32_t* refs_out,
+                             int32_t* remap, int32_t* num_live, void* workspace,
+                             hipStream_t stream);
+
 }  // namespace ccinfer::hipk

@@ -78,6 +78,9 @@ def _stream_reader():
 
 _stream = _stream_reader()
 
+# Index of torch's current device, by the call under torch.cuda.current_device() where it is there.
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
 
 class SideStream:
     """A side stream with its fork/join events, for prefill_attention(..., overlap=...): a

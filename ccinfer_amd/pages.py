@@ -1,0 +1,201 @@
+"""Pages of the paged KV cache over the C ABI: blocks copied, block tables changed with counted
+references, the pool compacted, for all layers in one call.
+
+Conventions are those of `ops`: device tensors on the current device, work on torch's current
+stream, nothing synchronised, CcinferError with the reference's codes for what the host can see
+and a device status word for what it cannot (as in build_batch_metadata).
+
+  k_cache, v_cache   one layer [slots, heads, head_dim] or [blocks, block_size, heads, head_dim],
+                     or all layers [layers, blocks, block_size, heads, head_dim] (the layers may
+                     lie apart, each is contiguous); bf16, or uint8 with k_scale / v_scale
+                     (float32, [layers, fp8_scale_numel] beside caches of all layers)
+  block_table        [rows, max_blocks_per_req] int32, -1 padded; context_lens [rows] int32
+  ref_counts         [blocks] int32: owners of each block, 0 = free
+"""
+from __future__ import annotations
+
+from functools import lru_cache
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .ops import _check, _dev_tensor, _require, _stream, _workspace, current_device
+
+KV_EXHAUSTED = 12      # status: not enough free blocks
+KV_INVALID_TABLE = 14  # status: a table row that the pool does not hold
+
+
+def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: str):
+    """The cache arguments of the C ABI: pointers, layers, strides, blocks, heads, head_dim,
+    block_size."""
+    fp8 = k_scale is not None
+    dtype = torch.uint8 if fp8 else torch.bfloat16
+    shape, stride = k_cache.shape, k_cache.stride()
+    _require(k_cache.dtype is dtype and v_cache.dtype is dtype and v_cache.shape == shape
+             and v_cache.stride() == stride and k_cache.get_device() == dev
+             and v_cache.get_device() == dev and fp8 == (v_scale is not None), op)
+    dims = len(shape)
+    layers, layer_stride = 1, 0
+    if dims == 5:
+        layers, nb, bs, h, d = shape
+        layer_stride = stride[0] * (1 if fp8 else 2)
+    elif dims == 4:
+        nb, bs, h, d = shape
+    else:
+        _require(dims == 3 and shape[0] % block_size == 0, op)
+        nb, bs, h, d = shape[0] // block_size, block_size, shape[1], shape[2]
+    inner = (bs * h * d, h * d, d, 1) if dims >= 4 else (h * d, d, 1)
+    _require(bs == block_size and (dims == 5 and stride[1:] == inner or stride == inner), op)
+    ksp = vsp = None
+    scale_stride = 0
+    if fp8:
+        need = nb * h * 16
+        for s in (k_scale, v_scale):
+            _require(s.dtype is torch.float32 and s.get_device() == dev, op)
+            if layers == 1:
+                _require(s.is_contiguous() and s.numel() >= need, op)
+            else:
+                _require(s.dim() == 2 and s.shape[0] == layers and s.shape[1] >= need
+                         and s.stride(1) == 1 and s.stride(0) == k_scale.stride(0), op)
+        scale_stride = k_scale.stride(0) if layers > 1 else 0
+        ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
+    return (k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, layers, layer_stride, scale_stride,
+            nb, h, d, block_size)
+
+
+def _indices(dev: int, op: str, *tensors) -> None:
+    for t in tensors:
+        _dev_tensor(t, torch.int32, op)
+        _require(t.get_device() == dev, op)
+
+
+def _status_word(status: Optional[torch.Tensor], dev: int, op: str) -> None:
+    _indices(dev, op, status)
+    _require(status.numel() == 1, op)
+
+
+def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: torch.Tensor,
+                   dst_blocks: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                   v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
+                   status: Optional[torch.Tensor] = None) -> None:
+    """Block dst_blocks[i] of every layer becomes a copy of src_blocks[i] (int32 [n]; K, V and
+    the scales of an fp8 cache). Pairs with a block outside the pool (-1, say) are skipped, as
+    are pairs that depend on an order: a destination that is another pair's destination with
+    another source, or another pair's source. `status` (int32 [1]), if given, becomes 6 then
+    and is left alone otherwise."""
+    op = "copy_kv_blocks"
+    dev = current_device()
+    _indices(dev, op, src_blocks, dst_blocks)
+    n = src_blocks.numel()
+    _require(dst_blocks.numel() == n, op)
+    if status is not None:
+        _status_word(status, dev, op)
+    kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
+        k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+    _check(_lib.load().ccinfer_copy_kv_blocks(
+        kp, vp, ksp, vsp, src_blocks.data_ptr() or None, dst_blocks.data_ptr() or None, n, layers,
+        ls, ss, nb, h, d, bs, None if status is None else status.data_ptr(), _stream()), op)
+
+
+@lru_cache(maxsize=1024)
+def update_tables_workspace_size(num_items: int, max_blocks_per_req: int, num_blocks: int) -> int:
+    return int(_lib.load().ccinfer_update_tables_workspace_size(num_items, max_blocks_per_req,
+                                                                num_blocks))
+
+
+def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
+                        ref_counts: torch.Tensor, dst_rows: torch.Tensor,
+                        src_rows: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+                        k_cache: Optional[torch.Tensor] = None,
+                        v_cache: Optional[torch.Tensor] = None,
+                        k_scale: Optional[torch.Tensor] = None,
+                        v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
+                        workspace: Optional[torch.Tensor] = None,
+                        status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Makes row dst_rows[i] hold the first min(lengths[i], source's context) tokens of row
+    src_rows[i] as it was before the call, then blocks for the tokens up to lengths[i]; changes
+    block_table, context_lens and ref_counts in place. src_rows None: of the row itself, an
+    entry -1: of none; lengths None or an entry -1: the source's context.
+
+    So one call forks (child, parent, -1), admits (row, -1, tokens), grows and truncates
+    (row, row, tokens), releases (row, -1, 0) and reorders beams (row, beam it continues, -1),
+    any of them for different rows at once. Whole blocks are shared and counted; a last block
+    filled in part, where it would be shared, is copied to one of the row's own. New blocks are
+    the lowest-numbered that were free before the call, in item order; blocks it releases are
+    free after it. Returns `status` (int32 [1]): 0, or, with nothing changed, 6 (a row or length
+    out of range, a row twice in dst_rows, a copy needed but no caches given), 14 (a row with a
+    context or blocks that the pool does not hold) or 12 (not enough free blocks)."""
+    op = "update_block_tables"
+    dev = current_device()
+    _indices(dev, op, block_table, context_lens, ref_counts, dst_rows)
+    _require(block_table.dim() == 2 and context_lens.numel() == block_table.shape[0], op)
+    rows, width = block_table.shape
+    n, nb = dst_rows.numel(), ref_counts.numel()
+    for t in (src_rows, lengths):
+        if t is not None:
+            _indices(dev, op, t)
+            _require(t.numel() == n, op)
+    if status is None:
+        status = torch.empty(1, dtype=torch.int32, device=block_table.device)
+    else:
+        _status_word(status, dev, op)
+    if k_cache is None:
+        _require(v_cache is None and k_scale is None and v_scale is None, op)
+        kp = vp = ksp = vsp = None
+        layers = ls = ss = h = d = 0
+        bs = cache_block_size
+    else:
+        _require(v_cache is not None, op)
+        kp, vp, ksp, vsp, layers, ls, ss, cache_blocks, h, d, bs = _layers(
+            k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+        _require(cache_blocks == nb, op)
+    ws, ws_bytes = _workspace(update_tables_workspace_size(n, width, nb), block_table.device,
+                              workspace)
+    _check(_lib.load().ccinfer_update_block_tables(
+        block_table.data_ptr(), context_lens.data_ptr(), ref_counts.data_ptr(),
+        dst_rows.data_ptr() or None, None if src_rows is None else src_rows.data_ptr() or None,
+        None if lengths is None else lengths.data_ptr() or None, n, rows, width, kp, vp, ksp, vsp,
+        layers, ls, ss, nb, h, d, bs, status.data_ptr(), None if ws is None else ws.data_ptr(),
+        ws_bytes, _stream()), op)
+    return status
+
+
+@lru_cache(maxsize=1024)
+def compact_workspace_size(num_blocks: int) -> int:
+    return int(_lib.load().ccinfer_compact_workspace_size(num_blocks))
+
+
+def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                      v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
+                      workspace: Optional[torch.Tensor] = None,
+                      out: Optional[dict] = None) -> dict:
+    """Moves the live blocks (count > 0) to the front of the pool, the ones past it, lowest first,
+    into the free blocks, lowest first; returns int32 device tensors block_table and ref_counts
+    with the new numbers, remap [blocks] (each block's new number, -1 for a free one) and
+    num_live [1]. Table entries of free blocks become -1, negative ones stay. `out` reuses
+    tensors of an earlier call; its block_table and ref_counts may be the inputs."""
+    op = "compact_kv_blocks"
+    dev = current_device()
+    _indices(dev, op, block_table, ref_counts)
+    _require(block_table.dim() == 2, op)
+    kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
+        k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+    _require(ref_counts.numel() == nb, op)
+    if out is None:
+        out = {"block_table": torch.empty_like(block_table),
+               "ref_counts": torch.empty_like(ref_counts), "remap": torch.empty_like(ref_counts),
+               "num_live": torch.empty(1, dtype=torch.int32, device=block_table.device)}
+    table, refs, remap, live = (out["block_table"], out["ref_counts"], out["remap"],
+                                out["num_live"])
+    _indices(dev, op, table, refs, remap, live)
+    _require(table.shape == block_table.shape and refs.numel() == nb and remap.numel() == nb
+             and live.numel() == 1, op)
+    ws, ws_bytes = _workspace(compact_workspace_size(nb), block_table.device, workspace)
+    rows, width = block_table.shape
+    _check(_lib.load().ccinfer_compact_kv_blocks(
+        block_table.data_ptr() or None, ref_counts.data_ptr(), rows, width, kp, vp, ksp, vsp,
+        layers, ls, ss, nb, h, d, bs, table.data_ptr() or None, refs.data_ptr(), remap.data_ptr(),
+        live.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _stream()), op)
+    return out

@@ -56,6 +56,8 @@ enum ccinfer_status {
     CCINFER_ERR_DEVICE_INVALID_VALUE = 3,  /* ErrorCode::CudaInvalidValue  */
     CCINFER_ERR_DEVICE_RUNTIME = 4,        /* ErrorCode::CudaRuntimeError  */
     CCINFER_ERR_INVALID_ARGUMENT = 6,      /* ErrorCode::InvalidArgument   */
+    CCINFER_ERR_KV_EXHAUSTED = 12,         /* ErrorCode::KVBlockExhausted  */
+    CCINFER_ERR_KV_INVALID_TABLE = 14,     /* ErrorCode::KVInvalidBlockTable */
     CCINFER_ERR_UNSUPPORTED = 26,          /* ErrorCode::Unsupported       */
     CCINFER_ERR_INTERNAL = 27              /* ErrorCode::InternalError     */
 };
@@ -305,6 +307,141 @@ int ccinfer_prefill_attention_fp8_overlap(
     int max_blocks_per_req, int num_q_heads, int num_kv_heads, int head_dim,
     int cache_block_size, void* workspace, size_t workspace_bytes, void* stream,
     void* side_stream, void* fork_event, void* join_event);
+
+/* ---- rotary positions ---------------------------------------------------------------
+ * How the frequencies of a table are scaled for contexts past the trained length. `params`
+ * is an array on the host: [0] factor, [1] the original number of positions, [2] and [3] the
+ * fast and slow bounds in turns over that length, [4] the factor m of cos and sin (0: the
+ * scaling's own), and for CCINFER_ROPE_FACTORS the pairs' own divisors from [5] on. */
+enum ccinfer_rope_scaling {
+    CCINFER_ROPE_NONE = 0,    /* f_p = theta^(-2p / rotary_dim); params unused             */
+    CCINFER_ROPE_LINEAR = 1,  /* f_p / factor                                              */
+    CCINFER_ROPE_NTK = 2,     /* theta * factor^(rotary_dim / (rotary_dim - 2))            */
+    CCINFER_ROPE_YARN = 3,    /* a ramp over the pairs from f_p to f_p / factor, between the
+                                 pairs that make `fast` and `slow` turns; m = 0.1 ln factor + 1 */
+    CCINFER_ROPE_BANDS = 4,   /* f_p where a pair makes `fast` turns or more, f_p / factor at
+                                 `slow` or fewer, blended linearly in the turns between    */
+    CCINFER_ROPE_FACTORS = 5  /* f_p / params[5 + p]                                       */
+};
+
+/* Frequencies of the rotary_dim / 2 pairs (radians a position) and m, on the host in double
+ * precision; touches no device. rotary_dim even and at most 512, theta > 1, factor >= 1,
+ * fast > slow > 0. */
+int ccinfer_rope_frequencies(int rotary_dim, double theta, int scaling, const double* params,
+                             double* frequencies, double* magnitude);
+
+/* rope_cache[i][p] = m (cos, sin)((first_position + i) f_p), float [num_positions]
+ * [rotary_dim / 2][2], the table that the calls below and ccinfer_qkv_prologue read (the
+ * reference fills one on the host, src/model/rope/rope_cache.cpp). `frequencies` is a host
+ * array that the call has read when it returns; angles are reduced in double precision, so
+ * a value is within 2 ulp of m at any position. May be captured into a graph. */
+int ccinfer_build_rope_cache(const double* frequencies, int rotary_dim, double magnitude,
+                             int first_position, int num_positions, void* rope_cache,
+                             void* stream);
+
+/* Rotates every head of q [num_tokens][num_q_heads][head_dim] and k (NULL with num_kv_heads
+ * 0: none) bf16 by table row positions[t] (launch_rope, src/kernel/pos/rope.cu:14-43, whose
+ * rotary_dim is head_dim and whose pairs are p, p + rotary_dim / 2). interleaved: the pairs
+ * are 2p, 2p + 1. Elements from rotary_dim on, and rows whose position is outside
+ * [0, rope_cache_max_position), are copied. inverse: the opposite angle (the gradient's
+ * direction). Strides in elements; a head's elements are contiguous. q_out / k_out may be
+ * q / k themselves (same pointer and strides), or memory apart from them. Float32 inside,
+ * rounded once. head_dim even, at most 1024. */
+int ccinfer_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                             const int32_t* positions, const void* rope_cache, void* q_out,
+                             int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                             int64_t k_out_token_stride, int64_t k_out_head_stride,
+                             int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                             int rotary_dim, int rope_cache_max_position, int interleaved,
+                             int inverse, void* stream);
+
+/* ccinfer_qkv_prologue with float32 inside and one rounding at the end, for models and caches
+ * that it does not take: y = x rsqrt(mean x^2 + eps) (w + weight_offset) of each q and k head
+ * (a NULL weight: no norm for that side; *_per_head: the weights are [heads][head_dim], else
+ * [head_dim]), the rotation of ccinfer_rotary_embedding, q to q_out [num_tokens]
+ * [num_q_heads][head_dim], K and V to their slots of a bf16 cache, or, with k_scale and
+ * v_scale, of an fp8 cache (layout and quantisation of ccinfer_write_kv_cache_fp8, straight
+ * from the float32 rows; a NaN is stored as E4M3's). qkv rows lie qkv_token_stride elements
+ * apart. Tokens whose slot is outside [0, max_slots) write no K/V; no two tokens may have the
+ * same slot. */
+int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void* q_norm_weight,
+                          int q_norm_per_head, const void* k_norm_weight, int k_norm_per_head,
+                          const int32_t* positions, const void* rope_cache,
+                          const int32_t* slot_mapping, void* q_out, void* k_cache, void* v_cache,
+                          float* k_scale, float* v_scale, int num_tokens, int num_q_heads,
+                          int num_kv_heads, int head_dim, int rotary_dim,
+                          int rope_cache_max_position, int max_slots, int interleaved, float eps,
+                          float weight_offset, void* stream);
+
+/* ---- pages of the cache ---------------------------------------------------------------
+ * Operators on the pool of blocks of all layers at once. k_cache / v_cache: layer 0 of
+ * [num_layers][num_blocks][cache_block_size][n_kv_heads][head_dim], bf16, or fp8 bytes with
+ * k_scale / v_scale; layer_stride in bytes and scale_layer_stride in floats lead from one
+ * layer to the next (unused for one layer). An fp8 cache has cache_block_size 16.
+ *
+ * ref_counts [num_blocks] says how many table rows (or other owners, a prefix cache say) hold
+ * a block; 0 is free. At most 2^24 blocks (CCINFER_ERR_UNSUPPORTED past that) for the calls
+ * that take counts. */
+
+/* Block dst_blocks[i] becomes a copy of src_blocks[i] in every layer, K, V and scales. Pairs
+ * with a block outside [0, num_blocks), and of a block with itself, are skipped. Pairs that
+ * depend on an order (a destination that is another pair's destination with another source,
+ * or another pair's source) are skipped too, and *status, if not NULL, is set to
+ * CCINFER_ERR_INVALID_ARGUMENT; it is not written otherwise. */
+int ccinfer_copy_kv_blocks(void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                           const int32_t* src_blocks, const int32_t* dst_blocks, int num_pairs,
+                           int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                           int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
+                           int32_t* status, void* stream);
+
+/* Workspace bytes of ccinfer_update_block_tables (0 for an invalid shape). */
+size_t ccinfer_update_tables_workspace_size(int num_items, int max_blocks_per_req,
+                                            int num_blocks);
+
+/* Changes rows of block_table [num_rows][max_blocks_per_req] (-1 padded) and context_lens
+ * [num_rows], and the counts with them. Item i makes row dst_rows[i] hold the first
+ * min(lengths[i], context of src_rows[i]) tokens of row src_rows[i] as it was before the call
+ * (-1: of none; src_rows NULL: of the row itself), followed by blocks for the tokens up to
+ * lengths[i] (-1, or lengths NULL: the source's context):
+ *   fork      (child, parent, -1)         admit    (row, -1, tokens)
+ *   grow      (row, row, more tokens)     truncate (row, row, fewer tokens)
+ *   release   (row, -1, 0)                beams    (row, the beam it goes on from, -1)
+ * Whole blocks are shared. A last block that is filled in part has one owner: where it would
+ * be shared, its tokens are copied to a block of the row's own. New blocks are the
+ * lowest-numbered ones that were free before the call, in item order; what the call releases
+ * is free after it. *status (on the device, always written): CCINFER_OK, or, with nothing
+ * changed, CCINFER_ERR_INVALID_ARGUMENT (a row or length out of range, two items of one row,
+ * a copy needed but no caches given), CCINFER_ERR_KV_INVALID_TABLE (a context outside the
+ * row, a block outside the pool or with count 0 among those held), or
+ * CCINFER_ERR_KV_EXHAUSTED. Caches NULL with num_layers 0: tables and counts alone. */
+int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int32_t* ref_counts,
+                                const int32_t* dst_rows, const int32_t* src_rows,
+                                const int32_t* lengths, int num_items, int num_rows,
+                                int max_blocks_per_req, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, int num_layers,
+                                int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                                int n_kv_heads, int head_dim, int cache_block_size,
+                                int32_t* status, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Workspace bytes of ccinfer_compact_kv_blocks (0 for an invalid shape). */
+size_t ccinfer_compact_workspace_size(int num_blocks);
+
+/* Moves the live blocks (count > 0) into blocks [0, *num_live): those that lie past it, lowest
+ * first, to the free blocks below it, lowest first; the others stay. Writes the tables with the
+ * new numbers (entries of free blocks and past the pool become -1, negative ones stay), the
+ * counts, and remap [num_blocks]: each block's new number, -1 for a free one. The outputs may
+ * be the inputs (block_table_out = block_table, ref_counts_out = ref_counts). num_rows 0: no
+ * tables. */
+int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_counts, int num_rows,
+                              int max_blocks_per_req, void* k_cache, void* v_cache,
+                              float* k_scale, float* v_scale, int num_layers,
+                              int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                              int n_kv_heads, int head_dim, int cache_block_size,
+                              int32_t* block_table_out, int32_t* ref_counts_out, int32_t* remap,
+                              int32_t* num_live, void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 /* Human-readable text for a status code (the reference's error_message()). */
 const char* ccinfer_error_message(int code);

@@ -1,0 +1,394 @@
+"""Copy, table update and compaction of the paged cache on the GPU, against the same done block by
+block (tests/_pages_ref.py): every number and every byte equal."""
+import numpy as np
+import pytest
+import torch
+
+import ccinfer_amd as cc
+from tests import _pages_ref as P
+from tests._util import say
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(a, dev):
+    return torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)
+
+
+class Pool:
+    """Caches of all layers as random bits; `apart`: the layers lie apart and start off a 16-byte
+    boundary (bf16)."""
+
+    def __init__(self, dev, seed, layers, blocks, h, d, bs=16, fp8=False, apart=False):
+        rng = np.random.default_rng(seed)
+        self.fp8, self.bs, self.blocks, self.layers = fp8, bs, blocks, layers
+        shape = (layers, blocks, bs, h, d)
+        n = blocks * bs * h * d
+        self.t = []
+        for _ in range(2):
+            a = torch.from_numpy(rng.integers(0, 256, shape).astype(np.uint8)).to(dev)
+            if not fp8:
+                a = torch.from_numpy(rng.integers(-2 ** 15, 2 ** 15, shape).astype(np.int16)) \
+                    .to(dev).view(torch.bfloat16)
+            if apart:
+                buf = torch.zeros(layers * (n + 9) + 1, dtype=a.dtype, device=dev)
+                v = torch.as_strided(buf, shape, (n + 9, bs * h * d, h * d, d, 1), 1)
+                v.copy_(a)
+                a = v
+            self.t.append(a)
+        self.s = [torch.from_numpy(rng.standard_normal((layers, blocks * h * 16))
+                                   .astype(np.float32)).to(dev) for _ in range(2)] if fp8 else [None, None]
+        self.kw = dict(k_scale=self.s[0], v_scale=self.s[1], cache_block_size=bs)
+        self.h = h
+
+    def caches(self):
+        return [x.contiguous().view(torch.uint8 if self.fp8 else torch.int16).cpu().numpy()
+                .reshape(self.layers, self.blocks, self.bs, -1) for x in self.t]
+
+    def scales(self):
+        return [x.cpu().numpy().reshape(self.layers, self.blocks, self.h, 16) for x in self.s] \
+            if self.fp8 else []
+
+    def flat(self):
+        return self.caches() + [x.reshape(self.layers, self.blocks, -1) for x in self.scales()]
+
+
+POOLS = [dict(layers=1, blocks=20, h=2, d=64), dict(layers=3, blocks=33, h=1, d=128, fp8=True),
+         dict(layers=2, blocks=17, h=3, d=40, apart=True), dict(layers=5, blocks=50, h=8, d=128),
+         dict(layers=2, blocks=40, h=1, d=6, bs=5), dict(layers=1, blocks=9, h=1, d=64, fp8=True),
+         dict(layers=2, blocks=12, h=1, d=8, bs=1)]
+
+
+# ---- copy ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_copy(gpu, pool):
+    say(f"copy {pool}")
+    p = Pool(gpu, 1, **pool)
+    rng = np.random.default_rng(5)
+    for n in (1, 2, p.blocks // 2):
+        order = rng.permutation(p.blocks)
+        dst, src = order[:n].copy(), rng.choice(order[n:], n)
+        status = torch.full((1,), 77, dtype=torch.int32, device=gpu)
+        want, _ = P.copy(p.flat(), src, dst, p.blocks)
+        cc.copy_kv_blocks(*p.t, i32(src, gpu), i32(dst, gpu), status=status, **p.kw)
+        assert all(np.array_equal(a, b) for a, b in zip(p.flat(), want))
+        assert status.item() == 77  # left alone
+
+
+def test_copy_one_layer_shapes(gpu):
+    say("copy one layer")
+    p = Pool(gpu, 2, 1, 10, 2, 64)
+    want, _ = P.copy(p.flat(), [3, 4], [9, 0], 10)
+    k, v = p.t
+    cc.copy_kv_blocks(k[0], v[0], i32([3], gpu), i32([9], gpu))                     # 4 dimensions
+    cc.copy_kv_blocks(k.view(160, 2, 64), v.view(160, 2, 64), i32([4], gpu), i32([0], gpu))
+    assert all(np.array_equal(a, b) for a, b in zip(p.flat(), want))
+    cc.copy_kv_blocks(k, v, i32([], gpu), i32([], gpu))                             # nothing
+    assert all(np.array_equal(a, b) for a, b in zip(p.flat(), want))
+
+
+@pytest.mark.parametrize("pairs", [
+    [(1, 2), (3, 2), (4, 5)],             # one destination, two sources
+    [(1, 2), (2, 3), (4, 5)],             # a chain
+    [(1, 2), (2, 1), (4, 5)],             # a swap
+    [(1, 2), (1, 2), (1, 3), (7, 7), (2, 2)],  # twice the same; blocks on themselves
+    [(-1, 2), (1, -1), (40, 3), (3, 40), (5, 2 ** 31 - 1), (-2 ** 31, 6), (4, 5)],
+    [(0, 9), (9, 9), (1, 8), (8, -1)],
+])
+def test_copy_pairs_that_depend_on_an_order(gpu, pairs):
+    say(f"copy {pairs}")
+    p = Pool(gpu, 3, 2, 40, 1, 64)
+    src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+    want, code = P.copy(p.flat(), src, dst, p.blocks)
+    status = torch.zeros(1, dtype=torch.int32, device=gpu)
+    cc.copy_kv_blocks(*p.t, i32(src, gpu), i32(dst, gpu), status=status)
+    assert all(np.array_equal(a, b) for a, b in zip(p.flat(), want))
+    assert status.item() == code
+
+
+# ---- update ----------------------------------------------------------------------------
+
+class Tables:
+    def __init__(self, dev, rows, width, blocks):
+        self.dev = dev
+        self.t = np.full((rows, width), -1, np.int32)
+        self.c, self.r = np.zeros(rows, np.int32), np.zeros(blocks, np.int32)
+        self.up()
+
+    def up(self):
+        self.dt, self.dc, self.dr = (i32(x, self.dev) for x in (self.t, self.c, self.r))
+
+    def step(self, p, dst, src, lengths, caches=True, **kw):
+        """One update on both sides; returns the status."""
+        dev = lambda x: None if x is None else i32(x, self.dev)  # noqa: E731
+        lists = p.caches(), p.scales()
+        t, c, r, cs, ss, code = P.update(self.t, self.c, self.r, dst, src, lengths, *lists, p.bs,
+                                         have_caches=caches)
+        args = p.t if caches else (None, None)
+        opts = p.kw if caches else dict(cache_block_size=p.bs)
+        status = cc.update_block_tables(self.dt, self.dc, self.dr, i32(dst, self.dev), dev(src),
+                                        dev(lengths), *args, **opts, **kw)
+        assert status.item() == code
+        for got, want in ((self.dt, t), (self.dc, c), (self.dr, r)):
+            assert np.array_equal(got.cpu().numpy(), want)
+        assert all(np.array_equal(a, b) for a, b in zip(p.caches(), cs))
+        assert all(np.array_equal(a, b) for a, b in zip(p.scales(), ss))
+        self.t, self.c, self.r = t, c, r
+        P.consistent(t, c, r, p.bs)
+        return code
+
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_update_random_steps(gpu, pool):
+    say(f"update {pool}")
+    p = Pool(gpu, 7, **{**pool, "blocks": 60})
+    rng = np.random.default_rng(11)
+    rows, width = 7, 9
+    x = Tables(gpu, rows, width, p.blocks)
+    codes = set()
+    for k in range(25):
+        n = int(rng.integers(1, rows + 1))
+        dst = rng.permutation(rows)[:n]
+        kind = rng.integers(0, 4, n)
+        src = np.where(kind == 0, -1, np.where(kind == 1, dst, rng.integers(0, rows, n)))
+        lengths = np.where(rng.random(n) < 0.4, -1, rng.integers(0, width * p.bs + 1, n))
+        if k % 5 == 4:
+            lengths = None
+        codes.add(x.step(p, dst, None if k % 7 == 6 else src, lengths))
+    assert 0 in codes
+
+
+def test_update_each_use(gpu):
+    say("update uses")
+    p = Pool(gpu, 8, 3, 64, 2, 64)
+    x = Tables(gpu, 6, 8, 64)
+    assert x.step(p, [0, 1], [-1, -1], [50, 33]) == 0          # admit
+    assert x.t[0, :4].tolist() == [0, 1, 2, 3] and x.t[1, :3].tolist() == [4, 5, 6]
+    assert x.step(p, [2, 3], [0, 0], None) == 0                # fork: three shared, one own each
+    assert x.t[2].tolist() == [0, 1, 2, 7, -1, -1, -1, -1] and x.r[0] == 3 and x.r[3] == 1
+    assert x.step(p, [0, 2], None, [64, 65]) == 0              # grow: in the block, into a next
+    assert x.step(p, [3], [3], [20]) == 0                      # back into a shared block: copied
+    assert x.t[3, 1] not in (1, -1) and x.r[1] == 2
+    assert x.step(p, [3], [3], [16]) == 0                      # whole blocks stay shared
+    assert x.step(p, [0, 1], [1, 0], None) == 0                # rows change places
+    assert x.c.tolist()[:2] == [33, 64]
+    assert x.step(p, [0, 1, 2, 3], [-1] * 4, [0] * 4) == 0     # release everything
+    assert not x.r.any()
+    assert x.step(p, [], [], []) == 0                          # nothing
+
+
+def test_update_refused_by_the_device_changes_nothing(gpu):
+    say("update refused")
+    p = Pool(gpu, 9, 2, 32, 1, 64)
+    x = Tables(gpu, 5, 8, 32)
+    assert x.step(p, [0, 1], [-1, -1], [40, 17]) == 0
+    for dst, src, lengths, code in [
+            ([2, 2], [0, 1], None, 6), ([5], [0], None, 6), ([-1], [0], None, 6),
+            ([2], [5], None, 6), ([2], [-2], None, 6), ([2], [0], [129], 6), ([2], [0], [-2], 6),
+            ([0, 1, 2, 3, 4], [0, 1, -1, -1, -1], [128] * 5, 12),  # 40 blocks of 32
+            ([2, 0], [0, 7], None, 6)]:
+        assert x.step(p, dst, src, lengths) == code, (dst, src, lengths)
+    assert x.step(p, [2], [0], None, caches=False) == 6        # a copy, and nothing to copy in
+    assert x.step(p, [2], [0], [32], caches=False) == 0        # whole blocks alone need none
+    assert x.step(p, [2], [-1], [0], caches=False) == 0
+    keep = x.t.copy(), x.c.copy(), x.r.copy()
+    for k, change in enumerate([lambda: x.t.__setitem__((0, 1), 32), lambda: x.t.__setitem__((0, 2), -1),
+                                lambda: x.c.__setitem__(0, 129), lambda: x.c.__setitem__(0, -1),
+                                lambda: x.r.__setitem__(x.t[0, 0], 0)]):
+        change()
+        x.up()
+        for dst, src in (([2], [0]), ([0], [-1])):
+            status = cc.update_block_tables(x.dt, x.dc, x.dr, i32(dst, gpu), i32(src, gpu), None,
+                                            *p.t)
+            assert status.item() == 14, k
+            for got, want in ((x.dt, x.t), (x.dc, x.c), (x.dr, x.r)):
+                assert np.array_equal(got.cpu().numpy(), want)
+        x.t, x.c, x.r = (a.copy() for a in keep)
+    x.up()
+    # five blocks are held: the last free one is handed out, then none is left
+    assert x.step(p, [2, 3, 4, 0], [-1, -1, -1, 0], [128, 128, 128, 96]) == 0
+    assert (x.r > 0).all() and x.step(p, [1], [1], [33]) == 12
+    assert x.step(p, [2, 1], [-1, 1], [0, 33]) == 12           # what it releases is free after it
+    assert x.step(p, [2], [-1], [0]) == 0 and x.step(p, [1], [1], [33]) == 0
+
+
+@pytest.mark.parametrize("blocks", [4095, 4096, 4097, 64 * 64 * 5 + 70])
+def test_update_over_many_chunks(gpu, blocks):
+    say(f"update {blocks} blocks")
+    p = Pool(gpu, 10, 1, blocks, 1, 2, bs=2)
+    rng = np.random.default_rng(blocks)
+    rows, width = 6, blocks // 2
+    x = Tables(gpu, rows, width, blocks)
+    # most of the pool held by one row, holes scattered by truncating and forking
+    assert x.step(p, [0, 1], [-1, -1], [blocks - 40, blocks // 2 - 7]) == 0
+    assert x.step(p, [0], [0], [blocks // 2 + 1]) == 0
+    assert x.step(p, [2, 3], [1, 0], None) == 0
+    assert x.step(p, [1], [-1], [0]) == 0
+    held = x.r.copy()
+    assert x.step(p, [4], [-1], [(int((held == 0).sum()) // 2) * 2]) == 0
+    assert x.step(p, [0, 5], [-1, 4], [0, -1]) == 0
+    for _ in range(4):
+        x.step(p, rng.permutation(rows)[:3], rng.integers(-1, rows, 3),
+               rng.integers(0, blocks // 8, 3))
+
+
+def test_update_refusals(gpu):
+    say("update refusals")
+    p = Pool(gpu, 1, 2, 8, 1, 64)
+    x = Tables(gpu, 3, 4, 8)
+    one = i32([0], gpu)
+    ws = torch.empty(64, dtype=torch.uint8, device=gpu)
+
+    def call(table=x.dt, ctx=x.dc, refs=x.dr, dst=one, src=one, lengths=one, k=p.t[0], v=p.t[1],
+             **kw):
+        return cc.update_block_tables(table, ctx, refs, dst, src, lengths, k, v, **kw)
+    call()
+    for i, kw in enumerate([dict(table=x.dt.long()), dict(ctx=x.dc[:2]), dict(refs=x.dr[:7]),
+                            dict(src=x.dc), dict(lengths=x.dc), dict(v=None), dict(k=None),
+                            dict(workspace=ws), dict(status=x.dc), dict(cache_block_size=8),
+                            dict(k_scale=torch.zeros(2, 128, device=gpu)), dict(table=x.dt.t()),
+                            dict(k=p.t[0].float(), v=p.t[1].float()), dict(v=p.t[1][:1])]):
+        with pytest.raises(cc.CcinferError) as e:
+            call(**kw)
+        assert e.value.code == 6, i
+
+
+# ---- compact ---------------------------------------------------------------------------
+
+def compact_both(gpu, p, table, refs, in_place=False):
+    wt, wr, wm, wn, wc = P.compact(table, refs, p.flat())
+    dt, dr = i32(table, gpu), i32(refs, gpu)
+    out = None
+    if in_place:
+        out = {"block_table": dt, "ref_counts": dr, "remap": torch.empty_like(dr),
+               "num_live": torch.empty(1, dtype=torch.int32, device=gpu)}
+    out = cc.compact_kv_blocks(dt, dr, *p.t, **p.kw, out=out)
+    assert out["num_live"].item() == wn
+    for name, want in (("block_table", wt), ("ref_counts", wr), ("remap", wm)):
+        assert np.array_equal(out[name].cpu().numpy(), want), name
+    # every live block's data; what is left behind is free
+    for a, b in zip(p.flat(), wc):
+        assert np.array_equal(a, b)
+    if not in_place:
+        assert np.array_equal(dt.cpu().numpy(), table) and np.array_equal(dr.cpu().numpy(), refs)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("pool", POOLS)
+def test_compact(gpu, pool, in_place):
+    say(f"compact {pool} {in_place}")
+    rng = np.random.default_rng(21)
+    for share in (0.0, 0.2, 0.5, 0.9, 1.0):
+        p = Pool(gpu, 22, **pool)
+        refs = np.where(rng.random(p.blocks) < share, rng.integers(1, 5, p.blocks), 0)
+        table = rng.integers(-3, p.blocks + 4, (4, 6))
+        compact_both(gpu, p, table.astype(np.int32), refs.astype(np.int32), in_place)
+
+
+@pytest.mark.parametrize("blocks,live", [(4096, 4096), (4096, 0), (8192, 4096), (8193, 4097),
+                                         (9000, 4095), (20000, 13000), (70000, 300)])
+def test_compact_over_many_chunks(gpu, blocks, live):
+    say(f"compact {blocks} {live}")
+    rng = np.random.default_rng(blocks + live)
+    p = Pool(gpu, 23, 1, blocks, 1, 2, bs=1)
+    refs = np.zeros(blocks, np.int32)
+    refs[rng.permutation(blocks)[:live]] = rng.integers(1, 9, live)
+    table = rng.integers(-1, blocks, (50, 301)).astype(np.int32)
+    compact_both(gpu, p, table, refs)
+
+
+def test_compact_without_tables(gpu):
+    say("compact no tables")
+    p = Pool(gpu, 24, 2, 30, 1, 64)
+    refs = np.zeros(30, np.int32)
+    refs[[3, 29, 17]] = 1
+    compact_both(gpu, p, np.zeros((0, 5), np.int32), refs)
+
+
+def test_compact_refusals(gpu):
+    say("compact refusals")
+    p = Pool(gpu, 1, 2, 8, 1, 64)
+    t, r = i32(np.zeros((2, 3)), gpu), i32(np.ones(8), gpu)
+    ok = cc.compact_kv_blocks(t, r, *p.t)
+    for i, call in enumerate([
+            lambda: cc.compact_kv_blocks(t, r[:7], *p.t),
+            lambda: cc.compact_kv_blocks(t.long(), r, *p.t),
+            lambda: cc.compact_kv_blocks(t, r, p.t[0], p.t[1][:1]),
+            lambda: cc.compact_kv_blocks(t, r, *p.t, out={**ok, "remap": r[:7]}),
+            lambda: cc.compact_kv_blocks(t, r, *p.t, workspace=t),
+            lambda: cc.compact_kv_blocks(t[0], r, *p.t)]):
+        with pytest.raises(cc.CcinferError) as e:
+            call()
+        assert e.value.code == 6, i
+
+
+# ---- far offsets, graphs ----------------------------------------------------------------
+
+def test_blocks_past_two_and_four_gib(gpu):
+    # one layer's K of 4.5 GiB: byte offsets past 2^32
+    say("pages far offsets")
+    blocks, h, d = 147456, 8, 128
+    k = torch.zeros(blocks, 16, h, d, dtype=torch.bfloat16, device=gpu)
+    v = torch.zeros(blocks, 16, h, d, dtype=torch.bfloat16, device=gpu)
+    far = blocks - 1
+    k[far], v[far], k[70000] = 3.0, 4.0, 5.0
+    cc.copy_kv_blocks(k, v, i32([far, 70000], gpu), i32([far - 1, 2], gpu))
+    assert (k[far - 1] == 3).all() and (v[far - 1] == 4).all() and (k[2] == 5).all()
+    assert not k[far - 2].any() and not k[3].any()
+    refs = torch.zeros(blocks, dtype=torch.int32, device=gpu)
+    refs[far], refs[0], refs[1] = 1, 1, 1
+    table = i32([[0, 1, far]], gpu)
+    out = cc.compact_kv_blocks(table, refs, k, v)
+    assert out["block_table"].tolist() == [[0, 1, 2]] and (k[2] == 3).all() and (v[2] == 4).all()
+    ctx = i32([40, 0], gpu)
+    table = i32([[0, 1, far], [-1, -1, -1]], gpu)
+    refs = torch.ones(blocks, dtype=torch.int32, device=gpu)
+    refs[far - 5] = 0
+    status = cc.update_block_tables(table, ctx, refs, i32([1], gpu), i32([0], gpu), None, k, v)
+    assert status.item() == 0 and table.tolist()[1] == [0, 1, far - 5]
+    assert (k[far - 5, :8] == 3).all() and not k[far - 5, 8:].any()
+
+
+def test_update_and_compact_in_replayed_graphs(gpu):
+    say("pages graph")
+    p, e = (Pool(gpu, 30, 2, 64, 2, 64) for _ in range(2))
+    x, y = Tables(gpu, 8, 6, 64), Tables(gpu, 8, 6, 64)
+    dst, src, n = i32(np.zeros(3), gpu), i32(np.zeros(3), gpu), i32(np.zeros(3), gpu)
+    status = torch.zeros(1, dtype=torch.int32, device=gpu)
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device=gpu)  # both graphs' and the eager calls'
+    out = {"block_table": x.dt, "ref_counts": x.dr, "remap": torch.empty_like(x.dr),
+           "num_live": torch.empty(1, dtype=torch.int32, device=gpu)}
+
+    def update():
+        cc.update_block_tables(x.dt, x.dc, x.dr, dst, src, n, *p.t, workspace=ws, status=status)
+
+    def compact():
+        cc.compact_kv_blocks(x.dt, x.dr, *p.t, workspace=ws, out=out)
+
+    dst.copy_(i32([0, 1, 2], gpu)), src.fill_(-1), n.fill_(0)
+    update()  # (of empty rows)
+    compact()
+    torch.cuda.synchronize()
+    graphs = []
+    for call in (update, compact):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+    rng = np.random.default_rng(31)
+    for k in range(8):
+        a, b, c = rng.permutation(8)[:3], rng.integers(-1, 8, 3), rng.integers(-1, 60, 3)
+        for t, v in ((dst, a), (src, b), (n, c)):
+            t.copy_(i32(v, gpu))
+        graphs[0].replay()
+        want = cc.update_block_tables(y.dt, y.dc, y.dr, i32(a, gpu), i32(b, gpu), i32(c, gpu), *e.t)
+        assert status.item() == want.item()
+        if k % 2:
+            graphs[1].replay()
+            o = cc.compact_kv_blocks(y.dt, y.dr, *e.t)
+            y.dt, y.dr = o["block_table"], o["ref_counts"]
+            assert torch.equal(out["remap"], o["remap"])
+        for u, w in ((x.dt, y.dt), (x.dc, y.dc), (x.dr, y.dr)):
+            assert torch.equal(u, w)
+        assert all(np.array_equal(u, w) for u, w in zip(p.flat(), e.flat()))
+        P.consistent(y.dt.cpu().numpy(), y.dc.cpu().numpy(), y.dr.cpu().numpy(), 16)
