@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <climits>
+#include <cmath>
 #include <cstring>
 #include <algorithm>
 #include <cstdint>
@@ -695,8 +696,10 @@ int ccinfer_build_rope_cache(const double* frequencies, int rotary_dim, double m
         !fits_int(static_cast<int64_t>(first_position) + num_positions))
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (!finite_bits(static_cast<float>(magnitude))) return CCINFER_ERR_INVALID_ARGUMENT;
+    // 2^31 positions at up to 2^16 radians each stay within the angles' 2^51 quarter turns
     for (int p = 0; p < rotary_dim / 2; ++p)
-        if (!finite_bits(frequencies[p])) return CCINFER_ERR_INVALID_ARGUMENT;
+        if (!finite_bits(frequencies[p]) || !(std::abs(frequencies[p]) <= 65536.0))
+            return CCINFER_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(rope_cache) % 8 != 0) return CCINFER_ERR_INVALID_ARGUMENT;
     return map_hip_error(build_rope_cache(frequencies, rotary_dim / 2, magnitude, first_position,
                                           num_positions, rope_cache, as_stream(stream)));
@@ -798,6 +801,7 @@ int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void*
     a.max_slots = max_slots;
     a.eps = eps;
     a.weight_offset = weight_offset;
+    a.per_elem = 1.0f / static_cast<float>(head_dim);
     return map_hip_error(rotary_rows(a, interleaved != 0, fp8, as_stream(stream)));
 }
 

@@ -265,6 +265,7 @@ struct RotaryArgs {
     const int32_t* slot_mapping = nullptr;
     int tokens = 0, head_dim = 0, rotary_dim = 0, rope_max = 0, max_slots = 0;
     float eps = 0.f, weight_offset = 0.f, sin_sign = 1.f;
+    float per_elem = 0.f;  // 1 / head_dim
 };
 
 hipError_t rotary_rows(const RotaryArgs& a, bool interleaved, bool fp8, hipStream_t stream);

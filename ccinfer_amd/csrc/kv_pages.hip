@@ -27,8 +27,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kChunk = 4096;                // blocks whose bitmap one workgroup takes
+constexpr int kChunk = 1024;                // blocks whose bitmap one workgroup takes
 constexpr int kChunkWords = kChunk / kWave;
+constexpr int kWaveWords = kChunkWords / kWaves;
+static_assert(kWaveWords * kWaves == kChunkWords && kChunkWords <= kWave);
 
 constexpr int kOk = 0;
 constexpr int kInvalidArgument = 6;    // ErrorCode::InvalidArgument
@@ -56,7 +58,7 @@ __device__ __forceinline__ void copy_bytes(const char* src, char* dst, int64_t b
             if (i + k * kThreads < n) v[k] = s[i + k * kThreads];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (i + k * kThreads < n) d[i + k * kThreads] = v[k];
+            if (i + k * kThreads < n) __builtin_nontemporal_store(v[k], &d[i + k * kThreads]);
     }
 }
 
@@ -133,13 +135,17 @@ __device__ __forceinline__ void free_bitmap(const int32_t* __restrict__ refs, in
                                             int32_t* __restrict__ counts) {
     __shared__ int wave_count[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int word = wave * kWaveWords;
+    int ref[kWaveWords];
+#pragma unroll
+    for (int k = 0; k < kWaveWords; ++k)
+        ref[k] = refs[min(c * kChunk + (word + k) * kWave + lane, blocks - 1)];
     int count = 0;
 #pragma unroll
-    for (int k = 0; k < kChunkWords / kWaves; ++k) {
-        const int word = wave * (kChunkWords / kWaves) + k;
-        const int b = c * kChunk + word * kWave + lane;
-        const uint64_t bits = __ballot(b < blocks && refs[min(b, blocks - 1)] <= 0);
-        if (lane == 0) bitmap[static_cast<int64_t>(c) * kChunkWords + word] = bits;
+    for (int k = 0; k < kWaveWords; ++k) {
+        const int b = c * kChunk + (word + k) * kWave + lane;
+        const uint64_t bits = __ballot(b < blocks && ref[k] <= 0);
+        if (lane == 0) bitmap[static_cast<int64_t>(c) * kChunkWords + word + k] = bits;
         count += __popcll(bits);
     }
     if (lane == 0) wave_count[wave] = count;
@@ -202,7 +208,9 @@ __device__ __forceinline__ void select_free(const uint64_t* __restrict__ bitmap,
         }
         __syncthreads();
         for (int k = wave; k < list_n; k += kWaves) {
-            uint64_t bits = bitmap[static_cast<int64_t>(list_chunk[k]) * kChunkWords + lane];
+            uint64_t bits = 0;
+            if (lane < kChunkWords)
+                bits = bitmap[static_cast<int64_t>(list_chunk[k]) * kChunkWords + lane];
             const int here = __popcll(bits);
             int rank = list_rank[k] + wave_inclusive(here) - here;
             for (; bits != 0 && rank < hi; bits &= bits - 1, ++rank)
@@ -431,6 +439,11 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const int32_t* r
     __shared__ int word_free[kChunkWords];  // free blocks of the chunk before a word
     const int c = blockIdx.x;
     const int lane = threadIdx.x & 63;
+    constexpr int kEach = kChunk / kThreads;
+    int counts[kEach];  // of this lane's blocks, asked for first
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+        counts[k] = refs[min(c * kChunk + k * kThreads + static_cast<int>(threadIdx.x), blocks - 1)];
     int all = 0, before = 0;
     for (int j = threadIdx.x; j < chunks; j += kThreads) {
         const int n = ws.counts[j];
@@ -455,15 +468,20 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const int32_t* r
     group_exclusive(below, holes_before);
     const int holes = holes_before;
     if (threadIdx.x < kWave) {
-        const int n = __popcll(ws.bitmap[static_cast<int64_t>(c) * kChunkWords + lane]);
-        word_free[lane] = wave_inclusive(n) - n;
+        int n = 0;
+        if (lane < kChunkWords)
+            n = __popcll(ws.bitmap[static_cast<int64_t>(c) * kChunkWords + lane]);
+        const int before_word = wave_inclusive(n) - n;
+        if (lane < kChunkWords) word_free[lane] = before_word;
     }
     __syncthreads();
     if (c == 0 && threadIdx.x == 0) {
         *num_live = n_live;
         ws.moves[0] = holes;
     }
-    for (int k = threadIdx.x; k < kChunk; k += kThreads) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int k = e * kThreads + threadIdx.x;
         const int b = c * kChunk + k;
         if (b >= blocks) break;
         const int word = k / kWave;
@@ -471,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const int32_t* r
         const uint64_t low = (1ull << (k % kWave)) - 1;
         const bool is_free = (bits >> (k % kWave)) & 1;
         const int free_rank = free_before + word_free[word] + __popcll(bits & low);
-        const int count = refs[b];
+        const int count = counts[e];
         int out = 0, to = -1;
         if (is_free) {
             if (b < n_live) ws.holes[free_rank] = b;
@@ -520,11 +538,12 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(const int32_t* t
         return;
     }
     const int parts = max(1, 2 * kv.layers);
-    const int64_t units = static_cast<int64_t>(ws.moves[0]) * parts;
+    const int moves = ws.moves[0];
+    const int64_t units = static_cast<int64_t>(moves) * parts;
     const int groups = gridDim.x - table_groups;
     for (int64_t q = blockIdx.x - table_groups; q < units; q += groups) {
-        const int j = static_cast<int>(q / parts);
-        const int part = static_cast<int>(q - static_cast<int64_t>(j) * parts);
+        const int part = static_cast<int>(q / moves);
+        const int j = static_cast<int>(q - static_cast<int64_t>(part) * moves);
         const int from = ws.movers[j], to = ws.holes[j];
         if (part == 0 && threadIdx.x == 0) {
             refs_out[to] = ws.counts_of[j];
@@ -540,7 +559,7 @@ hipError_t copy_kv_blocks(const KvLayers& kv, const int32_t* src, const int32_t*
                           int32_t* status, hipStream_t stream) {
     // enough workgroups to fill the chip, and no more lists checked than that takes
     const int parts = 2 * kv.layers;
-    const int split = std::min(parts, std::max(1, (4096 + pairs - 1) / pairs));
+    const int split = std::min(parts, std::max(1, (16384 + pairs - 1) / pairs));
     const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(split));
     return with_unit(kv, [&](auto unit) {
         copy_blocks_kernel<decltype(unit)><<<grid, kThreads, 0, stream>>>(kv, src, dst, pairs,
@@ -588,7 +607,7 @@ hipError_t compact_kv_blocks(const int32_t* table, const int32_t* refs, int64_t 
     const int table_groups =
         static_cast<int>(std::min<int64_t>(256, (entries + kThreads - 1) / kThreads));
     const int64_t most = static_cast<int64_t>(kv.blocks / 2 + 1) * std::max(1, 2 * kv.layers);
-    const int move_groups = static_cast<int>(std::min<int64_t>(2048, most));
+    const int move_groups = static_cast<int>(std::min<int64_t>(8192, most));
     return with_unit(kv, [&](auto unit) {
         compact_move_kernel<decltype(unit)>
             <<<static_cast<unsigned>(table_groups + move_groups), kThreads, 0, stream>>>(

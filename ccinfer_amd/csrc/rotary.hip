@@ -15,7 +15,9 @@
 // by memory (or, for a few tokens, by latency).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "attn_common.hpp"
 #include "fp8_row.hpp"
@@ -43,17 +45,21 @@ __device__ __forceinline__ float wave_max(float v) {
 // written by the same lane, so a call may write where it reads. Any even head_dim up to 1024,
 // any 2-byte alignment and stride.
 template <bool kInterleaved, bool kFp8>
-__global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
+__device__ __forceinline__ void rotary_row(const RotaryArgs& a, int64_t row) {
     constexpr int kSteps = kRotaryMaxHeadDim / 2 / kWave;
     const int lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
     const int heads = a.sec[0].heads + a.sec[1].heads + a.sec[2].heads;
-    if (row >= static_cast<int64_t>(a.tokens) * heads) return;
     const int t = static_cast<int>(row / heads);
     int h = static_cast<int>(row - static_cast<int64_t>(t) * heads);
-    int s = 0;
-    while (h >= a.sec[s].heads) h -= a.sec[s++].heads;
-    const RotarySection& c = a.sec[s];
+    RotarySection c = a.sec[0];
+    if (h >= c.heads) {
+        h -= c.heads;
+        c = a.sec[1];
+        if (h >= c.heads) {
+            h -= c.heads;
+            c = a.sec[2];
+        }
+    }
     int64_t out_row = t;
     if (c.to_cache) {
         out_row = a.slot_mapping[t];
@@ -76,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
         sum += x0[i] * x0[i] + x1[i] * x1[i];
     }
     float inv = 1.f;
-    if (c.norm) inv = rsqrtf(wave_sum(sum) / static_cast<float>(a.head_dim) + a.eps);
+    if (c.norm) inv = rsqrtf(wave_sum(sum) * a.per_elem + a.eps);
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -126,23 +132,280 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
     }
 }
 
+template <bool kInterleaved, bool kFp8>
+__global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
+    const int64_t rows = static_cast<int64_t>(a.tokens) *
+                         (a.sec[0].heads + a.sec[1].heads + a.sec[2].heads);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave; row < rows;
+         row += static_cast<int64_t>(gridDim.x) * kWaves)
+        rotary_row<kInterleaved, kFp8>(a, row);
+}
+
+// The kernel of the ordinary shapes. A row is held by G lanes (a power of two), one chunk of
+// sixteen elements a lane, as two segments of eight:
+//   split chunk       pairs p .. p + 7 of the half layout: elements p .. and R/2 + p ..
+//   contiguous chunk  elements e .. e + 15: interleaved pairs, elements past R, v rows
+// so both elements of every pair are in one lane in either layout. A wavefront holds 64 / G rows
+// of one section of one token, and all its loads are on their way before the first is needed.
+// Where the width is no multiple of a chunk, the last chunk is moved back to end with
+// it: its first elements are another lane's too, which counts them in the sum of squares and
+// writes the same values. Segments start at any even byte; the loads and stores claim 2-byte
+// alignment, which the hardware takes at full width.
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
+typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
+
+constexpr int kSegment = 8;
+constexpr int kChunkElems = 2 * kSegment;
+
+template <int Ctrl>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), Ctrl, 0xf, 0xf, true));
+}
+
+// op over groups of `lanes` (a power of two, the same for all) lanes; every lane gets the result.
+template <typename Op>
+__device__ __forceinline__ float group_reduce(float v, int lanes, Op op) {
+    if (lanes > 1) v = op(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
+    if (lanes > 2) v = op(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
+    if (lanes > 4) v = op(v, dpp<0x141>(v));  // row_half_mirror: the other quad of eight
+    if (lanes > 8) v = op(v, dpp<0x140>(v));  // row_mirror: the other eight of sixteen
+    if (lanes > 16) v = op(v, __shfl_xor(v, 16, 64));
+    if (lanes > 32) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+
+__device__ __forceinline__ float elem(const u32x4& w, int i) {
+    return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+}
+
+__device__ __forceinline__ u32x4 load_segment(const __bf16* p) {
+    return *reinterpret_cast<const u32x4_a2*>(p);
+}
+
+struct VecPlan {
+    int lanes;        // G
+    int split;        // split chunks of a rotated row (half layout), 0 for interleaved
+    int chunks;       // chunks of a q or k row
+    int plain;        // chunks of a v row
+    int units[3];     // wavefronts of a section and token
+    bool whole;       // no chunk was moved back, and no interleaved chunk crosses R
+};
+
+template <bool kInterleaved, bool kFp8, bool kWhole>
+__global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, VecPlan plan) {
+    const int lane = threadIdx.x & 63;
+    const int sub = lane & (plan.lanes - 1);
+    const int in_slab = lane / plan.lanes;
+    const int per_slab = kWave / plan.lanes;
+    const uint32_t units = plan.units[0] + plan.units[1] + plan.units[2];
+    const uint32_t total = static_cast<uint32_t>(a.tokens) * units;
+    const int half = a.rotary_dim / 2;
+    for (uint32_t id = blockIdx.x * kWaves +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+         id < total; id += gridDim.x * kWaves) {
+        const int t = static_cast<int>(id / units);
+        // asked for first: the table's row waits for the position, the rows for nothing
+        const int pos = a.positions[t];
+        const int slot = a.slot_mapping != nullptr ? a.slot_mapping[t] : -1;
+        int u = static_cast<int>(id - static_cast<uint32_t>(t) * units);
+        int s = 0;
+        while (u >= plan.units[s]) u -= plan.units[s++];
+        const RotarySection& c = a.sec[s];
+        const int chunks = s == 2 ? plan.plain : plan.chunks;
+        const bool live = sub < chunks;
+        const int chunk = min(sub, chunks - 1);
+        const bool split = s < 2 && chunk < plan.split;
+        // first pair (split) or element of the chunk, and how many of it are another lane's
+        int at, again, seg_a, seg_b;
+        if (split) {
+            at = min(chunk * kSegment, half - kSegment);
+            again = chunk * kSegment - at;
+            seg_a = at;
+            seg_b = half + at;
+        } else {
+            const int first = s < 2 && plan.split > 0 ? a.rotary_dim : 0;
+            const int e = first + (chunk - (s < 2 ? plan.split : 0)) * kChunkElems;
+            at = min(e, a.head_dim - kChunkElems);
+            again = e - at;
+            seg_a = at;
+            seg_b = at + kSegment;
+        }
+        const int h = u * per_slab + in_slab;
+        const bool store = live && h < c.heads;
+        const int h_in = min(h, c.heads - 1);
+        const __bf16* row = c.src + t * c.src_t + h_in * c.src_h;
+        const u32x4 xa = load_segment(row + seg_a), xb = load_segment(row + seg_b);
+        int64_t out_row = t;
+        if (c.to_cache) {
+            if (slot < 0 || slot >= a.max_slots) continue;
+            out_row = slot;
+        }
+        // (cos, sin) of the chunk's eight pairs; `turn` bit i: pair i is rotated (kWhole: any)
+        float cs[kSegment], sn[kSegment];
+        uint32_t turn = 0;
+        if (c.rotate) {
+            if (pos >= 0 && pos < a.rope_max) {
+                const float2* table = a.rope_cache + static_cast<int64_t>(pos) * half;
+                const int p0 = split ? at : at / 2;
+                if constexpr (kWhole) {
+                    turn = split || (kInterleaved && p0 < half);
+                    const float2* from = table + (turn ? p0 : 0);
+#pragma unroll
+                    for (int i = 0; i < kSegment / 2; ++i) {
+                        const f32x4 v = reinterpret_cast<const f32x4_a8*>(from)[i];
+                        cs[2 * i] = v[0], sn[2 * i] = v[1];
+                        cs[2 * i + 1] = v[2], sn[2 * i + 1] = v[3];
+                    }
+                } else {
+                    const bool in = split || kInterleaved;
+#pragma unroll
+                    for (int i = 0; i < kSegment; ++i) {
+                        const float2 v = table[min(p0 + i, half - 1)];
+                        cs[i] = v.x, sn[i] = v.y;
+                        turn |= in && p0 + i < half ? 1u << i : 0u;
+                    }
+                }
+            }
+        }
+        u32x4 wa{}, wb{};
+        if (c.norm) {
+            const __bf16* from = c.weight + h_in * c.weight_h;
+            wa = load_segment(from + seg_a);
+            wb = load_segment(from + seg_b);
+        }
+        if (a.sin_sign < 0.f) {
+#pragma unroll
+            for (int i = 0; i < kSegment; ++i) sn[i] = -sn[i];
+        }
+        float x[kChunkElems];
+#pragma unroll
+        for (int i = 0; i < kSegment; ++i) {
+            x[i] = elem(xa, i);
+            x[kSegment + i] = elem(xb, i);
+        }
+        if (c.norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kChunkElems; ++i) {
+                if constexpr (kWhole) {
+                    sum += x[i] * x[i];
+                } else {
+                    const bool mine = (split ? (i & (kSegment - 1)) : i) >= again;
+                    sum += mine ? x[i] * x[i] : 0.f;
+                }
+            }
+            sum = group_reduce(live ? sum : 0.f, plan.lanes,
+                               [](float p, float q) { return p + q; });
+            const float inv = rsqrtf(sum * a.per_elem + a.eps);
+#pragma unroll
+            for (int i = 0; i < kSegment; ++i) {
+                x[i] *= inv * (elem(wa, i) + a.weight_offset);
+                x[kSegment + i] *= inv * (elem(wb, i) + a.weight_offset);
+            }
+        }
+        // under a branch or a select, so that nothing of a pair that is not rotated meets
+        // another one's infinity
+        if (turn != 0) {
+#pragma unroll
+            for (int i = 0; i < kSegment; ++i) {
+                const int p = kInterleaved ? 2 * i : i;
+                const int q = kInterleaved ? 2 * i + 1 : kSegment + i;
+                const float u0 = x[p] * cs[i] - x[q] * sn[i];
+                const float u1 = x[q] * cs[i] + x[p] * sn[i];
+                const bool r = kWhole || ((turn >> i) & 1);
+                x[p] = r ? u0 : x[p];
+                x[q] = r ? u1 : x[q];
+            }
+        }
+        if (kFp8 && c.to_cache) {
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < kChunkElems; ++i) amax = fmaxf(amax, fabsf(x[i]));
+            amax = group_reduce(amax, plan.lanes,
+                                [](float p, float q) { return fmaxf(p, q); });
+            const float scale = fp8_row_scale(amax);
+            const float by = fp8_row_inverse(scale);
+            if (!store) continue;
+            uint8_t* dst = static_cast<uint8_t*>(c.dst) + out_row * c.dst_t + h * c.dst_h;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    q[i] = fp8_pair(x[g * kSegment + 2 * i] * by,
+                                    x[g * kSegment + 2 * i + 1] * by);
+                *reinterpret_cast<u32x2_a1*>(dst + (g == 0 ? seg_a : seg_b)) =
+                    u32x2{q[0] | q[1] << 16, q[2] | q[3] << 16};
+            }
+            if (sub == 0) c.scale[fp8_scale_index(out_row, h, c.heads)] = scale;
+            continue;
+        }
+        if (!store) continue;
+        __bf16* dst = static_cast<__bf16*>(c.dst) + out_row * c.dst_t + h * c.dst_h;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = pack_bf16x2(x[g * kSegment + 2 * i], x[g * kSegment + 2 * i + 1]);
+            __builtin_nontemporal_store(
+                w, reinterpret_cast<u32x4_a2*>(dst + (g == 0 ? seg_a : seg_b)));
+        }
+    }
+}
+
+// Whether the chunks above cover a row of this shape, and how.
+bool vec_plan(const RotaryArgs& a, bool interleaved, VecPlan& plan) {
+    const int d = a.head_dim, r = a.rotary_dim, tail = d - r;
+    if (d < kChunkElems) return false;
+    // a half-layout row has its rotated pairs in split chunks and the rest in contiguous ones:
+    // each part is empty or holds a chunk
+    if (!interleaved && (r / 2 < kSegment || (tail > 0 && tail < kChunkElems))) return false;
+    auto up = [](int n, int m) { return (n + m - 1) / m; };
+    plan.split = interleaved ? 0 : up(r / 2, kSegment);
+    plan.chunks = plan.split + up(interleaved ? d : tail, kChunkElems);
+    plan.plain = up(d, kChunkElems);
+    const int most = std::max(plan.chunks, plan.plain);
+    if (most > kWave) return false;
+    plan.lanes = 1;
+    while (plan.lanes < most) plan.lanes *= 2;
+    plan.whole = r % kChunkElems == 0 && d % kChunkElems == 0;
+    for (int s = 0; s < 3; ++s) plan.units[s] = up(a.sec[s].heads, kWave / plan.lanes);
+    return true;
+}
+
 }  // namespace
 
 hipError_t rotary_rows(const RotaryArgs& a, bool interleaved, bool fp8, hipStream_t stream) {
-    const int64_t rows =
-        static_cast<int64_t>(a.tokens) * (a.sec[0].heads + a.sec[1].heads + a.sec[2].heads);
-    const unsigned grid = static_cast<unsigned>((rows + kWaves - 1) / kWaves);
-    if (interleaved) {
-        if (fp8)
-            rotary_rows_kernel<true, true><<<grid, kThreads, 0, stream>>>(a);
+    constexpr int64_t kMostGroups = 1 << 20;  // the kernels go on from there
+    auto with = [&](auto inter, auto to_fp8) {
+        constexpr bool kInter = decltype(inter)::value, kFp8 = decltype(to_fp8)::value;
+        auto groups = [&](int64_t waves) {
+            return static_cast<unsigned>(std::min(kMostGroups, (waves + kWaves - 1) / kWaves));
+        };
+        const int64_t rows = static_cast<int64_t>(a.tokens) *
+                             (a.sec[0].heads + a.sec[1].heads + a.sec[2].heads);
+        VecPlan plan;
+        if (!vec_plan(a, kInter, plan)) {
+            rotary_rows_kernel<kInter, kFp8><<<groups(rows), kThreads, 0, stream>>>(a);
+            return;
+        }
+        const int64_t waves = static_cast<int64_t>(a.tokens) *
+                              (plan.units[0] + plan.units[1] + plan.units[2]);
+        if (plan.whole)
+            rotary_vec_kernel<kInter, kFp8, true><<<groups(waves), kThreads, 0, stream>>>(a, plan);
         else
-            rotary_rows_kernel<true, false><<<grid, kThreads, 0, stream>>>(a);
-    } else {
-        if (fp8)
-            rotary_rows_kernel<false, true><<<grid, kThreads, 0, stream>>>(a);
-        else
-            rotary_rows_kernel<false, false><<<grid, kThreads, 0, stream>>>(a);
-    }
+            rotary_vec_kernel<kInter, kFp8, false><<<groups(waves), kThreads, 0, stream>>>(a, plan);
+    };
+    using std::false_type;
+    using std::true_type;
+    if (interleaved)
+        fp8 ? with(true_type{}, true_type{}) : with(true_type{}, false_type{});
+    else
+        fp8 ? with(false_type{}, true_type{}) : with(false_type{}, false_type{});
     return hipGetLastError();
 }
 

@@ -333,8 +333,9 @@ int ccinfer_rope_frequencies(int rotary_dim, double theta, int scaling, const do
 /* rope_cache[i][p] = m (cos, sin)((first_position + i) f_p), float [num_positions]
  * [rotary_dim / 2][2], the table that the calls below and ccinfer_qkv_prologue read (the
  * reference fills one on the host, src/model/rope/rope_cache.cpp). `frequencies` is a host
- * array that the call has read when it returns; angles are reduced in double precision, so
- * a value is within 2 ulp of m at any position. May be captured into a graph. */
+ * array that the call has read when it returns (at most 65536 radians each); angles are
+ * reduced in double precision: an entry is off by 2^-22 m and 2^-51 of its angle. May be
+ * captured into a graph. */
 int ccinfer_build_rope_cache(const double* frequencies, int rotary_dim, double magnitude,
                              int first_position, int num_positions, void* rope_cache,
                              void* stream);

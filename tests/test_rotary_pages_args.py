@@ -99,6 +99,8 @@ def test_rope_cache_refusals(lib):
     a = list(ok)
     a[3] = 2 ** 31 - 2  # positions past 2^31
     assert lib.ccinfer_build_rope_cache(*a) == INVALID
+    f[5] = 65537.0
+    assert lib.ccinfer_build_rope_cache(*ok) == INVALID
     f[5] = INF
     assert lib.ccinfer_build_rope_cache(*ok) == INVALID
 
