@@ -20,7 +20,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _check, _dev_tensor, _require, _stream, _workspace, current_device
+from .ops import (INVALID_ARGUMENT, CcinferError, _check, _require, _stream, _workspace,
+                  current_device)
 
 KV_EXHAUSTED = 12      # status: not enough free blocks
 KV_INVALID_TABLE = 14  # status: a table row that the pool does not hold
@@ -32,23 +33,27 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
     fp8 = k_scale is not None
     dtype = torch.uint8 if fp8 else torch.bfloat16
     shape, stride = k_cache.shape, k_cache.stride()
-    _require(k_cache.dtype is dtype and v_cache.dtype is dtype and v_cache.shape == shape
-             and v_cache.stride() == stride and k_cache.get_device() == dev
-             and v_cache.get_device() == dev and fp8 == (v_scale is not None), op)
     dims = len(shape)
-    layers, layer_stride = 1, 0
+    _require(3 <= dims <= 5 and k_cache.dtype is dtype and v_cache.dtype is dtype
+             and v_cache.shape == shape
+             and k_cache.get_device() == dev and v_cache.get_device() == dev
+             and fp8 == (v_scale is not None), op)
+    h, d = shape[-2], shape[-1]
+    layers, layer_stride, scale_stride = 1, 0, 0
     if dims == 5:
-        layers, nb, bs, h, d = shape
+        layers, nb, bs = shape[:3]
         layer_stride = stride[0] * (1 if fp8 else 2)
-    elif dims == 4:
-        nb, bs, h, d = shape
+        vstride = v_cache.stride()
+        inner = (bs * h * d, h * d, d, 1)
+        _require((layers == 1 or vstride[0] == stride[0])
+                 and (stride[1:] == inner or k_cache[0].is_contiguous())
+                 and (vstride[1:] == inner or v_cache[0].is_contiguous()), op)
     else:
-        _require(dims == 3 and shape[0] % block_size == 0, op)
-        nb, bs, h, d = shape[0] // block_size, block_size, shape[1], shape[2]
-    inner = (bs * h * d, h * d, d, 1) if dims >= 4 else (h * d, d, 1)
-    _require(bs == block_size and (dims == 5 and stride[1:] == inner or stride == inner), op)
+        nb, bs = (shape[0], shape[1]) if dims == 4 else (shape[0] // block_size, block_size)
+        _require((dims == 4 or nb * bs == shape[0]) and k_cache.is_contiguous()
+                 and v_cache.is_contiguous(), op)
+    _require(bs == block_size, op)
     ksp = vsp = None
-    scale_stride = 0
     if fp8:
         need = nb * h * 16
         for s in (k_scale, v_scale):
@@ -57,22 +62,18 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
                 _require(s.is_contiguous() and s.numel() >= need, op)
             else:
                 _require(s.dim() == 2 and s.shape[0] == layers and s.shape[1] >= need
-                         and s.stride(1) == 1 and s.stride(0) == k_scale.stride(0), op)
+                         and s.stride() == k_scale.stride() and s.stride(1) == 1, op)
         scale_stride = k_scale.stride(0) if layers > 1 else 0
         ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
     return (k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, layers, layer_stride, scale_stride,
-            nb, h, d, block_size)
+            nb, h, d, bs)
 
 
-def _indices(dev: int, op: str, *tensors) -> None:
-    for t in tensors:
-        _dev_tensor(t, torch.int32, op)
-        _require(t.get_device() == dev, op)
-
-
-def _status_word(status: Optional[torch.Tensor], dev: int, op: str) -> None:
-    _indices(dev, op, status)
-    _require(status.numel() == 1, op)
+def _index(t: torch.Tensor, dev: int, op: str) -> int:
+    """Elements of a contiguous int32 tensor on the device."""
+    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+        raise CcinferError(INVALID_ARGUMENT, op)
+    return t.numel()
 
 
 def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: torch.Tensor,
@@ -85,12 +86,11 @@ def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: tor
     another source, or another pair's source. `status` (int32 [1]), if given, becomes 6 then
     and is left alone otherwise."""
     op = "copy_kv_blocks"
+    _require(k_cache.is_cuda, op)
     dev = current_device()
-    _indices(dev, op, src_blocks, dst_blocks)
-    n = src_blocks.numel()
-    _require(dst_blocks.numel() == n, op)
-    if status is not None:
-        _status_word(status, dev, op)
+    n = _index(src_blocks, dev, op)
+    _require(_index(dst_blocks, dev, op) == n
+             and (status is None or _index(status, dev, op) == 1), op)
     kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
         k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
     _check(_lib.load().ccinfer_copy_kv_blocks(
@@ -127,19 +127,18 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     out of range, a row twice in dst_rows, a copy needed but no caches given), 14 (a row with a
     context or blocks that the pool does not hold) or 12 (not enough free blocks)."""
     op = "update_block_tables"
+    _require(block_table.is_cuda, op)
     dev = current_device()
-    _indices(dev, op, block_table, context_lens, ref_counts, dst_rows)
-    _require(block_table.dim() == 2 and context_lens.numel() == block_table.shape[0], op)
-    rows, width = block_table.shape
-    n, nb = dst_rows.numel(), ref_counts.numel()
-    for t in (src_rows, lengths):
-        if t is not None:
-            _indices(dev, op, t)
-            _require(t.numel() == n, op)
+    _index(block_table, dev, op)
+    n, nb = _index(dst_rows, dev, op), _index(ref_counts, dev, op)
+    shape = block_table.shape
+    _require(len(shape) == 2 and _index(context_lens, dev, op) == shape[0]
+             and (src_rows is None or _index(src_rows, dev, op) == n)
+             and (lengths is None or _index(lengths, dev, op) == n)
+             and (status is None or _index(status, dev, op) == 1), op)
+    rows, width = shape
     if status is None:
         status = torch.empty(1, dtype=torch.int32, device=block_table.device)
-    else:
-        _status_word(status, dev, op)
     if k_cache is None:
         _require(v_cache is None and k_scale is None and v_scale is None, op)
         kp = vp = ksp = vsp = None
@@ -177,8 +176,10 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     num_live [1]. Table entries of free blocks become -1, negative ones stay. `out` reuses
     tensors of an earlier call; its block_table and ref_counts may be the inputs."""
     op = "compact_kv_blocks"
+    _require(block_table.is_cuda, op)
     dev = current_device()
-    _indices(dev, op, block_table, ref_counts)
+    _index(block_table, dev, op)
+    _index(ref_counts, dev, op)
     _require(block_table.dim() == 2, op)
     kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
         k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
@@ -189,9 +190,9 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
                "num_live": torch.empty(1, dtype=torch.int32, device=block_table.device)}
     table, refs, remap, live = (out["block_table"], out["ref_counts"], out["remap"],
                                 out["num_live"])
-    _indices(dev, op, table, refs, remap, live)
-    _require(table.shape == block_table.shape and refs.numel() == nb and remap.numel() == nb
-             and live.numel() == 1, op)
+    _index(table, dev, op)
+    _require(table.shape == block_table.shape and _index(refs, dev, op) == nb
+             and _index(remap, dev, op) == nb and _index(live, dev, op) == 1, op)
     ws, ws_bytes = _workspace(compact_workspace_size(nb), block_table.device, workspace)
     rows, width = block_table.shape
     _check(_lib.load().ccinfer_compact_kv_blocks(

@@ -13,7 +13,8 @@ from typing import List, Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _check, _dev_tensor, _kv_shape, _require, _stream, current_device, fp8_scale_numel
+from .ops import (CcinferError, _check, _dev_tensor, _require, _stream, current_device,
+                  fp8_scale_numel)
 
 ROPE_SCALINGS = ("none", "linear", "ntk", "yarn", "bands", "factors")
 _PARAMS = 5  # doubles before the pairs' own factors (enum ccinfer_rope_scaling)
@@ -82,35 +83,26 @@ def build_rope_cache(max_position: int, rotary_dim: int, theta: float = 10000.0,
     return out
 
 
-def _table(rope_cache: torch.Tensor, head_dim: int, op: str) -> Tuple[int, int]:
-    """(positions, rotary_dim) of a table."""
-    _dev_tensor(rope_cache, torch.float32, op)
-    shape = rope_cache.shape
-    _require(len(shape) == 3 and shape[2] == 2 and 2 <= 2 * shape[1] <= head_dim, op)
-    return shape[0], 2 * shape[1]
+# The smallest calls below take 2 us on the GPU, so their host side bounds them: the checks are
+# single expressions of few interpreter steps. Host time
+# of a call, launch included: rotary_embedding 9.3 -> @R us, qkv_norm_rope 11.6 -> @N us.
+
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _rows(x: torch.Tensor, op: str):
-    """Shape and strides of [tokens, heads, head_dim] rows."""
-    _require(x.dtype is torch.bfloat16 and x.is_cuda and x.dim() == 3, op)
-    shape, stride = x.shape, x.stride()
-    _require(stride[2] == 1 or shape[2] == 1, op)
-    return shape, stride
-
-
-def _out_rows(x: torch.Tensor, shape, stride, out: Optional[torch.Tensor], op: str):
-    """The output rows of x and their strides; no two of them may share memory."""
-    if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
-        return out, out.stride()
-    oshape, ostride = _rows(out, op)
+def _out_stride(x, shape, stride, out, dev: int, op: str):
+    """Strides of the output rows `out` of x; no two of them may share memory."""
     t, h, d = shape
-    st, sh, _ = ostride
-    apart = (sh >= d and st >= h * sh) or (st >= d and sh >= t * st) \
-        or (h == 1 and st >= d) or (t == 1 and sh >= d) or (t == 1 and h == 1)
-    same = out.data_ptr() == x.data_ptr()
-    _require(oshape == shape and apart and (not same or ostride == stride), op)
-    return out, ostride
+    ostride = out.stride()
+    if ostride == (h * d, d, 1):
+        apart = True
+    else:
+        st, sh, sd = ostride if out.dim() == 3 else (0, 0, 0)
+        apart = sd == 1 and ((sh >= d and st >= h * sh) or (st >= d and sh >= t * st)
+                             or (h == 1 and st >= d) or (t == 1 and sh >= d) or t * h == 1)
+    _require(apart and out.dtype is _BF16 and out.shape == shape and out.get_device() == dev
+             and (out.data_ptr() != x.data_ptr() or ostride == stride), op)
+    return ostride
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -126,29 +118,40 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     views whose heads are contiguous (slices of the packed projection); q_out = q and k_out = k
     rotate in place, any other outputs lie apart from the inputs."""
     op = "rotary_embedding"
-    shape, qs = _rows(q, op)
+    _require(q.is_cuda, op)
+    dev = current_device()
+    shape, qs, table = q.shape, q.stride(), rope_cache.shape
+    _require(len(shape) == 3 == len(table) and table[2] == 2 and qs[2] == 1
+             and q.dtype is _BF16 and positions.dtype is _I32 and rope_cache.dtype is _F32
+             and q.get_device() == dev and positions.get_device() == dev
+             and rope_cache.get_device() == dev and positions.is_contiguous()
+             and rope_cache.is_contiguous() and positions.numel() == shape[0] > 0, op)
     t, hq, d = shape
-    max_pos, rotary_dim = _table(rope_cache, d, op)
-    _dev_tensor(positions, torch.int32, op)
-    dev = q.get_device()
-    _require(t > 0 and positions.numel() == t and dev == current_device()
-             and positions.get_device() == dev and rope_cache.get_device() == dev, op)
-    q_out, qos = _out_rows(q, shape, qs, q_out, op)
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=_BF16, device=q.device)
+        qos = q_out.stride()
+    else:
+        qos = _out_stride(q, shape, qs, q_out, dev, op)
     if k is None:
         _require(k_out is None, op)
         hkv, ks, kos, kp, kop = 0, (0, 0), (0, 0), None, None
     else:
-        kshape, ks = _rows(k, op)
+        kshape, ks = k.shape, k.stride()
+        _require(len(kshape) == 3 and kshape[0] == t and kshape[2] == d and ks[2] == 1
+                 and k.dtype is _BF16 and k.get_device() == dev, op)
         hkv = kshape[1]
-        _require(kshape[0] == t and kshape[2] == d and k.get_device() == dev, op)
-        k_out, kos = _out_rows(k, kshape, ks, k_out, op)
+        if k_out is None:
+            k_out = torch.empty(kshape, dtype=_BF16, device=k.device)
+            kos = k_out.stride()
+        else:
+            kos = _out_stride(k, kshape, ks, k_out, dev, op)
         kp, kop = k.data_ptr(), k_out.data_ptr()
-        _require(k_out.get_device() == dev, op)
-    _require(q_out.get_device() == dev, op)
-    _check(_lib.load().ccinfer_rotary_embedding(
+    code = _lib.load().ccinfer_rotary_embedding(
         q.data_ptr(), qs[0], qs[1], kp, ks[0], ks[1], positions.data_ptr(),
         rope_cache.data_ptr(), q_out.data_ptr(), qos[0], qos[1], kop, kos[0], kos[1], t, hq, hkv,
-        d, rotary_dim, max_pos, interleaved, inverse, _stream()), op)
+        d, 2 * table[1], table[0], interleaved, inverse, _stream())
+    if code:
+        raise CcinferError(code, op)
     return q_out, k_out
 
 
@@ -156,10 +159,11 @@ def _norm_weight(w: Optional[torch.Tensor], heads: int, d: int, dev: int, op: st
     """(pointer, whether each head has its own) of a norm weight."""
     if w is None:
         return None, 0
-    _dev_tensor(w, torch.bfloat16, op)
-    shape = tuple(w.shape)
-    _require((shape == (d,) or shape == (heads, d)) and w.get_device() == dev, op)
-    return w.data_ptr(), len(shape) == 2
+    shape = w.shape
+    each = len(shape) == 2
+    _require(shape[-1:] == (d,) and (len(shape) == 1 or each and shape[0] == heads)
+             and w.dtype is _BF16 and w.is_contiguous() and w.get_device() == dev, op)
+    return w.data_ptr(), each
 
 
 def qkv_norm_rope(qkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
@@ -182,42 +186,48 @@ def qkv_norm_rope(qkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
     A bf16 cache takes K as the rows that rotary_embedding would return; an fp8 one is
     quantised from float32. No two tokens may have the same slot."""
     op = "qkv_norm_rope"
-    _require(qkv.dtype is torch.bfloat16 and qkv.is_cuda and qkv.dim() == 2, op)
-    _dev_tensor(positions, torch.int32, op)
-    _dev_tensor(slot_mapping, torch.int32, op)
-    fp8 = k_scale is not None
-    for c in (k_cache, v_cache):
-        _dev_tensor(c, torch.uint8 if fp8 else torch.bfloat16, op)
-    slots, hkv, d = _kv_shape(k_cache)
-    max_pos, rotary_dim = _table(rope_cache, d, op)
-    t, width = qkv.shape
+    _require(qkv.is_cuda, op)
+    dev = current_device()
+    shape, table, cache = qkv.shape, rope_cache.shape, k_cache.shape
     stride = qkv.stride()
-    dev = qkv.get_device()
-    _require(t > 0 and num_q_heads > 0 and width == (num_q_heads + 2 * hkv) * d and stride[1] == 1,
-             op)
-    _require(v_cache.shape == k_cache.shape and positions.numel() == t
-             and slot_mapping.numel() == t, op)
-    _require(dev == current_device() == k_cache.get_device() == v_cache.get_device()
-             == positions.get_device() == slot_mapping.get_device() == rope_cache.get_device(), op)
-    _require(max_slots is None or max_slots <= slots, op)
+    fp8 = k_scale is not None
+    kind = torch.uint8 if fp8 else _BF16
+    _require(len(shape) == 2 and len(table) == 3 and table[2] == 2 and stride[1] == 1
+             and 3 <= len(cache) <= 4 and qkv.dtype is _BF16 and k_cache.dtype is kind
+             and v_cache.dtype is kind and positions.dtype is _I32 and slot_mapping.dtype is _I32
+             and rope_cache.dtype is _F32 and qkv.get_device() == dev
+             and k_cache.get_device() == dev and v_cache.get_device() == dev
+             and positions.get_device() == dev and slot_mapping.get_device() == dev
+             and rope_cache.get_device() == dev and k_cache.is_contiguous()
+             and v_cache.is_contiguous() and positions.is_contiguous()
+             and slot_mapping.is_contiguous() and rope_cache.is_contiguous()
+             and v_cache.shape == cache and fp8 == (v_scale is not None), op)
+    hkv, d = cache[-2], cache[-1]
+    slots = cache[0] if len(cache) == 3 else cache[0] * cache[1]
+    t, width = shape
+    _require(t > 0 and num_q_heads > 0 and width == (num_q_heads + 2 * hkv) * d
+             and positions.numel() == t and slot_mapping.numel() == t
+             and (max_slots is None or max_slots <= slots), op)
     ksp = vsp = None
-    _require(fp8 == (v_scale is not None), op)
     if fp8:
+        need = fp8_scale_numel(slots, hkv)
         for s in (k_scale, v_scale):
-            _dev_tensor(s, torch.float32, op)
-            _require(s.numel() >= fp8_scale_numel(slots, hkv) and s.get_device() == dev, op)
+            _require(s.dtype is _F32 and s.is_contiguous() and s.numel() >= need
+                     and s.get_device() == dev, op)
         ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
     qw, q_each = _norm_weight(q_norm_weight, num_q_heads, d, dev, op)
     kw, k_each = _norm_weight(k_norm_weight, hkv, d, dev, op)
     if q_out is None:
-        q_out = torch.empty((t, num_q_heads, d), dtype=torch.bfloat16, device=qkv.device)
+        q_out = torch.empty((t, num_q_heads, d), dtype=_BF16, device=qkv.device)
     else:
-        _dev_tensor(q_out, torch.bfloat16, op)
-        _require(q_out.numel() == t * num_q_heads * d and q_out.get_device() == dev, op)
-    _check(_lib.load().ccinfer_qkv_norm_rope(
+        _require(q_out.dtype is _BF16 and q_out.is_contiguous()
+                 and q_out.numel() == t * num_q_heads * d and q_out.get_device() == dev, op)
+    code = _lib.load().ccinfer_qkv_norm_rope(
         qkv.data_ptr(), stride[0] if t > 1 else width, qw, q_each, kw, k_each,
         positions.data_ptr(), rope_cache.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, t, num_q_heads, hkv, d, rotary_dim,
-        max_pos, slots if max_slots is None else max_slots, interleaved, eps, weight_offset,
-        _stream()), op)
+        k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, t, num_q_heads, hkv, d, 2 * table[1],
+        table[0], slots if max_slots is None else max_slots, interleaved, eps, weight_offset,
+        _stream())
+    if code:
+        raise CcinferError(code, op)
     return q_out
