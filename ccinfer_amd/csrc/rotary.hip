@@ -41,12 +41,12 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// One wavefront per row; lane l takes the pairs l, l + 64, ... A row's elements are read and
-// written by the same lane, so a call may write where it reads. Any even head_dim up to 1024,
-// any 2-byte alignment and stride.
-template <bool kInterleaved, bool kFp8>
+// The heads that the kernel below leaves: under sixteen elements, and those of about a thousand
+// whose rotated part and rest do not fit its 64 lanes. One wavefront per row; lane l takes the
+// pairs l, l + 64, ... A row's elements are read and written by the same lane, so a call may
+// write where it reads.
+template <bool kInterleaved, bool kFp8, int kSteps>
 __device__ __forceinline__ void rotary_row(const RotaryArgs& a, int64_t row) {
-    constexpr int kSteps = kRotaryMaxHeadDim / 2 / kWave;
     const int lane = threadIdx.x & 63;
     const int heads = a.sec[0].heads + a.sec[1].heads + a.sec[2].heads;
     const int t = static_cast<int>(row / heads);
@@ -132,26 +132,36 @@ __device__ __forceinline__ void rotary_row(const RotaryArgs& a, int64_t row) {
     }
 }
 
-template <bool kInterleaved, bool kFp8>
+template <bool kInterleaved, bool kFp8, int kSteps>
 __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
     const int64_t rows = static_cast<int64_t>(a.tokens) *
                          (a.sec[0].heads + a.sec[1].heads + a.sec[2].heads);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave; row < rows;
          row += static_cast<int64_t>(gridDim.x) * kWaves)
-        rotary_row<kInterleaved, kFp8>(a, row);
+        rotary_row<kInterleaved, kFp8, kSteps>(a, row);
 }
 
-// The kernel of the ordinary shapes. A row is held by G lanes (a power of two), one chunk of
-// sixteen elements a lane, as two segments of eight:
+// The kernel for heads of sixteen elements or more. A row is held by G lanes (a power of two),
+// one chunk a lane, two segments of eight elements:
 //   split chunk       pairs p .. p + 7 of the half layout: elements p .. and R/2 + p ..
-//   contiguous chunk  elements e .. e + 15: interleaved pairs, elements past R, v rows
+//   tail chunk        two segments of the elements from R on (half layout)
+//   contiguous chunk  elements e .. e + 15: interleaved rows, v rows
 // so both elements of every pair are in one lane in either layout. A wavefront holds 64 / G rows
 // of one section of one token, and all its loads are on their way before the first is needed.
-// Where the width is no multiple of a chunk, the last chunk is moved back to end with
+// Where a length is no multiple of its chunk or segment, the last one is moved back to end with
 // it: its first elements are another lane's too, which counts them in the sum of squares and
-// writes the same values. Segments start at any even byte; the loads and stores claim 2-byte
-// alignment, which the hardware takes at full width.
+// writes the same values. Only where fewer than eight pairs are rotated, or fewer than eight
+// elements are not, does a segment reach into elements that are treated otherwise; they are left
+// out and stored one by one. kWhole: R and the head are multiples of sixteen, so there is
+// nothing of this. Segments start at any even byte; the loads and stores claim 2-byte alignment,
+// which the hardware takes at full width.
+//
+// Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 40.0 us with the
+// norm and the cache write, 5.2 TB/s, and a copy of as many bytes 41.1; 8191 tokens x 40 heads
+// half rotated 32.9 us. What that took: eight wavefronts a SIMD (60 registers; at five, with two
+// rows a lane sharing (cos, sin) and weights, 46.8 us) and stores with the streaming hint (41.5
+// without; a prefill that reads the rows afterwards takes the same time either way).
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
@@ -191,7 +201,7 @@ struct VecPlan {
     int chunks;       // chunks of a q or k row
     int plain;        // chunks of a v row
     int units[3];     // wavefronts of a section and token
-    bool whole;       // no chunk was moved back, and no interleaved chunk crosses R
+    bool whole;       // no segment was moved back, and no interleaved chunk crosses R
 };
 
 template <bool kInterleaved, bool kFp8, bool kWhole>
@@ -218,21 +228,32 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         const bool live = sub < chunks;
         const int chunk = min(sub, chunks - 1);
         const bool split = s < 2 && chunk < plan.split;
-        // first pair (split) or element of the chunk, and how many of it are another lane's
-        int at, again, seg_a, seg_b;
+        // where its segments start, and which of their elements are this lane's: [lo, hi)
+        int seg_a, seg_b, lo_a = 0, lo_b = 0, hi = kSegment;
+        bool others = false;  // the elements that are not may not be written
         if (split) {
-            at = min(chunk * kSegment, half - kSegment);
-            again = chunk * kSegment - at;
-            seg_a = at;
-            seg_b = half + at;
+            seg_a = max(0, min(chunk * kSegment, half - kSegment));
+            seg_b = half + seg_a;
+            lo_a = lo_b = chunk * kSegment - seg_a;
+            hi = min(kSegment, half);
+            others = half < kSegment;
+        } else if (s < 2 && plan.split > 0) {
+            const int ua = a.rotary_dim + (chunk - plan.split) * kChunkElems, ub = ua + kSegment;
+            seg_a = min(ua, a.head_dim - kSegment);
+            lo_a = ua - seg_a;
+            seg_b = ub < a.head_dim ? min(ub, a.head_dim - kSegment) : seg_a;
+            lo_b = ub < a.head_dim ? ub - seg_b : kSegment;
+            others = a.head_dim - a.rotary_dim < kSegment;
         } else {
-            const int first = s < 2 && plan.split > 0 ? a.rotary_dim : 0;
-            const int e = first + (chunk - (s < 2 ? plan.split : 0)) * kChunkElems;
-            at = min(e, a.head_dim - kChunkElems);
-            again = e - at;
-            seg_a = at;
-            seg_b = at + kSegment;
+            seg_a = min(chunk * kChunkElems, a.head_dim - kChunkElems);
+            seg_b = seg_a + kSegment;
+            lo_a = min(chunk * kChunkElems - seg_a, kSegment);
+            lo_b = max(chunk * kChunkElems - seg_b, 0);
         }
+        auto mine = [&](int i) {
+            return i < kSegment ? i >= lo_a && i < hi
+                                : i - kSegment >= lo_b && i - kSegment < hi;
+        };
         const int h = u * per_slab + in_slab;
         const bool store = live && h < c.heads;
         const int h_in = min(h, c.heads - 1);
@@ -249,10 +270,12 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         if (c.rotate) {
             if (pos >= 0 && pos < a.rope_max) {
                 const float2* table = a.rope_cache + static_cast<int64_t>(pos) * half;
-                const int p0 = split ? at : at / 2;
-                if constexpr (kWhole) {
-                    turn = split || (kInterleaved && p0 < half);
-                    const float2* from = table + (turn ? p0 : 0);
+                const int p0 = split ? seg_a : seg_a / 2;
+                // all of a half-layout chunk's pairs are rotated, or none
+                if (kWhole || (!kInterleaved && half >= kSegment)) {
+                    const bool in = split || (kInterleaved && p0 < half);
+                    turn = in ? 0xffu : 0u;
+                    const float2* from = table + (in ? p0 : 0);
 #pragma unroll
                     for (int i = 0; i < kSegment / 2; ++i) {
                         const f32x4 v = reinterpret_cast<const f32x4_a8*>(from)[i];
@@ -290,12 +313,10 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < kChunkElems; ++i) {
-                if constexpr (kWhole) {
+                if constexpr (kWhole)
                     sum += x[i] * x[i];
-                } else {
-                    const bool mine = (split ? (i & (kSegment - 1)) : i) >= again;
-                    sum += mine ? x[i] * x[i] : 0.f;
-                }
+                else
+                    sum += mine(i) ? x[i] * x[i] : 0.f;
             }
             sum = group_reduce(live ? sum : 0.f, plan.lanes,
                                [](float p, float q) { return p + q; });
@@ -315,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
                 const int q = kInterleaved ? 2 * i + 1 : kSegment + i;
                 const float u0 = x[p] * cs[i] - x[q] * sn[i];
                 const float u1 = x[q] * cs[i] + x[p] * sn[i];
-                const bool r = kWhole || ((turn >> i) & 1);
+                const bool r = kWhole || !kInterleaved || ((turn >> i) & 1);
                 x[p] = r ? u0 : x[p];
                 x[q] = r ? u1 : x[q];
             }
@@ -323,7 +344,8 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         if (kFp8 && c.to_cache) {
             float amax = 0.f;
 #pragma unroll
-            for (int i = 0; i < kChunkElems; ++i) amax = fmaxf(amax, fabsf(x[i]));
+            for (int i = 0; i < kChunkElems; ++i)
+                amax = kWhole || mine(i) ? fmaxf(amax, fabsf(x[i])) : amax;
             amax = group_reduce(amax, plan.lanes,
                                 [](float p, float q) { return fmaxf(p, q); });
             const float scale = fp8_row_scale(amax);
@@ -337,8 +359,15 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
                 for (int i = 0; i < 4; ++i)
                     q[i] = fp8_pair(x[g * kSegment + 2 * i] * by,
                                     x[g * kSegment + 2 * i + 1] * by);
-                *reinterpret_cast<u32x2_a1*>(dst + (g == 0 ? seg_a : seg_b)) =
-                    u32x2{q[0] | q[1] << 16, q[2] | q[3] << 16};
+                uint8_t* to = dst + (g == 0 ? seg_a : seg_b);
+                if (kWhole || !others) {
+                    *reinterpret_cast<u32x2_a1*>(to) = u32x2{q[0] | q[1] << 16, q[2] | q[3] << 16};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kSegment; ++i)
+                        if (mine(g * kSegment + i))
+                            to[i] = static_cast<uint8_t>(q[i / 2] >> (8 * (i & 1)));
+                }
             }
             if (sub == 0) c.scale[fp8_scale_index(out_row, h, c.heads)] = scale;
             continue;
@@ -351,23 +380,26 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 w[i] = pack_bf16x2(x[g * kSegment + 2 * i], x[g * kSegment + 2 * i + 1]);
-            __builtin_nontemporal_store(
-                w, reinterpret_cast<u32x4_a2*>(dst + (g == 0 ? seg_a : seg_b)));
+            __bf16* to = dst + (g == 0 ? seg_a : seg_b);
+            if (kWhole || !others) {
+                __builtin_nontemporal_store(w, reinterpret_cast<u32x4_a2*>(to));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kSegment; ++i)
+                    if (mine(g * kSegment + i)) to[i] = static_cast<__bf16>(x[g * kSegment + i]);
+            }
         }
     }
 }
 
 // Whether the chunks above cover a row of this shape, and how.
 bool vec_plan(const RotaryArgs& a, bool interleaved, VecPlan& plan) {
-    const int d = a.head_dim, r = a.rotary_dim, tail = d - r;
+    const int d = a.head_dim, r = a.rotary_dim;
     if (d < kChunkElems) return false;
-    // a half-layout row has its rotated pairs in split chunks and the rest in contiguous ones:
-    // each part is empty or holds a chunk
-    if (!interleaved && (r / 2 < kSegment || (tail > 0 && tail < kChunkElems))) return false;
     auto up = [](int n, int m) { return (n + m - 1) / m; };
     plan.split = interleaved ? 0 : up(r / 2, kSegment);
-    plan.chunks = plan.split + up(interleaved ? d : tail, kChunkElems);
     plan.plain = up(d, kChunkElems);
+    plan.chunks = interleaved ? plan.plain : plan.split + up(d - r, kChunkElems);
     const int most = std::max(plan.chunks, plan.plain);
     if (most > kWave) return false;
     plan.lanes = 1;
@@ -390,7 +422,11 @@ hipError_t rotary_rows(const RotaryArgs& a, bool interleaved, bool fp8, hipStrea
                              (a.sec[0].heads + a.sec[1].heads + a.sec[2].heads);
         VecPlan plan;
         if (!vec_plan(a, kInter, plan)) {
-            rotary_rows_kernel<kInter, kFp8><<<groups(rows), kThreads, 0, stream>>>(a);
+            if (a.head_dim <= 2 * kWave)
+                rotary_rows_kernel<kInter, kFp8, 1><<<groups(rows), kThreads, 0, stream>>>(a);
+            else
+                rotary_rows_kernel<kInter, kFp8, kRotaryMaxHeadDim / 2 / kWave>
+                    <<<groups(rows), kThreads, 0, stream>>>(a);
             return;
         }
         const int64_t waves = static_cast<int64_t>(a.tokens) *

@@ -457,3 +457,37 @@ def test_on_a_side_stream_and_in_a_replayed_graph(gpu):
         table.fill_(7.0)
         graph.replay()
         same(results())
+
+
+# ---- every width -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,widths", [(16, range(2, 18, 2)), (18, range(2, 20, 2)),
+                                      (128, (2, 14, 16, 18, 110, 112, 118, 120, 122, 124, 126)),
+                                      (64, (6, 12, 34, 48, 50, 56, 58, 62)), (14, (2, 8, 14)),
+                                      (1024, (1002, 1000, 16, 1022)), (1008, (990,))])
+def test_every_width(gpu, d, widths, interleaved):
+    # parts of a head shorter than a segment of eight, and parts that end inside one; in place
+    # and beside, with the norm into both kinds of cache
+    t, hq, hkv = 9, 3, 2
+    for rotary in widths:
+        say(f"width {d} {rotary} {interleaved}")
+        q, k, pos, tab = make_rotary(gpu, d + rotary, t, hq, hkv, d, rotary)
+        q[5], k[6] = math.inf, math.nan  # stay in their rows
+        q[7, 1, rotary - 1] = math.inf   # stays in its pair
+        table = torch.from_numpy(tab).to(gpu)
+        with np.errstate(invalid="ignore"):
+            wq, sq = R.rotate(f64(q), pos, tab, interleaved)
+        qo, ko = cc.rotary_embedding(q, k, i32(pos, gpu), table, interleaved)
+        for row in range(t):
+            if row not in (5, 7):
+                R.assert_bf16(f64(qo)[row], wq[row], sq[row], f"q row {row}")
+        assert np.array_equal(np.isfinite(f64(qo)[7]), np.isfinite(wq[7]))
+        assert np.array_equal(bits(qo)[..., rotary:], bits(q)[..., rotary:])
+        cc.rotary_embedding(q, k, i32(pos, gpu), table, interleaved, q_out=q, k_out=k)
+        assert np.array_equal(bits(q), bits(qo)) and np.array_equal(bits(k), bits(ko))
+        for fp8 in (False, True):
+            s = make_norm(gpu, d + rotary, t, hq, hkv, d, rotary, fp8)
+            before = snap(s)
+            q2 = run_norm(s, gpu, hq, interleaved=interleaved)
+            check_norm(s, q2, hq, hkv, d, interleaved, 1e-6, 0.0, before, fp8)
