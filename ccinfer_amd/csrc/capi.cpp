@@ -284,7 +284,7 @@ bool kv_layers_of(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
     const bool fp8 = k_scale != nullptr;
     if (fp8 && cache_block_size != kFp8Block) return false;
     const int64_t token = static_cast<int64_t>(n_kv_heads) * head_dim * (fp8 ? 1 : 2);
-    if (!fits_int(token) || !fits_int(token * cache_block_size) ||
+    if (!fits_int(token) || token * cache_block_size > (1 << 30) ||
         !fits_int(static_cast<int64_t>(num_blocks) * cache_block_size))
         return false;
     // layers one after the other: none begins inside another one
@@ -816,7 +816,7 @@ int ccinfer_copy_kv_blocks(void* k_cache, void* v_cache, float* k_scale, float* 
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (num_pairs < 0 || (num_pairs > 0 && (!src_blocks || !dst_blocks)))
         return CCINFER_ERR_INVALID_ARGUMENT;
-    if (num_pairs > kPagesMaxBlocks - 1) return CCINFER_ERR_UNSUPPORTED;
+    if (num_pairs > kPagesMaxPairs) return CCINFER_ERR_UNSUPPORTED;
     if (num_pairs == 0) return CCINFER_OK;
     return map_hip_error(
         copy_kv_blocks(kv, src_blocks, dst_blocks, num_pairs, status, as_stream(stream)));

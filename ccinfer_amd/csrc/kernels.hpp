@@ -283,10 +283,11 @@ struct KvLayers {
     int64_t block_bytes() const { return token_bytes * block_size; }
 };
 
-// Blocks that the bitmap of free blocks covers at most (and one more than a copy's pairs).
+// Blocks that the bitmap of free blocks covers at most.
 constexpr int kPagesMaxBlocks = 1 << 24;
-// Items of a table update at most (a workgroup each; a launch holds 2^32 work-items).
-constexpr int kPagesMaxItems = 1 << 20;
+// Items of a table update, and pairs of a copy, at most: each is compared with every other one.
+constexpr int kPagesMaxItems = 1 << 14;
+constexpr int kPagesMaxPairs = 1 << 17;
 
 hipError_t copy_kv_blocks(const KvLayers& kv, const int32_t* src, const int32_t* dst, int pairs,
                           int32_t* status, hipStream_t stream);

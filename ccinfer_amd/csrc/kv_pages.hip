@@ -300,9 +300,8 @@ __device__ __forceinline__ void select_free(const uint64_t* __restrict__ bitmap,
 
 // ---- update ------------------------------------------------------------------
 
-// What the first launch says of an item.
+// What the first launch says of an item that can be done.
 struct ItemPlan {
-    int32_t status;
     int32_t need;    // blocks from the pool
     int32_t shared;  // leading blocks that are the source row's
     int32_t total;   // blocks of the new row
@@ -315,6 +314,7 @@ struct ItemPlan {
 struct UpdateWorkspace {
     uint64_t* bitmap;
     int32_t* counts;
+    int32_t* needs;  // blocks that an item needs, or the status that it fails with, negated
     ItemPlan* plans;
     int32_t* staged;  // [items][width]: the blocks that the new row takes from the source row
 };
@@ -329,11 +329,13 @@ size_t update_layout(int items, int width, int blocks, char* ws, UpdateWorkspace
     };
     char* bitmap = take(static_cast<size_t>(chunks) * kChunkWords * sizeof(uint64_t));
     char* counts = take(static_cast<size_t>(chunks) * sizeof(int32_t));
+    char* needs = take(static_cast<size_t>(items) * sizeof(int32_t));
     char* plans = take(static_cast<size_t>(items) * sizeof(ItemPlan));
     char* staged = take(static_cast<size_t>(items) * width * sizeof(int32_t));
     if (out != nullptr)
         *out = {reinterpret_cast<uint64_t*>(bitmap), reinterpret_cast<int32_t*>(counts),
-                reinterpret_cast<ItemPlan*>(plans), reinterpret_cast<int32_t*>(staged)};
+                reinterpret_cast<int32_t*>(needs), reinterpret_cast<ItemPlan*>(plans),
+                reinterpret_cast<int32_t*>(staged)};
     return at;
 }
 
@@ -361,17 +363,15 @@ __global__ __launch_bounds__(kThreads) void update_plan_kernel(TableUpdate u, Kv
     for (int j = threadIdx.x; j < u.items; j += kThreads) bad |= j != i && u.dst[j] == d;
     ItemPlan p{};
     p.from = -1;
-    if (__syncthreads_or(bad)) {
-        p.status = kInvalidArgument;
-        if (threadIdx.x == 0) ws.plans[i] = p;
-        return;
-    }
+    auto tell = [&](int status) {
+        if (threadIdx.x == 0) {
+            ws.needs[i] = status == kOk ? p.need : -status;
+            ws.plans[i] = p;
+        }
+    };
+    if (__syncthreads_or(bad)) return tell(kInvalidArgument);
     const int have = s < 0 ? 0 : src_ctx;
-    if (have < 0 || have > most || old < 0 || old > most) {
-        p.status = kInvalidTable;
-        if (threadIdx.x == 0) ws.plans[i] = p;
-        return;
-    }
+    if (have < 0 || have > most || old < 0 || old > most) return tell(kInvalidTable);
     p.length = asked < 0 ? have : asked;
     const int kept = min(p.length, have);
     const int known = (kept + bs - 1) / bs;
@@ -387,18 +387,14 @@ __global__ __launch_bounds__(kThreads) void update_plan_kernel(TableUpdate u, Kv
     }
     for (int j = threadIdx.x; j < p.held; j += kThreads)
         bad |= !good(j < kThreads ? dst_entry : dst_row[j]);
-    if (__syncthreads_or(bad)) {
-        p.status = kInvalidTable;
-    } else {
-        const int last = known > 0 ? src_row[known - 1] : -1;
-        // a block that is filled in part goes on being written: it may have one owner only
-        const bool copied = p.part > 0 && (s != d || u.refs[last] > 1);
-        p.shared = known - (copied ? 1 : 0);
-        p.need = p.total - p.shared;
-        p.from = copied ? last : -1;
-        if (copied && kv.layers == 0) p.status = kInvalidArgument;
-    }
-    if (threadIdx.x == 0) ws.plans[i] = p;
+    if (__syncthreads_or(bad)) return tell(kInvalidTable);
+    const int last = known > 0 ? src_row[known - 1] : -1;
+    // a block that is filled in part goes on being written: it may have one owner only
+    const bool copied = p.part > 0 && (s != d || u.refs[last] > 1);
+    p.shared = known - (copied ? 1 : 0);
+    p.need = p.total - p.shared;
+    p.from = copied ? last : -1;
+    tell(copied && kv.layers == 0 ? kInvalidArgument : kOk);
 }
 
 // Workgroup (i, y): y = 0 changes the table row and the counts of item i; every y copies its
@@ -414,17 +410,18 @@ __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, K
     ItemPlan p{};
     p.from = -1;
     if (i < u.items) p = ws.plans[i];
+    if (blockIdx.y > 0 && p.from < 0) return;
     uint64_t word = 0;
     if (kSmall && tid < chunks * kChunkWords) word = ws.bitmap[tid];
     // sums over the items and the pool: blocks asked for, those of the items before this one,
     // free ones, items of each failure
     int v[5] = {}, all[5];
     for (int j = tid; j < u.items; j += kThreads) {
-        const ItemPlan q = ws.plans[j];
-        v[0] += q.need;
-        v[1] += j < i ? q.need : 0;
-        v[3] += q.status == kInvalidArgument;
-        v[4] += q.status == kInvalidTable;
+        const int need = ws.needs[j];
+        v[0] += max(need, 0);
+        v[1] += j < i ? max(need, 0) : 0;
+        v[3] += need == -kInvalidArgument;
+        v[4] += need == -kInvalidTable;
     }
     if constexpr (kSmall) {
         v[2] = __popcll(word);
@@ -433,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, K
     }
     PartCopy<T> ahead;
     const int parts = 2 * kv.layers;
-    const bool copies = p.from >= 0 && static_cast<int>(blockIdx.y) < parts;
+    const bool copies = p.from >= 0;  // then there are as many parts as workgroups, or more
     if (copies) ahead.start(kv, blockIdx.y, p.from, p.part);
     group_exclusive(v, all);
     const int status = all[3] > 0   ? kInvalidArgument
@@ -677,8 +674,11 @@ hipError_t update_block_tables(const TableUpdate& u, const KvLayers& kv, void* w
         u, kv, kv.blocks, chunks, ws);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    const dim3 grid(static_cast<unsigned>(std::max(1, u.items)),
-                    static_cast<unsigned>(std::max(1, 2 * kv.layers)));
+    // Workgroups of an item share its parts: as many as there are parts where the items are few,
+    // and one where they are so many that they fill the chip themselves.
+    const int items = std::max(1, u.items);
+    const int split = std::max(1, std::min(2 * kv.layers, (4096 + items - 1) / items));
+    const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(split));
     return with_unit(kv, [&](auto unit) {
         using T = decltype(unit);
         if (chunks * kChunkWords <= kThreads)

@@ -146,22 +146,26 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
 // one chunk a lane, two segments of eight elements:
 //   split chunk       pairs p .. p + 7 of the half layout: elements p .. and R/2 + p ..
 //   tail chunk        two segments of the elements from R on (half layout)
-//   contiguous chunk  elements e .. e + 15: interleaved rows, v rows
-// so both elements of every pair are in one lane in either layout. A wavefront holds 64 / G rows
+//   other rows        two segments of the row: interleaved ones, with their pairs inside, and v
+// so both elements of every pair are in one lane in either layout, and the lanes' first (and
+// second) segments lie side by side: a load or store takes whole lines. A wavefront holds 64 / G rows
 // of one section of one token, and all its loads are on their way before the first is needed.
 // Where a length is no multiple of its chunk or segment, the last one is moved back to end with
 // it: its first elements are another lane's too, which counts them in the sum of squares and
 // writes the same values. Only where fewer than eight pairs are rotated, or fewer than eight
 // elements are not, does a segment reach into elements that are treated otherwise; they are left
-// out and stored one by one. kWhole: R and the head are multiples of sixteen, so there is
-// nothing of this. Segments start at any even byte; the loads and stores claim 2-byte alignment,
+// out and stored one by one. kWhole: the head is a multiple of sixteen and R of sixteen
+// (interleaved: eight), so there is nothing of this. Segments start at any even byte; the loads and stores claim 2-byte alignment,
 // which the hardware takes at full width.
 //
-// Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 40.0 us with the
-// norm and the cache write, 5.2 TB/s, and a copy of as many bytes 41.1; 8191 tokens x 40 heads
-// half rotated 32.9 us. What that took: eight wavefronts a SIMD (60 registers; at five, with two
-// rows a lane sharing (cos, sin) and weights, 46.8 us) and stores with the streaming hint (41.5
-// without; a prefill that reads the rows afterwards takes the same time either way).
+// Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 38.4 us with the
+// norm and the cache write, 5.4 TB/s, and a copy of as many bytes 41.1; 8191 tokens x 40 heads
+// half rotated 31.0 us. What that took: eight wavefronts a SIMD (63 registers; at five, with two
+// rows a lane sharing (cos, sin) and weights, 46.8 us), stores with the streaming hint (41.5
+// without; a prefill that reads the rows afterwards takes the same time either way), and whole
+// lines a store (a lane's two segments side by side instead: 28 % more bytes written where they
+// are streamed). A half-layout row rotated in 50 or 120 of 128 elements takes nine lanes, so a
+// wavefront holds four rows instead of eight: 47 us instead of 32 (one wavefront a row: 124).
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
@@ -237,18 +241,18 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
             lo_a = lo_b = chunk * kSegment - seg_a;
             hi = min(kSegment, half);
             others = half < kSegment;
-        } else if (s < 2 && plan.split > 0) {
-            const int ua = a.rotary_dim + (chunk - plan.split) * kChunkElems, ub = ua + kSegment;
-            seg_a = min(ua, a.head_dim - kSegment);
-            lo_a = ua - seg_a;
-            seg_b = ub < a.head_dim ? min(ub, a.head_dim - kSegment) : seg_a;
-            lo_b = ub < a.head_dim ? ub - seg_b : kSegment;
-            others = a.head_dim - a.rotary_dim < kSegment;
         } else {
-            seg_a = min(chunk * kChunkElems, a.head_dim - kChunkElems);
-            seg_b = seg_a + kSegment;
-            lo_a = min(chunk * kChunkElems - seg_a, kSegment);
-            lo_b = max(chunk * kChunkElems - seg_b, 0);
+            const bool tail = s < 2 && plan.split > 0;
+            const int n = tail ? chunks - plan.split : chunks;
+            const int ua = tail ? a.rotary_dim + (chunk - plan.split) * kSegment
+                                : chunk * kSegment;
+            const int ub = ua + n * kSegment;
+            const bool two = ub < a.head_dim;
+            seg_a = min(ua, a.head_dim - kSegment);
+            seg_b = two ? min(ub, a.head_dim - kSegment) : seg_a;
+            lo_a = ua - seg_a;
+            lo_b = two ? ub - seg_b : kSegment;
+            others = tail && a.head_dim - a.rotary_dim < kSegment;
         }
         auto mine = [&](int i) {
             return i < kSegment ? i >= lo_a && i < hi
@@ -270,25 +274,35 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         if (c.rotate) {
             if (pos >= 0 && pos < a.rope_max) {
                 const float2* table = a.rope_cache + static_cast<int64_t>(pos) * half;
-                const int p0 = split ? seg_a : seg_a / 2;
-                // all of a half-layout chunk's pairs are rotated, or none
-                if (kWhole || (!kInterleaved && half >= kSegment)) {
-                    const bool in = split || (kInterleaved && p0 < half);
-                    turn = in ? 0xffu : 0u;
-                    const float2* from = table + (in ? p0 : 0);
+                auto load_pairs = [&](int i0, int n, int first) {  // n pairs from `first` on
 #pragma unroll
                     for (int i = 0; i < kSegment / 2; ++i) {
-                        const f32x4 v = reinterpret_cast<const f32x4_a8*>(from)[i];
+                        if (2 * i < i0 || 2 * i >= i0 + n) continue;
+                        const f32x4 v =
+                            *reinterpret_cast<const f32x4_a8*>(table + first + 2 * i - i0);
                         cs[2 * i] = v[0], sn[2 * i] = v[1];
                         cs[2 * i + 1] = v[2], sn[2 * i + 1] = v[3];
                     }
-                } else {
-                    const bool in = split || kInterleaved;
+                };
+                if (!kInterleaved && (kWhole || half >= kSegment)) {
+                    // all of a chunk's pairs are rotated, or none
+                    turn = split ? 0xffu : 0u;
+                    load_pairs(0, kSegment, split ? seg_a : 0);
+                } else if (kWhole) {
+                    // all of a segment's four pairs, or none
+                    const int pa = seg_a / 2, pb = seg_b / 2;
+                    turn = (pa < half ? 0x0fu : 0u) | (pb < half ? 0xf0u : 0u);
+                    load_pairs(0, kSegment / 2, pa < half ? pa : 0);
+                    load_pairs(kSegment / 2, kSegment / 2, pb < half ? pb : 0);
+                } else if (split || kInterleaved) {
 #pragma unroll
                     for (int i = 0; i < kSegment; ++i) {
-                        const float2 v = table[min(p0 + i, half - 1)];
+                        const int p = split            ? i
+                                      : i < kSegment / 2 ? seg_a / 2 + i
+                                                         : seg_b / 2 + i - kSegment / 2;
+                        const float2 v = table[min(p, half - 1)];
                         cs[i] = v.x, sn[i] = v.y;
-                        turn |= in && p0 + i < half ? 1u << i : 0u;
+                        turn |= p < half ? 1u << i : 0u;
                     }
                 }
             }
@@ -329,9 +343,11 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         }
         // under a branch or a select, so that nothing of a pair that is not rotated meets
         // another one's infinity
-        if (turn != 0) {
 #pragma unroll
-            for (int i = 0; i < kSegment; ++i) {
+        for (int g = 0; g < 2; ++g) {  // four pairs at a time
+            if ((turn >> (4 * g) & 0xfu) == 0) continue;
+#pragma unroll
+            for (int i = 4 * g; i < 4 * g + 4; ++i) {
                 const int p = kInterleaved ? 2 * i : i;
                 const int q = kInterleaved ? 2 * i + 1 : kSegment + i;
                 const float u0 = x[p] * cs[i] - x[q] * sn[i];
@@ -404,7 +420,7 @@ bool vec_plan(const RotaryArgs& a, bool interleaved, VecPlan& plan) {
     if (most > kWave) return false;
     plan.lanes = 1;
     while (plan.lanes < most) plan.lanes *= 2;
-    plan.whole = r % kChunkElems == 0 && d % kChunkElems == 0;
+    plan.whole = r % (interleaved ? kSegment : kChunkElems) == 0 && d % kChunkElems == 0;
     for (int s = 0; s < 3; ++s) plan.units[s] = up(a.sec[s].heads, kWave / plan.lanes);
     return true;
 }

@@ -52,7 +52,7 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
         nb, bs = (shape[0], shape[1]) if dims == 4 else (shape[0] // block_size, block_size)
         _require((dims == 4 or nb * bs == shape[0]) and k_cache.is_contiguous()
                  and v_cache.is_contiguous(), op)
-    _require(bs == block_size, op)
+    _require(bs == block_size and nb < 2 ** 31, op)
     ksp = vsp = None
     if fp8:
         need = nb * h * 16

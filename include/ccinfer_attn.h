@@ -364,7 +364,7 @@ int ccinfer_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_he
  * [num_q_heads][head_dim], K and V to their slots of a bf16 cache, or, with k_scale and
  * v_scale, of an fp8 cache (layout and quantisation of ccinfer_write_kv_cache_fp8, straight
  * from the float32 rows; a NaN is stored as E4M3's). qkv rows lie qkv_token_stride elements
- * apart. Tokens whose slot is outside [0, max_slots) write no K/V; no two tokens may have the
+ * apart; q_out and the caches lie apart from them. Tokens whose slot is outside [0, max_slots) write no K/V; no two tokens may have the
  * same slot. */
 int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void* q_norm_weight,
                           int q_norm_per_head, const void* k_norm_weight, int k_norm_per_head,
@@ -379,11 +379,13 @@ int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void*
  * Operators on the pool of blocks of all layers at once. k_cache / v_cache: layer 0 of
  * [num_layers][num_blocks][cache_block_size][n_kv_heads][head_dim], bf16, or fp8 bytes with
  * k_scale / v_scale; layer_stride in bytes and scale_layer_stride in floats lead from one
- * layer to the next (unused for one layer). An fp8 cache has cache_block_size 16.
+ * layer to the next (unused for one layer). A block of one layer's K has at most 2^30 bytes;
+ * an fp8 cache has cache_block_size 16. The scales of an fp8 cache start as zeros (or anything
+ * finite): the attention multiplies those of a block's slots that hold no token by 0.
  *
  * ref_counts [num_blocks] says how many table rows (or other owners, a prefix cache say) hold
- * a block; 0 is free. At most 2^24 blocks (CCINFER_ERR_UNSUPPORTED past that) for the calls
- * that take counts. */
+ * a block; 0 is free. CCINFER_ERR_UNSUPPORTED for more than 2^24 blocks in the calls that take
+ * counts, 2^14 items of an update and 2^17 pairs of a copy. */
 
 /* Block dst_blocks[i] becomes a copy of src_blocks[i] in every layer, K, V and scales. Pairs
  * with a block outside [0, num_blocks), and of a block with itself, are skipped. Pairs that

@@ -392,3 +392,20 @@ def test_update_and_compact_in_replayed_graphs(gpu):
             assert torch.equal(u, w)
         assert all(np.array_equal(u, w) for u, w in zip(p.flat(), e.flat()))
         P.consistent(y.dt.cpu().numpy(), y.dc.cpu().numpy(), y.dr.cpu().numpy(), 16)
+
+
+# ---- many items ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,fp8", [(300, False), (1500, True), (5000, False)])
+def test_update_of_many_rows(gpu, rows, fp8):
+    # more items than a workgroup has lanes, and more than leave one workgroup for each part
+    say(f"update {rows} rows {fp8}")
+    p = Pool(gpu, 50, 3, 4 * rows, 1, 32, fp8=fp8)
+    rng = np.random.default_rng(rows)
+    x = Tables(gpu, rows, 3, p.blocks)
+    some = rng.permutation(rows)[:rows // 2]
+    assert x.step(p, some, np.full(len(some), -1), rng.integers(1, 20, len(some))) == 0
+    rest = np.setdiff1d(np.arange(rows), some)
+    assert x.step(p, rest, rng.choice(some, len(rest)), None) == 0      # forks
+    assert x.step(p, np.arange(rows), None, x.c + 1) == 0               # a step of every row
+    assert x.step(p, rng.permutation(rows), rng.integers(-1, rows, rows), None) == 0  # all change

@@ -491,3 +491,27 @@ def test_every_width(gpu, d, widths, interleaved):
             before = snap(s)
             q2 = run_norm(s, gpu, hq, interleaved=interleaved)
             check_norm(s, q2, hq, hkv, d, interleaved, 1e-6, 0.0, before, fp8)
+
+
+def test_tensors_of_another_device_are_refused(gpu, monkeypatch):
+    say("other device")
+    from ccinfer_amd import pages, rope
+    s = make_norm(gpu, 3, 4, 4, 2, 64, 64, False)
+    table, pos = torch.from_numpy(s["tab"]).to(gpu), i32(s["pos"], gpu)
+    k = s["k"].view(-1, 16, 2, 64)
+    counts = torch.zeros(len(k), dtype=torch.int32, device=gpu)
+    rows = torch.full((2, 3), -1, dtype=torch.int32, device=gpu)
+    calls = [lambda: cc.build_rope_cache(len(table), 64, out=table),
+             lambda: cc.rotary_embedding(k[0, :4], None, pos, table),
+             lambda: run_norm(s, gpu, 4),
+             lambda: cc.copy_kv_blocks(k, k, counts[:1], counts[:1]),
+             lambda: cc.update_block_tables(rows, counts[:2], counts, counts[:0], None, None),
+             lambda: cc.compact_kv_blocks(rows, counts, k, k)]
+    for call in calls:
+        call()
+    for module in (rope, pages):
+        monkeypatch.setattr(module, "current_device", lambda: 1)
+    for i, call in enumerate(calls):
+        with pytest.raises(cc.CcinferError) as e:
+            call()
+        assert e.value.code == 6, i

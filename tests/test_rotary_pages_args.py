@@ -148,8 +148,11 @@ def test_copy_refusals(lib):
         a[i] = bad
         assert fn(*a) == INVALID, (i, bad)
     a = list(ok)
-    a[6] = 1 << 24
+    a[6] = (1 << 17) + 1
     assert fn(*a) == UNSUPPORTED
+    a = list(ok)
+    a[7], a[10], a[11], a[12], a[13] = 1, 1, 4096, 256, 1024  # a block past 2^30 bytes
+    assert fn(*a) == INVALID
     fp8 = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 4, 3, layer // 2, 64 * 8 * 16, 64, 8, 128, 16, None,
            None]
     for i, bad in [(9, 64 * 8 * 16 - 1), (13, 32), (8, layer // 2 - 1)]:
@@ -179,7 +182,11 @@ def test_update_refusals(lib):
     a[16] = (1 << 24) + 1  # blocks past the bitmap
     a[22] = 1 << 40
     assert fn(*a) == UNSUPPORTED
+    a = list(ok)
+    a[6], a[22] = (1 << 14) + 1, 1 << 40
+    assert fn(*a) == UNSUPPORTED
     assert lib.ccinfer_update_tables_workspace_size(4, 32, (1 << 24) + 1) == 0
+    assert lib.ccinfer_update_tables_workspace_size((1 << 14) + 1, 32, 64) == 0
     for bad in [(-1, 32, 64), (4, 0, 64), (4, 32, 0), (1 << 19, 1 << 13, 64)]:
         assert lib.ccinfer_update_tables_workspace_size(*bad) == 0, bad
 
