@@ -148,15 +148,16 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
 //   tail chunk        two segments of the elements from R on (half layout)
 //   other rows        two segments of the row: interleaved ones, with their pairs inside, and v
 // so both elements of every pair are in one lane in either layout, and the lanes' first (and
-// second) segments lie side by side: a load or store takes whole lines. A wavefront holds 64 / G rows
-// of one section of one token, and all its loads are on their way before the first is needed.
-// Where a length is no multiple of its chunk or segment, the last one is moved back to end with
-// it: its first elements are another lane's too, which counts them in the sum of squares and
-// writes the same values. Only where fewer than eight pairs are rotated, or fewer than eight
-// elements are not, does a segment reach into elements that are treated otherwise; they are left
-// out and stored one by one. kWhole: the head is a multiple of sixteen and R of sixteen
-// (interleaved: eight), so there is nothing of this. Segments start at any even byte; the loads and stores claim 2-byte alignment,
-// which the hardware takes at full width.
+// second) segments lie side by side: a load or store takes whole lines. A wavefront holds 64 / G
+// rows of one section of one token, and all its loads are on their way before the first is
+// needed; no row is split between wavefronts, so a call may write where it reads. Where a length
+// is no multiple of its segment, the last one is moved back to end with it: its first elements
+// are another lane's too, which counts them in the sum of squares and writes the same values.
+// Only where fewer than eight pairs are rotated, or fewer than eight elements are not, does a
+// segment reach into elements that are treated otherwise; they are left out, and the rest is
+// stored element by element. kWhole: the head is a multiple of sixteen and R of sixteen
+// (interleaved: eight), so there is nothing of this. Segments start at any even byte; the loads
+// and stores claim 2-byte alignment, which the hardware takes at full width.
 //
 // Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 38.4 us with the
 // norm and the cache write, 5.4 TB/s, and a copy of as many bytes 41.1; 8191 tokens x 40 heads
@@ -205,7 +206,7 @@ struct VecPlan {
     int chunks;       // chunks of a q or k row
     int plain;        // chunks of a v row
     int units[3];     // wavefronts of a section and token
-    bool whole;       // no segment was moved back, and no interleaved chunk crosses R
+    bool whole;       // no segment was moved back, and none crosses R
 };
 
 template <bool kInterleaved, bool kFp8, bool kWhole>

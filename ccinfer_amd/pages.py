@@ -23,6 +23,8 @@ from . import _lib
 from .ops import (INVALID_ARGUMENT, CcinferError, _check, _require, _stream, _workspace,
                   current_device)
 
+_I32 = torch.int32
+
 KV_EXHAUSTED = 12      # status: not enough free blocks
 KV_INVALID_TABLE = 14  # status: a table row that the pool does not hold
 
@@ -45,14 +47,14 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
         layer_stride = stride[0] * (1 if fp8 else 2)
         vstride = v_cache.stride()
         inner = (bs * h * d, h * d, d, 1)
-        _require((layers == 1 or vstride[0] == stride[0])
+        _require((stride == vstride or layers == 1 or vstride[0] == stride[0])
                  and (stride[1:] == inner or k_cache[0].is_contiguous())
-                 and (vstride[1:] == inner or v_cache[0].is_contiguous()), op)
+                 and (vstride[1:] == inner or v_cache[0].is_contiguous())
+                 and bs == block_size and nb < 2 ** 31, op)
     else:
         nb, bs = (shape[0], shape[1]) if dims == 4 else (shape[0] // block_size, block_size)
         _require((dims == 4 or nb * bs == shape[0]) and k_cache.is_contiguous()
-                 and v_cache.is_contiguous(), op)
-    _require(bs == block_size and nb < 2 ** 31, op)
+                 and v_cache.is_contiguous() and bs == block_size and nb < 2 ** 31, op)
     ksp = vsp = None
     if fp8:
         need = nb * h * 16
@@ -71,7 +73,7 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
 
 def _index(t: torch.Tensor, dev: int, op: str) -> int:
     """Elements of a contiguous int32 tensor on the device."""
-    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous():
         raise CcinferError(INVALID_ARGUMENT, op)
     return t.numel()
 
@@ -91,11 +93,12 @@ def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: tor
     n = _index(src_blocks, dev, op)
     _require(_index(dst_blocks, dev, op) == n
              and (status is None or _index(status, dev, op) == 1), op)
-    kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
-        k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
-    _check(_lib.load().ccinfer_copy_kv_blocks(
-        kp, vp, ksp, vsp, src_blocks.data_ptr() or None, dst_blocks.data_ptr() or None, n, layers,
-        ls, ss, nb, h, d, bs, None if status is None else status.data_ptr(), _stream()), op)
+    cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+    code = _lib.load().ccinfer_copy_kv_blocks(
+        *cache[:4], src_blocks.data_ptr() or None, dst_blocks.data_ptr() or None, n, *cache[4:],
+        None if status is None else status.data_ptr(), _stream())
+    if code:
+        raise CcinferError(code, op)
 
 
 @lru_cache(maxsize=1024)
@@ -129,34 +132,36 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     op = "update_block_tables"
     _require(block_table.is_cuda, op)
     dev = current_device()
-    _index(block_table, dev, op)
-    n, nb = _index(dst_rows, dev, op), _index(ref_counts, dev, op)
-    shape = block_table.shape
-    _require(len(shape) == 2 and _index(context_lens, dev, op) == shape[0]
+    shape, n, nb = block_table.shape, dst_rows.numel(), ref_counts.numel()
+    _require(len(shape) == 2 and block_table.dtype is _I32 and context_lens.dtype is _I32
+             and ref_counts.dtype is _I32 and dst_rows.dtype is _I32
+             and block_table.get_device() == dev and context_lens.get_device() == dev
+             and ref_counts.get_device() == dev and dst_rows.get_device() == dev
+             and block_table.is_contiguous() and context_lens.is_contiguous()
+             and ref_counts.is_contiguous() and dst_rows.is_contiguous()
+             and context_lens.numel() == shape[0]
              and (src_rows is None or _index(src_rows, dev, op) == n)
              and (lengths is None or _index(lengths, dev, op) == n)
              and (status is None or _index(status, dev, op) == 1), op)
     rows, width = shape
     if status is None:
-        status = torch.empty(1, dtype=torch.int32, device=block_table.device)
+        status = torch.empty(1, dtype=_I32, device=block_table.device)
     if k_cache is None:
         _require(v_cache is None and k_scale is None and v_scale is None, op)
-        kp = vp = ksp = vsp = None
-        layers = ls = ss = h = d = 0
-        bs = cache_block_size
+        cache = (None, None, None, None, 0, 0, 0, nb, 0, 0, cache_block_size)
     else:
         _require(v_cache is not None, op)
-        kp, vp, ksp, vsp, layers, ls, ss, cache_blocks, h, d, bs = _layers(
-            k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
-        _require(cache_blocks == nb, op)
+        cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+        _require(cache[7] == nb, op)
     ws, ws_bytes = _workspace(update_tables_workspace_size(n, width, nb), block_table.device,
                               workspace)
-    _check(_lib.load().ccinfer_update_block_tables(
+    code = _lib.load().ccinfer_update_block_tables(
         block_table.data_ptr(), context_lens.data_ptr(), ref_counts.data_ptr(),
         dst_rows.data_ptr() or None, None if src_rows is None else src_rows.data_ptr() or None,
-        None if lengths is None else lengths.data_ptr() or None, n, rows, width, kp, vp, ksp, vsp,
-        layers, ls, ss, nb, h, d, bs, status.data_ptr(), None if ws is None else ws.data_ptr(),
-        ws_bytes, _stream()), op)
+        None if lengths is None else lengths.data_ptr() or None, n, rows, width, *cache,
+        status.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _stream())
+    if code:
+        raise CcinferError(code, op)
     return status
 
 
@@ -181,8 +186,8 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     _index(block_table, dev, op)
     _index(ref_counts, dev, op)
     _require(block_table.dim() == 2, op)
-    kp, vp, ksp, vsp, layers, ls, ss, nb, h, d, bs = _layers(
-        k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+    cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
+    nb = cache[7]
     _require(ref_counts.numel() == nb, op)
     if out is None:
         out = {"block_table": torch.empty_like(block_table),
@@ -196,7 +201,7 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     ws, ws_bytes = _workspace(compact_workspace_size(nb), block_table.device, workspace)
     rows, width = block_table.shape
     _check(_lib.load().ccinfer_compact_kv_blocks(
-        block_table.data_ptr() or None, ref_counts.data_ptr(), rows, width, kp, vp, ksp, vsp,
-        layers, ls, ss, nb, h, d, bs, table.data_ptr() or None, refs.data_ptr(), remap.data_ptr(),
-        live.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _stream()), op)
+        block_table.data_ptr() or None, ref_counts.data_ptr(), rows, width, *cache,
+        table.data_ptr() or None, refs.data_ptr(), remap.data_ptr(), live.data_ptr(),
+        None if ws is None else ws.data_ptr(), ws_bytes, _stream()), op)
     return out
