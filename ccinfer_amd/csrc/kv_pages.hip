@@ -389,8 +389,18 @@ __global__ __launch_bounds__(kThreads) void update_plan_kernel(TableUpdate u, Kv
         bad |= !good(j < kThreads ? dst_entry : dst_row[j]);
     if (__syncthreads_or(bad)) return tell(kInvalidTable);
     const int last = known > 0 ? src_row[known - 1] : -1;
-    // a block that is filled in part goes on being written: it may have one owner only
-    const bool copied = p.part > 0 && (s != d || u.refs[last] > 1);
+    // A block that is filled in part goes on being written: it may have one owner only. A row
+    // that is cut back into a block of its own leaves it to rows that take it over as a whole
+    // block in the same call.
+    bool taken = false;
+    if (p.part > 0 && s == d && u.src != nullptr && old >= known * bs) {
+        for (int j = threadIdx.x; j < u.items; j += kThreads) {
+            const int n = u.lengths != nullptr ? u.lengths[j] : -1;
+            taken |= u.src[j] == d && j != i && (n < 0 || n >= known * bs);
+        }
+        taken = __syncthreads_or(taken);
+    }
+    const bool copied = p.part > 0 && (s != d || u.refs[last] > 1 || taken);
     p.shared = known - (copied ? 1 : 0);
     p.need = p.total - p.shared;
     p.from = copied ? last : -1;
@@ -430,7 +440,7 @@ __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, K
     }
     PartCopy<T> ahead;
     const int parts = 2 * kv.layers;
-    const bool copies = p.from >= 0;  // then there are as many parts as workgroups, or more
+    const bool copies = p.from >= 0 && kv.layers > 0;  // parts: at least as many as workgroups
     if (copies) ahead.start(kv, blockIdx.y, p.from, p.part);
     group_exclusive(v, all);
     const int status = all[3] > 0   ? kInvalidArgument

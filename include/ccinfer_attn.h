@@ -410,8 +410,8 @@ size_t ccinfer_update_tables_workspace_size(int num_items, int max_blocks_per_re
  *   fork      (child, parent, -1)         admit    (row, -1, tokens)
  *   grow      (row, row, more tokens)     truncate (row, row, fewer tokens)
  *   release   (row, -1, 0)                beams    (row, the beam it goes on from, -1)
- * Whole blocks are shared. A last block that is filled in part has one owner: where it would
- * be shared, its tokens are copied to a block of the row's own. New blocks are the
+ * Whole blocks are shared. A last block that is filled in part has one owner: where it is
+ * shared, or would be, its tokens are copied to a block of the row's own. New blocks are the
  * lowest-numbered ones that were free before the call, in item order; what the call releases
  * is free after it. *status (on the device, always written): CCINFER_OK, or, with nothing
  * changed, CCINFER_ERR_INVALID_ARGUMENT (a row or length out of range, two items of one row,

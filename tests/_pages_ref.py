@@ -45,7 +45,10 @@ def update(table, ctx, refs, dst, src, lengths, caches, scales, bs, have_caches=
         if any(not (0 <= b < len(refs)) or refs[b] <= 0 for b in held + old):
             bad_table = True
             continue
-        copied = kept % bs != 0 and (s != d or refs[held[-1]] > 1)
+        # rows that take the last block over as a whole block of theirs in the same call
+        takers = [j for j in range(n) if src[j] == d and dst[j] != d
+                  and min(have, have if lengths[j] < 0 else lengths[j]) >= len(held) * bs]
+        copied = kept % bs != 0 and (s != d or refs[held[-1]] > 1 or bool(takers))
         if copied and not have_caches:
             invalid = True
         need.append((d, want, kept, held, old, copied))
@@ -99,10 +102,13 @@ def compact(table, refs, caches):
 
 
 def consistent(table, ctx, refs, bs):
-    """Every block that a row holds is counted once for each row that holds it."""
+    """Every block that a row holds is counted once for each row that holds it, and a block that
+    a row has filled in part is held by that row alone."""
     count = np.zeros_like(refs)
     for row, n in zip(table, ctx):
         held = row[:-(-int(n) // bs)]
         assert np.all(held >= 0) and np.all(row[len(held):] == -1)
         np.add.at(count, held, 1)
     assert np.array_equal(count, refs)
+    for row, n in zip(table, ctx):
+        assert n % bs == 0 or refs[row[int(n) // bs]] == 1

@@ -178,6 +178,25 @@ def test_update_each_use(gpu):
     assert x.step(p, [], [], []) == 0                          # nothing
 
 
+def test_row_cut_back_into_a_block_that_another_takes_over(gpu):
+    # row 0 ends inside block 1 from now on, while row 1 is forked from it with block 1 whole: one
+    # of them has to have its own
+    say("update cut and fork")
+    for fp8 in (False, True):
+        p = Pool(gpu, 12, 2, 32, 1, 64, fp8=fp8)
+        x = Tables(gpu, 4, 4, 32)
+        assert x.step(p, [0], [-1], [50]) == 0
+        assert x.step(p, [0, 1], [0, 0], [20, 50]) == 0
+        assert x.t[0, 1] != x.t[1, 1] and x.t[0, 0] == x.t[1, 0]
+        # the other fork ends in the block too: its tokens are copied, row 0 keeps the block
+        b = x.t[0, 1]
+        assert x.step(p, [2, 0], [0, 0], [18, 17]) == 0 and x.t[0, 1] == b != x.t[2, 1]
+        # ends before the block, or at its start
+        assert x.step(p, [2, 0, 3], [0, 0, 0], [7, 18, 16]) == 0 and x.t[0, 1] == b
+        assert x.step(p, [0, 2, 3], [1, 1, 1], [32, -1, 33]) == 0
+        assert x.step(p, [1, 0, 3], [1, 1, 1], [30, 32, 31]) == 0
+
+
 def test_update_refused_by_the_device_changes_nothing(gpu):
     say("update refused")
     p = Pool(gpu, 9, 2, 32, 1, 64)
