@@ -12,12 +12,13 @@
 // next term is under 2e-9 ((pi/4)^11 / 11!).
 //
 // The table is only written, so the rate of plain stores bounds it: 2^20 positions x 32 pairs
-// (268 MB) take 42.9 us, 6.3 TB/s, where a fill of 2 GiB reaches 6.9. Two pairs (16 bytes) a
-// store, streamed; the two-double-operation reduction keeps the arithmetic (about 27 operations
-// an entry) under the stores' time.
+// (268 MB) take 40.8 us, 6.6 TB/s, where a fill of 2 GiB reaches 6.9. Two entries (16 bytes) a
+// store, streamed; the reduction in three double operations keeps the arithmetic (about 27
+// operations an entry) under the stores' time.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -28,7 +29,7 @@ namespace ccinfer::hipk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSteps = 2;  // positions of a lane
+constexpr int kSteps = 2;
 
 // Frequencies in quarter turns a position, by value: the call needs no upload and can be
 // captured.
@@ -57,35 +58,49 @@ __device__ __forceinline__ float2 cos_sin_quarters(double n, double g, float m) 
 
 typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
 
-// A workgroup takes kSteps times `rows` positions; lane (row, column) the kPer pairs of its
-// column. Two steps share the frequencies' load; with one, 40960 x 64 pairs take 5.9 us instead
-// of 5.2, with eight 2^20 x 32 pairs 48.5 us instead of 42.9 (too few workgroups write at once).
-template <int kPer>
+constexpr int kGroupEntries = 2 * kThreads;  // entries that a workgroup stores at a time, 4 KiB
+constexpr int kMagicBits = 20;
+
+// The table as one run of entries: a workgroup takes kSteps times 4 KiB of it, a lane two
+// entries side by side, whatever the number of pairs. (By positions, a workgroup's share is no
+// multiple of a line at most widths, and its edges are written in two parts: 4.5 to 4.8 TB/s
+// instead of 6.3.) One step takes 44.6 us instead of 41.4 for 2^20 x 32 pairs, four 45.3.
+// `magic` is 2^20 / pairs rounded up: x * magic >> 20 is x / pairs for x < pairs + 512. The
+// workgroup's own division is on the scalar unit, in 32 bits where the table allows it (in 64
+// 42.4 us instead of 40.8).
 __global__ __launch_bounds__(kThreads) void rope_table_kernel(Quarters quarters, int pairs,
-                                                              int rows, int count, int first,
-                                                              float m, float2* __restrict__ out) {
-    const int columns = pairs / kPer;
-    const int row = threadIdx.x / columns;
-    if (row >= rows) return;
-    const int p = (threadIdx.x - row * columns) * kPer;
-    double g[kPer];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) g[k] = quarters.per_position[p + k];
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kSteps * rows;
-    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kSteps * rows + row; i0 < count;
-         i0 += step) {
+                                                              uint32_t magic,
+                                                              int64_t entries, int first, float m,
+                                                              float2* __restrict__ out) {
+    __shared__ double g[kRopeMaxPairs];
+    for (int p = threadIdx.x; p < pairs; p += kThreads) g[p] = quarters.per_position[p];
+    __syncthreads();
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kSteps * kGroupEntries;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kSteps * kGroupEntries; base < entries;
+         base += step) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-            const int64_t i = i0 + k * rows;
-            if (i >= count) break;
-            const double n = static_cast<double>(first + i);
-            float2* to = out + i * pairs + p;
-            if constexpr (kPer == 2) {
-                const float2 a = cos_sin_quarters(n, g[0], m), b = cos_sin_quarters(n, g[1], m);
+            const int64_t from = base + k * kGroupEntries;  // of the workgroup
+            const int row =
+                entries <= INT_MAX
+                    ? static_cast<int>(static_cast<uint32_t>(from) / static_cast<uint32_t>(pairs))
+                    : static_cast<int>(from / pairs);
+            const uint32_t x =
+                static_cast<uint32_t>(from - static_cast<int64_t>(row) * pairs) + 2 * threadIdx.x;
+            const int64_t e = from + 2 * threadIdx.x;
+            if (e >= entries) return;
+            const uint32_t q = x * magic >> kMagicBits;
+            const int p0 = static_cast<int>(x - q * pairs);
+            const bool wraps = p0 + 1 == pairs;
+            const int p1 = wraps ? 0 : p0 + 1;
+            const int n0 = first + row + static_cast<int>(q), n1 = n0 + (wraps ? 1 : 0);
+            const float2 a = cos_sin_quarters(static_cast<double>(n0), g[p0], m);
+            if (e + 1 < entries) {
+                const float2 b = cos_sin_quarters(static_cast<double>(n1), g[p1], m);
                 __builtin_nontemporal_store(f32x4{a.x, a.y, b.x, b.y},
-                                            reinterpret_cast<f32x4_a8*>(to));
+                                            reinterpret_cast<f32x4_a8*>(out + e));
             } else {
-                *to = cos_sin_quarters(n, g[0], m);
+                out[e] = a;
             }
         }
     }
@@ -175,18 +190,14 @@ hipError_t build_rope_cache(const double* freq, int pairs, double magnitude, int
                             void* out, hipStream_t stream) {
     Quarters quarters{};
     for (int p = 0; p < pairs; ++p) quarters.per_position[p] = freq[p] * (2.0 / M_PI);
-    const int rows = kThreads / (pairs % 2 == 0 ? pairs / 2 : pairs);
-    const int each = rows * kSteps;
-    const unsigned grid = static_cast<unsigned>(
-        std::min<int64_t>(1 << 22, (static_cast<int64_t>(count) + each - 1) / each));
-    auto* to = static_cast<float2*>(out);
-    const float m = static_cast<float>(magnitude);
-    if (pairs % 2 == 0)
-        rope_table_kernel<2><<<grid, kThreads, 0, stream>>>(quarters, pairs, rows, count, first, m,
-                                                            to);
-    else
-        rope_table_kernel<1><<<grid, kThreads, 0, stream>>>(quarters, pairs, rows, count, first, m,
-                                                            to);
+    const int64_t entries = static_cast<int64_t>(count) * pairs;
+    constexpr int64_t kEach = kSteps * kGroupEntries;
+    const unsigned grid =
+        static_cast<unsigned>(std::min<int64_t>(1 << 22, (entries + kEach - 1) / kEach));
+    const uint32_t magic = ((1u << kMagicBits) + pairs - 1) / pairs;
+    rope_table_kernel<<<grid, kThreads, 0, stream>>>(quarters, pairs, magic, entries, first,
+                                                     static_cast<float>(magnitude),
+                                                     static_cast<float2*>(out));
     return hipGetLastError();
 }
 

@@ -51,6 +51,22 @@ def test_table(gpu, positions, rotary, first, scaling):
     assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
 
 
+def test_table_of_more_than_2_31_entries(gpu):
+    say("table 2^31 entries")
+    count, rotary = (1 << 23) + 1, 512  # 17.2 GB
+    freq, _ = cc.rope_frequencies(rotary, 1e4)
+    out = torch.zeros(count, rotary // 2, 2, device=gpu)
+    cc.build_rope_cache(count, rotary, 1e4, out=out)
+    for n in (0, 1, (1 << 22) - 1, 1 << 22, (1 << 23) - 1, 1 << 23):
+        ang = np.longdouble(n) * np.array(freq, np.longdouble)
+        bound = np.abs(ang) * 2.0 ** -51 + 6 * 2.0 ** -24
+        got = f64(out[n])
+        assert np.all(np.abs(got[:, 0] - np.cos(ang)) <= bound)
+        assert np.all(np.abs(got[:, 1] - np.sin(ang)) <= bound)
+    length = out.view(-1, 2)[:: 9973].double().square().sum(-1)
+    assert (length - 1).abs().max().item() < 1e-5  # every entry sampled is a point of the circle
+
+
 def test_table_quarter_turns(gpu):
     # frequencies of exactly 1 (pair 0): position n is n radians; signs over all quadrants
     got = f64(cc.build_rope_cache(64, 2, 1e4))
