@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
         rotary_row<kInterleaved, kFp8, kSteps>(a, row);
 }
 
-// The kernel for heads of sixteen elements or more. A row is held by G lanes (a power of two),
+// The kernel for heads of sixteen elements or more. A row is held by G lanes,
 // one chunk a lane, two segments of eight elements:
 //   split chunk       pairs p .. p + 7 of the half layout: elements p .. and R/2 + p ..
 //   tail chunk        two segments of the elements from R on (half layout)
@@ -166,7 +166,8 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
 // without; a prefill that reads the rows afterwards takes the same time either way), and whole
 // lines a store (a lane's two segments side by side instead: 28 % more bytes written where they
 // are streamed). A half-layout row rotated in 50 or 120 of 128 elements takes nine lanes, so a
-// wavefront holds four rows instead of eight: 47 us instead of 32 (one wavefront a row: 124).
+// wavefront holds seven rows instead of eight, and loads in parts of lines: 40 us instead of 32
+// (one wavefront a row: 124).
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
@@ -180,16 +181,22 @@ __device__ __forceinline__ float dpp(float v) {
         __builtin_amdgcn_update_dpp(0, __float_as_int(v), Ctrl, 0xf, 0xf, true));
 }
 
-// op over groups of `lanes` (a power of two, the same for all) lanes; every lane gets the result.
+// op over the `lanes` lanes that hold a row, the same ones' order in each, so that every lane gets
+// the same bits: pairs of lanes where they are a power of two, else one after the other.
 template <typename Op>
-__device__ __forceinline__ float group_reduce(float v, int lanes, Op op) {
-    if (lanes > 1) v = op(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
-    if (lanes > 2) v = op(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
-    if (lanes > 4) v = op(v, dpp<0x141>(v));  // row_half_mirror: the other quad of eight
-    if (lanes > 8) v = op(v, dpp<0x140>(v));  // row_mirror: the other eight of sixteen
-    if (lanes > 16) v = op(v, __shfl_xor(v, 16, 64));
-    if (lanes > 32) v = op(v, __shfl_xor(v, 32, 64));
-    return v;
+__device__ __forceinline__ float row_reduce(float v, int lanes, bool power, int first, Op op) {
+    if (power) {
+        if (lanes > 1) v = op(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
+        if (lanes > 2) v = op(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
+        if (lanes > 4) v = op(v, dpp<0x141>(v));  // row_half_mirror: the other quad of eight
+        if (lanes > 8) v = op(v, dpp<0x140>(v));  // row_mirror: the other eight of sixteen
+        if (lanes > 16) v = op(v, __shfl_xor(v, 16, 64));
+        if (lanes > 32) v = op(v, __shfl_xor(v, 32, 64));
+        return v;
+    }
+    float all = __shfl(v, first, 64);
+    for (int i = 1; i < lanes; ++i) all = op(all, __shfl(v, first + i, 64));
+    return all;
 }
 
 __device__ __forceinline__ float elem(const u32x4& w, int i) {
@@ -202,6 +209,7 @@ __device__ __forceinline__ u32x4 load_segment(const __bf16* p) {
 
 struct VecPlan {
     int lanes;        // G
+    bool power;       // G is a power of two
     int split;        // split chunks of a rotated row (half layout), 0 for interleaved
     int chunks;       // chunks of a q or k row
     int plain;        // chunks of a v row
@@ -212,8 +220,8 @@ struct VecPlan {
 template <bool kInterleaved, bool kFp8, bool kWhole>
 __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, VecPlan plan) {
     const int lane = threadIdx.x & 63;
-    const int sub = lane & (plan.lanes - 1);
     const int in_slab = lane / plan.lanes;
+    const int sub = lane - in_slab * plan.lanes;
     const int per_slab = kWave / plan.lanes;
     const uint32_t units = plan.units[0] + plan.units[1] + plan.units[2];
     const uint32_t total = static_cast<uint32_t>(a.tokens) * units;
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
         while (u >= plan.units[s]) u -= plan.units[s++];
         const RotarySection& c = a.sec[s];
         const int chunks = s == 2 ? plan.plain : plan.chunks;
-        const bool live = sub < chunks;
+        const bool live = sub < chunks && in_slab < per_slab;
         const int chunk = min(sub, chunks - 1);
         const bool split = s < 2 && chunk < plan.split;
         // where its segments start, and which of their elements are this lane's: [lo, hi)
@@ -333,8 +341,8 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
                 else
                     sum += mine(i) ? x[i] * x[i] : 0.f;
             }
-            sum = group_reduce(live ? sum : 0.f, plan.lanes,
-                               [](float p, float q) { return p + q; });
+            sum = row_reduce(live ? sum : 0.f, plan.lanes, plan.power, lane - sub,
+                             [](float p, float q) { return p + q; });
             const float inv = rsqrtf(sum * a.per_elem + a.eps);
 #pragma unroll
             for (int i = 0; i < kSegment; ++i) {
@@ -363,8 +371,8 @@ __global__ __launch_bounds__(kThreads, 8) void rotary_vec_kernel(RotaryArgs a, V
 #pragma unroll
             for (int i = 0; i < kChunkElems; ++i)
                 amax = kWhole || mine(i) ? fmaxf(amax, fabsf(x[i])) : amax;
-            amax = group_reduce(amax, plan.lanes,
-                                [](float p, float q) { return fmaxf(p, q); });
+            amax = row_reduce(amax, plan.lanes, plan.power, lane - sub,
+                              [](float p, float q) { return fmaxf(p, q); });
             const float scale = fp8_row_scale(amax);
             const float by = fp8_row_inverse(scale);
             if (!store) continue;
@@ -419,8 +427,14 @@ bool vec_plan(const RotaryArgs& a, bool interleaved, VecPlan& plan) {
     plan.chunks = interleaved ? plan.plain : plan.split + up(d - r, kChunkElems);
     const int most = std::max(plan.chunks, plan.plain);
     if (most > kWave) return false;
-    plan.lanes = 1;
-    while (plan.lanes < most) plan.lanes *= 2;
+    int power = 1;
+    while (power < most) power *= 2;
+    // A power of two of lanes has the shorter reduction; as many lanes as chunks hold more rows a
+    // wavefront. At nine chunks (7 rows or 4) the rotation of 8191 tokens x 40 heads takes 40 us
+    // or 48, with norm and fp8 write 68 or 81; at five (12 or 8) a head of 64 rotated in 30 with
+    // the norm 31 or 33; at six (10 or 8) the rotation 23.7 or 22.9, with the norm 28.1 or 25.9.
+    plan.lanes = kWave / most * 2 >= kWave / power * 3 ? most : power;
+    plan.power = plan.lanes == power;
     plan.whole = r % (interleaved ? kSegment : kChunkElems) == 0 && d % kChunkElems == 0;
     for (int s = 0; s < 3; ++s) plan.units[s] = up(a.sec[s].heads, kWave / plan.lanes);
     return true;
