@@ -14,14 +14,13 @@ and a device status word for what it cannot (as in build_batch_metadata).
 """
 from __future__ import annotations
 
-from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .ops import (INVALID_ARGUMENT, CcinferError, _check, _require, _stream, _workspace,
-                  current_device)
+from .ops import (INVALID_ARGUMENT, CcinferError, _check, _known_size, _require, _stream,
+                  _workspace, current_device)
 
 _I32 = torch.int32
 
@@ -101,8 +100,8 @@ def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: tor
         raise CcinferError(code, op)
 
 
-@lru_cache(maxsize=1024)
 def update_tables_workspace_size(num_items: int, max_blocks_per_req: int, num_blocks: int) -> int:
+    """Workspace bytes of update_block_tables (0 for an invalid shape)."""
     return int(_lib.load().ccinfer_update_tables_workspace_size(num_items, max_blocks_per_req,
                                                                 num_blocks))
 
@@ -153,8 +152,8 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
         _require(v_cache is not None, op)
         cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
         _require(cache[7] == nb, op)
-    ws, ws_bytes = _workspace(update_tables_workspace_size(n, width, nb), block_table.device,
-                              workspace)
+    ws, ws_bytes = _workspace(_known_size(update_tables_workspace_size, n, width, nb),
+                              block_table.device, workspace)
     code = _lib.load().ccinfer_update_block_tables(
         block_table.data_ptr(), context_lens.data_ptr(), ref_counts.data_ptr(),
         dst_rows.data_ptr() or None, None if src_rows is None else src_rows.data_ptr() or None,
@@ -165,8 +164,8 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     return status
 
 
-@lru_cache(maxsize=1024)
 def compact_workspace_size(num_blocks: int) -> int:
+    """Workspace bytes of compact_kv_blocks (0 for an invalid shape)."""
     return int(_lib.load().ccinfer_compact_workspace_size(num_blocks))
 
 
@@ -198,7 +197,8 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     _index(table, dev, op)
     _require(table.shape == block_table.shape and _index(refs, dev, op) == nb
              and _index(remap, dev, op) == nb and _index(live, dev, op) == 1, op)
-    ws, ws_bytes = _workspace(compact_workspace_size(nb), block_table.device, workspace)
+    ws, ws_bytes = _workspace(_known_size(compact_workspace_size, nb), block_table.device,
+                              workspace)
     rows, width = block_table.shape
     _check(_lib.load().ccinfer_compact_kv_blocks(
         block_table.data_ptr() or None, ref_counts.data_ptr(), rows, width, *cache,
