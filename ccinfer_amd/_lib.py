@@ -74,7 +74,7 @@ SIGNATURES = {
     "ccinfer_update_block_tables": (
         _c_int,
         [_vp] * 6 + [_c_int] * 3 + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
-        + [_vp, _vp, _c_size, _vp],
+        + [_vp] * 4 + [_c_size, _vp],
     ),
     "ccinfer_compact_workspace_size": (_c_size, [_c_int]),
     "ccinfer_compact_kv_blocks": (

@@ -11,6 +11,7 @@
 // Device errors map as in src/backend/cuda/cuda_utils.h:13-36.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -768,7 +769,8 @@ int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void*
                          rope_cache_max_position) ||
         !fits_int(heads * head_dim) || qkv_token_stride < heads * head_dim)
         return CCINFER_ERR_INVALID_ARGUMENT;
-    if (!finite_bits(eps) || !(eps > 0.0f) || !finite_bits(weight_offset))
+    // a normal number: the reciprocal root does not take smaller ones
+    if (!finite_bits(eps) || !(eps >= FLT_MIN) || !finite_bits(weight_offset))
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(rope_cache) % 8 != 0) return CCINFER_ERR_INVALID_ARGUMENT;
     const bool fp8 = k_scale != nullptr;
@@ -838,8 +840,8 @@ int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int
                                 float* k_scale, float* v_scale, int num_layers,
                                 int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
                                 int n_kv_heads, int head_dim, int cache_block_size,
-                                int32_t* status, void* workspace, size_t workspace_bytes,
-                                void* stream) {
+                                int32_t* copy_src, int32_t* copy_dst, int32_t* status,
+                                void* workspace, size_t workspace_bytes, void* stream) {
     KvLayers kv;
     const bool bare = !k_cache && !v_cache && !k_scale && !v_scale && num_layers == 0;
     if (!(bare ? kv_pool_of(num_blocks, cache_block_size, kv)
@@ -851,6 +853,7 @@ int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int
         num_rows <= 0 || max_blocks_per_req <= 0)
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (num_items > 0 && !dst_rows) return CCINFER_ERR_INVALID_ARGUMENT;
+    if ((copy_src == nullptr) != (copy_dst == nullptr)) return CCINFER_ERR_INVALID_ARGUMENT;
     if (!fits_int(static_cast<int64_t>(num_rows) * max_blocks_per_req) ||
         !fits_int(static_cast<int64_t>(num_items) * max_blocks_per_req) ||
         !fits_int(static_cast<int64_t>(max_blocks_per_req) * cache_block_size))
@@ -870,6 +873,8 @@ int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int
     u.src = src_rows;
     u.lengths = lengths;
     u.items = num_items;
+    u.copy_src = copy_src;
+    u.copy_dst = copy_dst;
     u.status = status;
     return map_hip_error(update_block_tables(u, kv, workspace, as_stream(stream)));
 }

@@ -301,6 +301,8 @@ struct TableUpdate {
     const int32_t* src = nullptr;
     const int32_t* lengths = nullptr;
     int items = 0;
+    int32_t* copy_src = nullptr;  // [items] each, or NULL: the copies of partial blocks
+    int32_t* copy_dst = nullptr;
     int32_t* status = nullptr;
 };
 

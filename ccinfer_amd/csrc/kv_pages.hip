@@ -405,7 +405,7 @@ __global__ __launch_bounds__(kThreads) void update_plan_kernel(TableUpdate u, Kv
     p.shared = known - (copied ? 1 : 0);
     p.need = p.total - p.shared;
     p.from = copied ? last : -1;
-    tell(copied && kv.layers == 0 ? kInvalidArgument : kOk);
+    tell(copied && kv.layers == 0 && u.copy_src == nullptr ? kInvalidArgument : kOk);
 }
 
 // Workgroup (i, y): y = 0 changes the table row and the counts of item i; every y copies its
@@ -453,6 +453,8 @@ __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, K
                        : all[0] > all[2] ? kExhausted
                                          : kOk;
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *u.status = status;
+    const bool tells = u.copy_src != nullptr && blockIdx.y == 0 && i < u.items;
+    if (status != kOk && tells && tid == 0) u.copy_src[i] = u.copy_dst[i] = -1;
     if (status != kOk || i >= u.items) return;
 
     const int lo = all[1];
@@ -490,8 +492,13 @@ __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, K
     } else if (copies) {
         select(lo + 1, [&](int, int b) { to = b; });
     }
-    if (!copies) return;
+    if (!copies && !tells) return;
     __syncthreads();
+    if (tells && tid == 0) {
+        u.copy_src[i] = p.from;
+        u.copy_dst[i] = p.from >= 0 ? to : -1;
+    }
+    if (!copies) return;
     ahead.finish(kv, p.from, to, p.part);
     for (int part = blockIdx.y + gridDim.y; part < parts; part += gridDim.y)
         copy_part<T>(kv, part, p.from, to, p.part);

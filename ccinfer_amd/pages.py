@@ -14,7 +14,7 @@ and a device status word for what it cannot (as in build_batch_metadata).
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -114,7 +114,9 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
                         k_scale: Optional[torch.Tensor] = None,
                         v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
                         workspace: Optional[torch.Tensor] = None,
-                        status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                        status: Optional[torch.Tensor] = None,
+                        copies: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                        ) -> torch.Tensor:
     """Makes row dst_rows[i] hold the first min(lengths[i], source's context) tokens of row
     src_rows[i] as it was before the call, then blocks for the tokens up to lengths[i]; changes
     block_table, context_lens and ref_counts in place. src_rows None: of the row itself, an
@@ -126,8 +128,12 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     filled in part, where it would be shared, is copied to one of the row's own. New blocks are
     the lowest-numbered that were free before the call, in item order; blocks it releases are
     free after it. Returns `status` (int32 [1]): 0, or, with nothing changed, 6 (a row or length
-    out of range, a row twice in dst_rows, a copy needed but no caches given), 14 (a row with a
-    context or blocks that the pool does not hold) or 12 (not enough free blocks)."""
+    out of range, a row twice in dst_rows, a copy needed but neither caches nor lists given), 14
+    (a row with a context or blocks that the pool does not hold) or 12 (not enough free blocks).
+
+    `copies`: two int32 tensors of as many elements as dst_rows, which receive the block that
+    each item copied and its copy (-1, -1: none). With them the caches may be None: where layers
+    are held one by one, copy_kv_blocks(layer's k, v, *copies) for each of them does the copies."""
     op = "update_block_tables"
     _require(block_table.is_cuda, op)
     dev = current_device()
@@ -145,6 +151,10 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     rows, width = shape
     if status is None:
         status = torch.empty(1, dtype=_I32, device=block_table.device)
+    copy_src = copy_dst = None
+    if copies is not None:
+        _require(_index(copies[0], dev, op) == n and _index(copies[1], dev, op) == n, op)
+        copy_src, copy_dst = copies[0].data_ptr() or None, copies[1].data_ptr() or None
     if k_cache is None:
         _require(v_cache is None and k_scale is None and v_scale is None, op)
         cache = (None, None, None, None, 0, 0, 0, nb, 0, 0, cache_block_size)
@@ -158,7 +168,7 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
         block_table.data_ptr(), context_lens.data_ptr(), ref_counts.data_ptr(),
         dst_rows.data_ptr() or None, None if src_rows is None else src_rows.data_ptr() or None,
         None if lengths is None else lengths.data_ptr() or None, n, rows, width, *cache,
-        status.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _stream())
+        copy_src, copy_dst, status.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _stream())
     if code:
         raise CcinferError(code, op)
     return status

@@ -360,7 +360,7 @@ int ccinfer_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_he
 /* ccinfer_qkv_prologue with float32 inside and one rounding at the end, for models and caches
  * that it does not take: y = x rsqrt(mean x^2 + eps) (w + weight_offset) of each q and k head
  * (a NULL weight: no norm for that side; *_per_head: the weights are [heads][head_dim], else
- * [head_dim]), the rotation of ccinfer_rotary_embedding, q to q_out [num_tokens]
+ * [head_dim]; eps at least 2^-126), the rotation of ccinfer_rotary_embedding, q to q_out [num_tokens]
  * [num_q_heads][head_dim], K and V to their slots of a bf16 cache, or, with k_scale and
  * v_scale, of an fp8 cache (layout and quantisation of ccinfer_write_kv_cache_fp8, straight
  * from the float32 rows; a NaN is stored as E4M3's). qkv rows lie qkv_token_stride elements
@@ -415,9 +415,12 @@ size_t ccinfer_update_tables_workspace_size(int num_items, int max_blocks_per_re
  * lowest-numbered ones that were free before the call, in item order; what the call releases
  * is free after it. *status (on the device, always written): CCINFER_OK, or, with nothing
  * changed, CCINFER_ERR_INVALID_ARGUMENT (a row or length out of range, two items of one row,
- * a copy needed but no caches given), CCINFER_ERR_KV_INVALID_TABLE (a context outside the
+ * a copy needed but neither caches nor lists given), CCINFER_ERR_KV_INVALID_TABLE (a context outside the
  * row, a block outside the pool or with count 0 among those held), or
- * CCINFER_ERR_KV_EXHAUSTED. Caches NULL with num_layers 0: tables and counts alone. */
+ * CCINFER_ERR_KV_EXHAUSTED. copy_src / copy_dst [num_items], or both NULL: the block that item
+ * i copied and its copy, -1 where it copied none or the call failed. Caches NULL with
+ * num_layers 0: tables and counts alone; the copies are then the caller's, from these two
+ * lists (ccinfer_copy_kv_blocks for each layer held by itself). */
 int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int32_t* ref_counts,
                                 const int32_t* dst_rows, const int32_t* src_rows,
                                 const int32_t* lengths, int num_items, int num_rows,
@@ -425,8 +428,8 @@ int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int
                                 float* k_scale, float* v_scale, int num_layers,
                                 int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
                                 int n_kv_heads, int head_dim, int cache_block_size,
-                                int32_t* status, void* workspace, size_t workspace_bytes,
-                                void* stream);
+                                int32_t* copy_src, int32_t* copy_dst, int32_t* status,
+                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* Workspace bytes of ccinfer_compact_kv_blocks (0 for an invalid shape). */
 size_t ccinfer_compact_workspace_size(int num_blocks);

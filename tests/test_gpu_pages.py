@@ -428,3 +428,59 @@ def test_update_of_many_rows(gpu, rows, fp8):
     assert x.step(p, rest, rng.choice(some, len(rest)), None) == 0      # forks
     assert x.step(p, np.arange(rows), None, x.c + 1) == 0               # a step of every row
     assert x.step(p, rng.permutation(rows), rng.integers(-1, rows, rows), None) == 0  # all change
+
+
+# ---- layers held one by one ----------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_copies_told_and_done_layer_by_layer(gpu, fp8):
+    say(f"copies told {fp8}")
+    p, q = (Pool(gpu, 60, 3, 60, 2, 64, fp8=fp8) for _ in range(2))  # the same bits
+    x, y = Tables(gpu, 7, 9, 60), Tables(gpu, 7, 9, 60)
+    rng = np.random.default_rng(61)
+    told = 0
+    for k in range(20):
+        n = int(rng.integers(1, 8))
+        dst, src = rng.permutation(7)[:n], rng.integers(-1, 7, n)
+        lengths = np.where(rng.random(n) < 0.5, -1, rng.integers(0, 9 * 16 + 1, n))
+        if k == 10:
+            lengths[0] = 9 * 16 + 1  # fails: nothing to copy
+        ctx0 = x.c.copy()
+        a, b = (torch.full((n,), 77, dtype=torch.int32, device=gpu) for _ in range(2))
+        code = x.step(p, dst, src, lengths, copies=(a, b))
+        assert (code == 6) == (k == 10)
+        c, d = (torch.full((n,), 77, dtype=torch.int32, device=gpu) for _ in range(2))
+        status = cc.update_block_tables(y.dt, y.dc, y.dr, i32(dst, gpu), i32(src, gpu),
+                                        i32(lengths, gpu), copies=(c, d))
+        assert status.item() == code and torch.equal(a, c) and torch.equal(b, d)
+        for u, w in ((x.dt, y.dt), (x.dc, y.dc), (x.dr, y.dr)):
+            assert torch.equal(u, w)
+        if code:
+            assert (a == -1).all() and (b == -1).all()
+        told += int((a >= 0).sum())
+        for layer in range(3):
+            s = {} if not fp8 else {"k_scale": q.s[0][layer], "v_scale": q.s[1][layer]}
+            cc.copy_kv_blocks(q.t[0][layer], q.t[1][layer], c, d, **s)
+        # A whole block is copied there, its held tokens here. The tokens past those are written
+        # before they are read, as a server's step does; then what is held is the same.
+        table, ctx = x.t, x.c
+        for i in range(n if code == 0 else 0):
+            kept = min(int(ctx[dst[i]]), int(ctx0[src[i]]) if src[i] >= 0 else 0)
+            for pos in range(kept, int(ctx[dst[i]])):
+                blk = table[dst[i], pos // 16]
+                for u in (*p.t, *q.t):
+                    u[:, blk, pos % 16] = pos % 7
+                for u in (*p.s, *q.s) if fp8 else ():
+                    u.view(3, 60, 2, 16)[:, blk, :, pos % 16] = pos
+        for row, n_row in zip(table, ctx):
+            for j, blk in enumerate(row[:-(-int(n_row) // 16)]):
+                tokens = min(16, int(n_row) - 16 * j)
+                for u, w in zip(p.caches(), q.caches()):
+                    assert np.array_equal(u[:, blk, :tokens], w[:, blk, :tokens])
+                for u, w in zip(p.scales(), q.scales()):
+                    assert np.array_equal(u[:, blk, :, :tokens], w[:, blk, :, :tokens])
+    assert told > 5
+    one = i32([0], gpu)
+    for bad in ((one, i32([0, 1], gpu)), (one, one.long())):
+        with pytest.raises(cc.CcinferError):
+            cc.update_block_tables(y.dt, y.dc, y.dr, one, one, None, copies=bad)

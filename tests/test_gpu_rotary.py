@@ -531,3 +531,44 @@ def test_tensors_of_another_device_are_refused(gpu, monkeypatch):
         with pytest.raises(cc.CcinferError) as e:
             call()
         assert e.value.code == 6, i
+
+
+def test_copied_elements_keep_their_bits(gpu):
+    # every bf16 but the NaNs, subnormal ones among them: past the rotated part, in rows at
+    # positions outside the table, and in v rows
+    say("copied bits")
+    h, d = 4, 128
+    every = np.arange(1 << 16, dtype=np.uint16)
+    every = every[(every & 0x7fff) <= 0x7f80]
+    t = -(-len(every) // (h * d))
+    x = np.resize(every, (t, h, d))
+    for rotary in (64, 100):
+        tab = torch.from_numpy(R.table(8, rotary)).to(gpu)
+        for inter in (False, True):
+            q = from_u16(x, gpu)
+            out, _ = cc.rotary_embedding(q, None, i32(np.arange(t) % 8, gpu), tab, inter)
+            assert np.array_equal(u16(out)[..., rotary:], x[..., rotary:])
+            out, _ = cc.rotary_embedding(q, None, i32(np.full(t, -1), gpu), tab, inter)
+            assert np.array_equal(u16(out), x)
+            qkv = from_u16(np.tile(x.reshape(t, h * d), (1, 3)), gpu)
+            k, v = (torch.zeros(t, h, d, dtype=torch.bfloat16, device=gpu) for _ in "kv")
+            out = cc.qkv_norm_rope(qkv, None, None, i32(np.full(t, -1), gpu), tab,
+                                   i32(np.arange(t), gpu), k, v, h, interleaved=inter)
+            for got in (out, k, v):
+                assert np.array_equal(u16(got), x)
+
+
+def test_smallest_eps_and_rows_of_zeros(gpu):
+    say("smallest eps")
+    t, hq, hkv, d = 7, 4, 2, 128
+    for fp8 in (False, True):
+        s = make_norm(gpu, 14, t, hq, hkv, d, d, fp8)
+        s["qkv"][4:6] = 0
+        s["qkv"][6] *= 2.0 ** -70  # squares under the smallest normal number
+        eps = float(np.float32(2.0 ** -126))
+        q = run_norm(s, gpu, hq, eps=eps)
+        assert not q[4:6].any()
+        s["qkv"][6] = 0  # (float32 squares of the row are no measure for it)
+        assert torch.isfinite(q).all()
+        (wq, sq), _, _ = want_norm(s, hq, hkv, d, False, eps, 0.0)
+        R.assert_bf16(f64(q)[:6], wq[:6], sq[:6], "q")

@@ -129,7 +129,7 @@ def test_norm_rope_refusals(lib):
     for i, bad in [(0, None), (1, 1535), (6, None), (7, None), (7, FAKE + 4), (8, None), (9, None),
                    (10, None), (11, None), (12, FAKE), (13, FAKE), (14, 0), (15, 0), (16, 0),
                    (17, 0), (17, 127), (17, 1026), (18, 0), (18, 3), (18, 130), (19, 0), (20, 0),
-                   (22, 0.0), (22, -1.0), (22, NAN), (22, INF), (23, NAN), (23, INF)]:
+                   (22, 0.0), (22, -1.0), (22, 1e-39), (22, NAN), (22, INF), (23, NAN), (23, INF)]:
         a = list(ok)
         a[i] = bad
         assert fn(*a) == INVALID, (i, bad)
@@ -170,20 +170,21 @@ def test_update_refusals(lib):
     need = lib.ccinfer_update_tables_workspace_size(4, 32, 64)
     assert need > 0
     ok = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 4, 8, 32, FAKE, FAKE, None, None, 3, layer, 0, 64, 8,
-          128, 16, FAKE, FAKE, need, None]
+          128, 16, None, None, FAKE, FAKE, need, None]
     for i, bad in [(0, None), (1, None), (2, None), (3, None), (6, -1), (7, 0), (8, 0), (9, None),
                    (10, None), (11, FAKE), (12, FAKE), (13, 0), (14, layer - 2), (16, 0), (17, 0),
-                   (18, 0), (19, 0), (20, None), (21, None), (21, FAKE + 8), (22, need - 1)]:
+                   (18, 0), (19, 0), (20, FAKE), (21, FAKE), (22, None), (23, None),
+                   (23, FAKE + 8), (24, need - 1)]:
         a = list(ok)
         a[i] = bad
         assert fn(*a) == INVALID, (i, bad)
     a = list(ok)
     a[9:16] = [None, None, None, None, 0, 0, 0]
     a[16] = (1 << 24) + 1  # blocks past the bitmap
-    a[22] = 1 << 40
+    a[24] = 1 << 40
     assert fn(*a) == UNSUPPORTED
     a = list(ok)
-    a[6], a[22] = (1 << 14) + 1, 1 << 40
+    a[6], a[24] = (1 << 14) + 1, 1 << 40
     assert fn(*a) == UNSUPPORTED
     assert lib.ccinfer_update_tables_workspace_size(4, 32, (1 << 24) + 1) == 0
     assert lib.ccinfer_update_tables_workspace_size((1 << 14) + 1, 32, 64) == 0
