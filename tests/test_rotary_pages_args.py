@@ -1,5 +1,5 @@
 """The rotary and page entries on the CPU: refusals before any device is touched, frequencies of
-the scalings against their formulas, and the checkers of the GPU tests against themselves."""
+the scalings against their formulas, and the references of the GPU tests against themselves."""
 import ctypes
 import math
 
@@ -222,7 +222,7 @@ def test_python_entries_refuse_host_tensors():
         assert e.value.code == INVALID
 
 
-# ---- the checkers -----------------------------------------------------------------------
+# ---- the references -----------------------------------------------------------------------
 
 def test_reference_rotation_turns_back_and_is_its_own_gradient():
     rng = np.random.default_rng(1)
