@@ -3,7 +3,8 @@
 //
 // The reference keeps its allocator on the host (src/cache/kv_cache_manager.cpp): a request that
 // is forked, cut back or finished costs a walk over host lists and an upload of its table row.
-// Here the pool is one array of reference counts on the device (0 = free); what a call hands out
+// Here the pool is one array of reference counts on the device (0 = free; a count below 0, from
+// owners that were not counted, is neither free nor held); what a call hands out
 // is always the lowest-numbered free blocks, in item order, so its results do not depend on the
 // order in which workgroups run. The only atomics are integer additions to the counts.
 //
@@ -187,7 +188,7 @@ __device__ __forceinline__ void free_bitmap(const int32_t* __restrict__ refs, in
 #pragma unroll
     for (int k = 0; k < kWaveWords; ++k) {
         const int b = c * kChunk + (word + k) * kWave + lane;
-        const uint64_t bits = __ballot(b < blocks && ref[k] <= 0);
+        const uint64_t bits = __ballot(b < blocks && ref[k] == 0);
         if (lane == 0) bitmap[static_cast<int64_t>(c) * kChunkWords + word + k] = bits;
         count += __popcll(bits);
     }
@@ -546,8 +547,9 @@ __global__ __launch_bounds__(kThreads) void free_bitmap_kernel(const int32_t* re
     free_bitmap(refs, blocks, blockIdx.x, bitmap, counts);
 }
 
-// The live blocks from n_live on (the movers) and the free ones below n_live (the holes) are
-// equally many, at most half of the pool; the j-th lowest mover goes to the j-th lowest hole.
+// The live blocks (all that are not free) from n_live on (the movers) and the free ones below
+// n_live (the holes) are equally many, at most half of the pool; the j-th lowest mover goes to
+// the j-th lowest hole.
 // Workgroup c lists those of its chunk and writes its blocks' counts and new numbers, the
 // movers' own (known once all holes are) aside.
 __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const int32_t* refs, int blocks,

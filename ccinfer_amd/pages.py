@@ -10,7 +10,8 @@ and a device status word for what it cannot (as in build_batch_metadata).
                      lie apart, each is contiguous); bf16, or uint8 with k_scale / v_scale
                      (float32, [layers, fp8_scale_numel] beside caches of all layers)
   block_table        [rows, max_blocks_per_req] int32, -1 padded; context_lens [rows] int32
-  ref_counts         [blocks] int32: owners of each block, 0 = free
+  ref_counts         [blocks] int32: owners of each block, 0 = free; a block given up more often
+                     than it was counted is below 0 and not handed out again
 """
 from __future__ import annotations
 
@@ -184,8 +185,8 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
                       v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
                       workspace: Optional[torch.Tensor] = None,
                       out: Optional[dict] = None) -> dict:
-    """Moves the live blocks (count > 0) to the front of the pool, the ones past it, lowest first,
-    into the free blocks, lowest first; returns int32 device tensors block_table and ref_counts
+    """Moves the live blocks (count not 0) to the front of the pool, the ones past it, lowest
+    first, into the free blocks, lowest first; returns int32 device tensors block_table and ref_counts
     with the new numbers, remap [blocks] (each block's new number, -1 for a free one) and
     num_live [1]. Table entries of free blocks become -1, negative ones stay. `out` reuses
     tensors of an earlier call; its block_table and ref_counts may be the inputs."""

@@ -384,8 +384,10 @@ int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void*
  * finite): the attention multiplies those of a block's slots that hold no token by 0.
  *
  * ref_counts [num_blocks] says how many table rows (or other owners, a prefix cache say) hold
- * a block; 0 is free. CCINFER_ERR_UNSUPPORTED for more than 2^24 blocks in the calls that take
- * counts, 2^14 items of an update and 2^17 pairs of a copy. */
+ * a block; 0 is free. A block that is given up more often than it was counted ends below 0:
+ * it is not handed out again, and a row that still holds it gets
+ * CCINFER_ERR_KV_INVALID_TABLE. CCINFER_ERR_UNSUPPORTED for more than 2^24 blocks in the calls
+ * that take counts, 2^14 items of an update and 2^17 pairs of a copy. */
 
 /* Block dst_blocks[i] becomes a copy of src_blocks[i] in every layer, K, V and scales. Pairs
  * with a block outside [0, num_blocks), and of a block with itself, are skipped. Pairs that
@@ -416,7 +418,7 @@ size_t ccinfer_update_tables_workspace_size(int num_items, int max_blocks_per_re
  * is free after it. *status (on the device, always written): CCINFER_OK, or, with nothing
  * changed, CCINFER_ERR_INVALID_ARGUMENT (a row or length out of range, two items of one row,
  * a copy needed but neither caches nor lists given), CCINFER_ERR_KV_INVALID_TABLE (a context outside the
- * row, a block outside the pool or with count 0 among those held), or
+ * row, a block outside the pool or with a count below 1 among those held), or
  * CCINFER_ERR_KV_EXHAUSTED. copy_src / copy_dst [num_items], or both NULL: the block that item
  * i copied and its copy, -1 where it copied none or the call failed. Caches NULL with
  * num_layers 0: tables and counts alone; the copies are then the caller's, from these two
@@ -434,9 +436,9 @@ int ccinfer_update_block_tables(int32_t* block_table, int32_t* context_lens, int
 /* Workspace bytes of ccinfer_compact_kv_blocks (0 for an invalid shape). */
 size_t ccinfer_compact_workspace_size(int num_blocks);
 
-/* Moves the live blocks (count > 0) into blocks [0, *num_live): those that lie past it, lowest
- * first, to the free blocks below it, lowest first; the others stay. Writes the tables with the
- * new numbers (entries of free blocks and past the pool become -1, negative ones stay), the
+/* Moves the live blocks (count not 0) into blocks [0, *num_live): those that lie past it,
+ * lowest first, to the free blocks below it, lowest first; the others stay. Writes the tables
+ * with the new numbers (entries of free blocks and past the pool become -1, negative ones stay), the
  * counts, and remap [num_blocks]: each block's new number, -1 for a free one. The outputs may
  * be the inputs (block_table_out = block_table, ref_counts_out = ref_counts). num_rows 0: no
  * tables. */

@@ -484,3 +484,49 @@ def test_copies_told_and_done_layer_by_layer(gpu, fp8):
     for bad in ((one, i32([0, 1], gpu)), (one, one.long())):
         with pytest.raises(cc.CcinferError):
             cc.update_block_tables(y.dt, y.dc, y.dr, one, one, None, copies=bad)
+
+
+# ---- counts below zero ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("blocks", [24, 30000])
+def test_block_given_up_too_often_is_never_handed_out(gpu, blocks):
+    # rows 0 and 1 hold block 5, which is counted once: both leave in one call, its count is -1,
+    # and no later row may get it. 30000: past the blocks that one workgroup's words cover.
+    say(f"count below zero {blocks}")
+    p = Pool(gpu, 70, 1, blocks, 1, 8)
+    rows = i32([[5, -1, -1, -1], [5, -1, -1, -1], [-1] * 4, [-1] * 4], gpu)
+    ctx, refs = i32([16, 16, 0, 0], gpu), i32(np.ones(blocks), gpu)
+    refs[[2, 9, blocks - 1]] = 0
+
+    def step(dst, src, lengths):
+        return cc.update_block_tables(rows, ctx, refs, i32(dst, gpu), i32(src, gpu),
+                                      i32(lengths, gpu), *p.t).item()
+    assert step([0, 1], [-1, -1], [0, 0]) == 0
+    assert refs[5].item() == -1 and not ctx.any()
+    assert step([0], [-1], [16]) == 0 and rows[0].tolist() == [2, -1, -1, -1]
+    assert step([1], [-1], [32]) == 0 and rows[1].tolist() == [9, blocks - 1, -1, -1]
+    assert step([2], [-1], [16]) == 12                     # nothing is left
+    rows[3, 0], ctx[3] = 5, 16                             # a row that holds it all the same
+    assert step([3], [3], [10]) == 14 and step([2], [3], [-1]) == 14
+    assert refs[5].item() == -1 and rows[3].tolist() == [5, -1, -1, -1]
+
+
+@pytest.mark.parametrize("blocks", [24, 3000])
+def test_compaction_keeps_blocks_of_counts_below_zero(gpu, blocks):
+    # such a block is not free: nothing is moved over it, and it goes on with its count
+    say(f"compact count below zero {blocks}")
+    p = Pool(gpu, 71, 2, blocks, 1, 8)
+    refs = np.zeros(blocks, np.int32)
+    refs[[1, 4, blocks - 1]], refs[[0, blocks - 3]] = (2, 1, 3), (-1, -2)
+    table = np.array([[1, 4, blocks - 1], [0, blocks - 3, 7]], np.int32)
+    # the same with the counts' signs aside, which the reference takes as it should
+    wt, wr, wm, wn, wc = P.compact(table, np.abs(refs), p.flat())
+    out = cc.compact_kv_blocks(i32(table, gpu), i32(refs, gpu), *p.t)
+    assert out["num_live"].item() == wn == 5
+    assert np.array_equal(out["block_table"].cpu().numpy(), wt)
+    assert np.array_equal(out["remap"].cpu().numpy(), wm)
+    sign = np.zeros(blocks, np.int32)
+    sign[wm[refs != 0]] = np.sign(refs[refs != 0])
+    assert np.array_equal(out["ref_counts"].cpu().numpy(), wr * sign)
+    for a, b in zip(p.flat(), wc):
+        assert np.array_equal(a, b)
