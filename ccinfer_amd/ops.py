@@ -17,7 +17,8 @@ Tensors are device tensors (torch on ROCm: "cuda" is the HIP device). Layouts:
   context_lens         [batch] int32; query_start_loc [batch + 1] int32
   slot_mapping         [total_tokens] int32
 Work is enqueued on torch's current stream; workspaces come from torch's caching
-allocator unless passed in (scratch: no initialisation needed).
+allocator unless passed in (scratch: no initialisation needed; contiguous, on the tensors'
+device).
 """
 from __future__ import annotations
 
@@ -241,12 +242,20 @@ def _size(query, *args) -> int:
     return _known_size(query, *args) if type(args[-1]) is int else query(*args)
 
 
+def _workspace_bytes(device, workspace: torch.Tensor) -> int:
+    """Bytes of a caller's workspace: contiguous (an expanded view has less memory than elements)
+    and on the device of the call's tensors."""
+    _require(workspace.is_cuda and workspace.get_device() == device.index
+             and workspace.is_contiguous(), "workspace")
+    return workspace.numel() * workspace.element_size()
+
+
 def _workspace(nbytes: int, device, workspace: Optional[torch.Tensor]):
     if nbytes == 0:
         return None, 0
     if workspace is not None:
-        have = workspace.numel() * workspace.element_size()
-        _require(workspace.is_cuda and have >= nbytes, "workspace")
+        have = _workspace_bytes(device, workspace)
+        _require(have >= nbytes, "workspace")
         return workspace, have
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
@@ -256,8 +265,7 @@ def _prefill_workspace(nbytes: int, device, workspace: Optional[torch.Tensor]):
     split tiles that the size query counts in: the call itself refuses one that is too small."""
     if nbytes == 0 or workspace is None:
         return _workspace(nbytes, device, workspace)
-    _require(workspace.is_cuda, "workspace")
-    return workspace, workspace.numel() * workspace.element_size()
+    return workspace, _workspace_bytes(device, workspace)
 
 
 def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
