@@ -32,6 +32,7 @@ KV_INVALID_TABLE = 14  # status: a table row that the pool does not hold
 def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: str):
     """The cache arguments of the C ABI: pointers, layers, strides, blocks, heads, head_dim,
     block_size."""
+    _require(block_size > 0, op)
     fp8 = k_scale is not None
     dtype = torch.uint8 if fp8 else torch.bfloat16
     shape, stride = k_cache.shape, k_cache.stride()

@@ -530,3 +530,24 @@ def test_compaction_keeps_blocks_of_counts_below_zero(gpu, blocks):
     assert np.array_equal(out["ref_counts"].cpu().numpy(), wr * sign)
     for a, b in zip(p.flat(), wc):
         assert np.array_equal(a, b)
+
+
+# ---- arguments -----------------------------------------------------------------------------
+
+def test_block_size_of_zero_is_refused(gpu):
+    say("block size 0")
+    p = Pool(gpu, 72, 1, 8, 1, 64)
+    k, v = (x.view(8 * 16, 1, 64) for x in p.t)
+    x = Tables(gpu, 2, 4, 8)
+    one = i32([0], gpu)
+    for bs in (0, -16):
+        for i, call in enumerate([
+                lambda: cc.copy_kv_blocks(k, v, one, one, cache_block_size=bs),
+                lambda: cc.compact_kv_blocks(x.dt, x.dr, k, v, cache_block_size=bs),
+                lambda: cc.update_block_tables(x.dt, x.dc, x.dr, one, one, one, k, v,
+                                               cache_block_size=bs),
+                lambda: cc.update_block_tables(x.dt, x.dc, x.dr, one, one, one,
+                                               cache_block_size=bs)]):
+            with pytest.raises(cc.CcinferError) as e:
+                call()
+            assert e.value.code == 6, (bs, i)
