@@ -37,8 +37,8 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
     dtype = torch.uint8 if fp8 else torch.bfloat16
     shape, stride = k_cache.shape, k_cache.stride()
     dims = len(shape)
-    _require(3 <= dims <= 5 and k_cache.dtype is dtype and v_cache.dtype is dtype
-             and v_cache.shape == shape
+    _require(3 <= dims <= 5 and max(shape) < 2 ** 31 and k_cache.dtype is dtype
+             and v_cache.dtype is dtype and v_cache.shape == shape
              and k_cache.get_device() == dev and v_cache.get_device() == dev
              and fp8 == (v_scale is not None), op)
     h, d = shape[-2], shape[-1]
@@ -51,11 +51,11 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
         _require((stride == vstride or layers == 1 or vstride[0] == stride[0])
                  and (stride[1:] == inner or k_cache[0].is_contiguous())
                  and (vstride[1:] == inner or v_cache[0].is_contiguous())
-                 and bs == block_size and nb < 2 ** 31, op)
+                 and bs == block_size, op)
     else:
         nb, bs = (shape[0], shape[1]) if dims == 4 else (shape[0] // block_size, block_size)
         _require((dims == 4 or nb * bs == shape[0]) and k_cache.is_contiguous()
-                 and v_cache.is_contiguous() and bs == block_size and nb < 2 ** 31, op)
+                 and v_cache.is_contiguous() and bs == block_size, op)
     ksp = vsp = None
     if fp8:
         need = nb * h * 16
@@ -92,7 +92,7 @@ def copy_kv_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src_blocks: tor
     _require(k_cache.is_cuda, op)
     dev = current_device()
     n = _index(src_blocks, dev, op)
-    _require(_index(dst_blocks, dev, op) == n
+    _require(2 ** 31 > _index(dst_blocks, dev, op) == n
              and (status is None or _index(status, dev, op) == 1), op)
     cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
     code = _lib.load().ccinfer_copy_kv_blocks(
@@ -140,7 +140,9 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     _require(block_table.is_cuda, op)
     dev = current_device()
     shape, n, nb = block_table.shape, dst_rows.numel(), ref_counts.numel()
-    _require(len(shape) == 2 and block_table.dtype is _I32 and context_lens.dtype is _I32
+    _require(len(shape) == 2 and max(shape) < 2 ** 31 and n < 2 ** 31 and nb < 2 ** 31
+             and 0 < cache_block_size < 2 ** 31
+             and block_table.dtype is _I32 and context_lens.dtype is _I32
              and ref_counts.dtype is _I32 and dst_rows.dtype is _I32
              and block_table.get_device() == dev and context_lens.get_device() == dev
              and ref_counts.get_device() == dev and dst_rows.get_device() == dev
@@ -196,7 +198,7 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     dev = current_device()
     _index(block_table, dev, op)
     _index(ref_counts, dev, op)
-    _require(block_table.dim() == 2, op)
+    _require(block_table.dim() == 2 and max(block_table.shape) < 2 ** 31, op)
     cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
     nb = cache[7]
     _require(ref_counts.numel() == nb, op)

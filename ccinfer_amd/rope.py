@@ -122,11 +122,12 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     dev = current_device()
     shape, qs, table = q.shape, q.stride(), rope_cache.shape
     _require(len(shape) == 3 == len(table) and table[2] == 2 and qs[2] == 1
+             and max(shape) < 2 ** 31 > table[0] and 2 * table[1] <= shape[2]
              and q.dtype is _BF16 and positions.dtype is _I32 and rope_cache.dtype is _F32
              and q.get_device() == dev and positions.get_device() == dev
              and rope_cache.get_device() == dev and positions.is_contiguous()
              and rope_cache.is_contiguous()
-             and 2 ** 31 > positions.numel() == shape[0] > 0, op)
+             and positions.numel() == shape[0] > 0, op)
     t, hq, d = shape
     if q_out is None:
         q_out = torch.empty(shape, dtype=_BF16, device=q.device)
@@ -139,6 +140,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     else:
         kshape, ks = k.shape, k.stride()
         _require(len(kshape) == 3 and kshape[0] == t and kshape[2] == d and ks[2] == 1
+                 and kshape[1] < 2 ** 31
                  and k.dtype is _BF16 and k.get_device() == dev, op)
         hkv = kshape[1]
         if k_out is None:
@@ -206,9 +208,11 @@ def qkv_norm_rope(qkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
     hkv, d = cache[-2], cache[-1]
     slots = cache[0] if len(cache) == 3 else cache[0] * cache[1]
     t, width = shape
+    if max_slots is None:
+        max_slots = slots
     _require(2 ** 31 > t > 0 and num_q_heads > 0 and width == (num_q_heads + 2 * hkv) * d
-             and positions.numel() == t and slot_mapping.numel() == t
-             and (max_slots is None or max_slots <= slots), op)
+             and width < 2 ** 31 > table[0] and 2 * table[1] <= d and positions.numel() == t
+             and slot_mapping.numel() == t and 0 < max_slots <= slots and max_slots < 2 ** 31, op)
     ksp = vsp = None
     if fp8:
         need = fp8_scale_numel(slots, hkv)
@@ -227,8 +231,7 @@ def qkv_norm_rope(qkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
         qkv.data_ptr(), stride[0] if t > 1 else width, qw, q_each, kw, k_each,
         positions.data_ptr(), rope_cache.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(),
         k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, t, num_q_heads, hkv, d, 2 * table[1],
-        table[0], slots if max_slots is None else max_slots, interleaved, eps, weight_offset,
-        _stream())
+        table[0], max_slots, interleaved, eps, weight_offset, _stream())
     if code:
         raise CcinferError(code, op)
     return q_out

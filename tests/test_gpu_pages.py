@@ -551,3 +551,52 @@ def test_block_size_of_zero_is_refused(gpu):
             with pytest.raises(cc.CcinferError) as e:
                 call()
             assert e.value.code == 6, (bs, i)
+
+
+def test_lists_and_tables_of_more_than_31_bits_are_refused(gpu):
+    # lengths that a 32-bit argument would take for 5 elements, 2 rows or 3 columns
+    say("past 31 bits")
+    p = Pool(gpu, 73, 1, 8, 1, 64)
+    x = Tables(gpu, 2, 4, 8)
+    one = i32([0], gpu)
+    far = torch.zeros(2 ** 32 + 8, dtype=torch.int32, device=gpu)
+    long, tall, wide = far[:2 ** 32 + 5], far[:2 ** 32 + 2], far[:2 ** 32 + 3]
+    for i, call in enumerate([
+            lambda: cc.copy_kv_blocks(*p.t, long, long),
+            lambda: cc.update_block_tables(tall.view(-1, 1), tall, x.dr, one, one, one, *p.t),
+            lambda: cc.update_block_tables(wide.view(1, -1), one, x.dr, one, one, one, *p.t),
+            lambda: cc.update_block_tables(x.dt, x.dc, x.dr, long, long, long, *p.t),
+            lambda: cc.update_block_tables(x.dt, x.dc, x.dr, one, one, one,
+                                           cache_block_size=2 ** 32 + 16),
+            lambda: cc.update_block_tables(x.dt, x.dc, far, one, one, one),
+            lambda: cc.compact_kv_blocks(tall.view(-1, 1), x.dr, *p.t,
+                                         out={"block_table": tall.view(-1, 1), "ref_counts": x.dr,
+                                              "remap": torch.empty_like(x.dr), "num_live": one}),
+            lambda: cc.compact_kv_blocks(wide.view(1, -1), x.dr, *p.t,
+                                         out={"block_table": wide.view(1, -1), "ref_counts": x.dr,
+                                              "remap": torch.empty_like(x.dr), "num_live": one})]):
+        with pytest.raises(cc.CcinferError) as e:
+            call()
+        assert e.value.code == 6, i
+
+
+
+def test_caches_of_more_than_31_bits_a_side_are_refused(gpu):
+    # 2^32 + 2 elements a head, heads or layers, 2^32 + 16 tokens a block
+    say("caches past 31 bits")
+    far = torch.zeros(17, 2 ** 32 + 16, dtype=torch.uint8, device=gpu)
+    k = far.view(-1)[:16 * (2 ** 32 + 2)].view(torch.bfloat16)
+    one, refs, rows = i32([0], gpu), i32([1], gpu), i32([[0]], gpu)
+    tokens = far[:2].view(-1).view(torch.bfloat16)
+    for i, cache in enumerate([k.view(1, 1, 4, 1, -1), k.view(1, 1, 4, -1, 1),
+                               tokens.view(1, 1, -1, 1, 1), k.view(-1, 1, 4, 1, 2)]):
+        for call in (lambda: cc.copy_kv_blocks(cache, cache, one, one,
+                                               cache_block_size=cache.shape[2]),
+                     lambda: cc.update_block_tables(rows, one, refs, one, None, None, cache, cache,
+                                                    cache_block_size=cache.shape[2]),
+                     lambda: cc.compact_kv_blocks(rows, refs, cache, cache,
+                                                  cache_block_size=cache.shape[2])):
+            assert max(cache.shape) > 2 ** 32
+            with pytest.raises(cc.CcinferError) as e:
+                call()
+            assert e.value.code == 6, (i, cache.shape)

@@ -572,3 +572,40 @@ def test_smallest_eps_and_rows_of_zeros(gpu):
         assert torch.isfinite(q).all()
         (wq, sq), _, _ = want_norm(s, hq, hkv, d, False, eps, 0.0)
         R.assert_bf16(f64(q)[:6], wq[:6], sq[:6], "q")
+
+
+def test_caches_of_more_than_31_bits_of_slots_are_refused(gpu):
+    # 2^32 + 16 slots, which a 32-bit argument would take for 16
+    say("slots past 31 bits")
+    far = torch.zeros(2 ** 32 + 16, 1, 2, dtype=torch.bfloat16, device=gpu)
+    qkv = torch.ones(1, 6, dtype=torch.bfloat16, device=gpu)
+    table = torch.from_numpy(R.table(4, 2)).to(gpu)
+    pos, slot = i32([-1], gpu), i32([20], gpu)
+    for most in (None, 2 ** 32 + 16):
+        with pytest.raises(cc.CcinferError) as e:
+            cc.qkv_norm_rope(qkv, None, None, pos, table, slot, far, far, 1, max_slots=most)
+        assert e.value.code == 6
+    cc.qkv_norm_rope(qkv, None, None, pos, table, slot, far, far, 1, max_slots=2 ** 31 - 1)
+    assert (far[20] == 1).all()
+
+
+def test_rows_and_tables_of_more_than_31_bits_are_refused(gpu):
+    # lengths that a 32-bit argument would take for 1 head, 64 elements or 5 positions
+    say("rows past 31 bits")
+    few = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=gpu)
+    heads = torch.zeros(1, 2 ** 32 + 1, 2, dtype=torch.bfloat16, device=gpu)
+    table, pos = torch.from_numpy(R.table(8, 64)).to(gpu), i32([6], gpu)
+    narrow = torch.from_numpy(R.table(8, 2)).to(gpu)
+    out = torch.empty_like(heads)
+    long = torch.zeros(1, 1, 2 ** 32 + 64, dtype=torch.bfloat16, device=gpu)
+    far = torch.zeros(2 ** 32 + 5, 1, 2, device=gpu)
+    for i, call in enumerate([
+            lambda: cc.rotary_embedding(heads, None, pos, narrow, q_out=out),
+            lambda: cc.rotary_embedding(heads[:, :1], heads, pos, narrow, k_out=out),
+            lambda: cc.rotary_embedding(long, None, pos, table, q_out=out.view(-1)[:2 ** 32 + 64]
+                                        .view(1, 1, -1)),
+            lambda: cc.rotary_embedding(few, None, pos, far),
+            lambda: cc.rotary_embedding(few, None, pos, far[:2 ** 32 + 4].view(2, -1, 2))]):
+        with pytest.raises(cc.CcinferError) as e:
+            call()
+        assert e.value.code == 6, i
