@@ -600,3 +600,30 @@ def test_caches_of_more_than_31_bits_a_side_are_refused(gpu):
             with pytest.raises(cc.CcinferError) as e:
                 call()
             assert e.value.code == 6, (i, cache.shape)
+
+
+# ---- blocks of more than one round of loads, scales past a workgroup, single bytes ------------
+
+# Parts of more than 2048 units (a round of a workgroup's loads) of 16, 2 and 1 bytes, more than
+# 256 scales a block, and fp8 caches whose tokens or starts are no multiples of 16 bytes.
+WIDE_POOLS = [dict(layers=2, blocks=20, h=32, d=128), dict(layers=2, blocks=20, h=32, d=128, fp8=True),
+              dict(layers=2, blocks=20, h=8, d=128, bs=32), dict(layers=2, blocks=20, h=8, d=256),
+              dict(layers=2, blocks=17, h=9, d=36, apart=True),
+              dict(layers=3, blocks=20, h=1, d=72, fp8=True),
+              dict(layers=2, blocks=17, h=18, d=68, fp8=True),
+              dict(layers=2, blocks=17, h=3, d=40, apart=True, fp8=True)]
+
+
+@pytest.mark.parametrize("pool", WIDE_POOLS)
+def test_copy_of_wide_blocks(gpu, pool):
+    test_copy(gpu, pool)
+
+
+@pytest.mark.parametrize("pool", WIDE_POOLS)
+def test_update_of_wide_blocks(gpu, pool):
+    test_update_random_steps(gpu, pool)
+
+
+@pytest.mark.parametrize("pool", WIDE_POOLS)
+def test_compact_of_wide_blocks(gpu, pool):
+    test_compact(gpu, pool, False)

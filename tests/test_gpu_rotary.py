@@ -609,3 +609,26 @@ def test_rows_and_tables_of_more_than_31_bits_are_refused(gpu):
         with pytest.raises(cc.CcinferError) as e:
             call()
         assert e.value.code == 6, i
+
+
+def test_rows_whose_squares_are_under_the_smallest_normal_number(gpu):
+    # Elements near 2^-70 beside an eps of 2^-126: float32 squares near 2^-140, which may be lost.
+    # Then 1 / sqrt(mean + eps) is too large by a share of mean / (2 eps), 2^-15 here.
+    say("tiny rows")
+    t, hq, hkv, d = 7, 4, 2, 128
+    eps = float(np.float32(2.0 ** -126))
+    for rotary in (d, 96, 100):
+        s = make_norm(gpu, 15, t, hq, hkv, d, rotary, False)
+        s["qkv"] *= 2.0 ** -70
+        q = run_norm(s, gpu, hq, eps=eps)
+        at = np.flatnonzero((s["slot"] >= 0) & (s["slot"] < s["slots"]))
+        x = f64(s["qkv"]).reshape(t, hq + 2 * hkv, d)
+        lost = (x ** 2).mean(-1, keepdims=True) / (2 * eps)
+        assert lost.max() < 2.0 ** -14
+        (wq, sq), (wk, sk), _ = want_norm(s, hq, hkv, d, False, eps, 0.0)
+        for got, want, size, share, rows in (
+                (f64(q), wq, sq, lost[:, :hq], np.arange(t)),
+                (f64(s["k"])[s["slot"][at]], wk[at], sk[at], lost[at, hq:hq + hkv], at)):
+            bound = np.abs(want) * R.BF16 + size * (R.F32 + share) * (1 + R.BF16) + 1e-38
+            assert np.all(np.abs(got - want) <= bound), rotary
+            assert np.abs(got).max(-1).min() > 2.0 ** -9  # (an answer of zeros is none)
