@@ -10,7 +10,8 @@
 //
 // Quantisation of one row x[0..D): amax = max |x|; scale = the smallest power of two P
 // (at least 2^-126) with amax <= 448 P; q = e4m3(clamp(x / P, +-448)) rounded to nearest
-// even (an all-zero row stores zeros and scale 0). Dequantised value = q * scale. Per-row
+// even (an all-zero row stores zeros and scale 0; this source is built without regard to NaNs,
+// so what one is stored as is left open). Dequantised value = q * scale. Per-row
 // scales make appends exact: a decode step writes one new row and never has to requantise
 // earlier rows of the block. A power-of-two scale (as in the OCP microscaling formats'
 // E8M0 scales) loses no relative precision -- x / P is exact and E4M3 has the same

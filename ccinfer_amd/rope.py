@@ -187,7 +187,8 @@ def qkv_norm_rope(qkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
     v_scale as in ops.write_kv_cache_fp8). It computes in float32 and rounds once, where
     qkv_prologue rounds as the reference's five kernels do, so the two differ in last places.
     A bf16 cache takes K as the rows that rotary_embedding would return; an fp8 one is
-    quantised from float32. No two tokens may have the same slot."""
+    quantised from float32. A row whose sum of squares passes float32's largest number becomes
+    zeros. No two tokens may have the same slot."""
     op = "qkv_norm_rope"
     _require(qkv.is_cuda, op)
     dev = current_device()

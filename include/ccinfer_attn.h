@@ -209,8 +209,8 @@ int ccinfer_decode_attention_noalloc(const void* q, const void* k_cache, const v
  * scale per cache row in k_scale / v_scale, indexed ((slot / 16) * n_kv_heads + kv_head) * 16
  * + slot % 16 (arrays of ceil(max_slots / 16) * 16 * n_kv_heads floats). A row x is stored
  * as e4m3(clamp(x / P, +-448)) with scale P, the smallest power of two >= 2^-126 with
- * max|x| <= 448 P (round to nearest even; an all-zero row stores zeros and scale 0); its
- * value is byte * scale. The attention entries accept any fp32 scale; a power of two takes
+ * max|x| <= 448 P (round to nearest even; an all-zero row stores zeros and scale 0; what an
+ * element that is a NaN stores is not defined); its value is byte * scale. The attention entries accept any fp32 scale; a power of two takes
  * the faster conversion in the fp8 prefill. Halves decode bytes.
  *
  * Replaces launch_write_kv_cache (src/kernel/cuda_kernels.h:80-83) for an fp8 cache:
@@ -360,12 +360,14 @@ int ccinfer_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_he
 /* ccinfer_qkv_prologue with float32 inside and one rounding at the end, for models and caches
  * that it does not take: y = x rsqrt(mean x^2 + eps) (w + weight_offset) of each q and k head
  * (a NULL weight: no norm for that side; *_per_head: the weights are [heads][head_dim], else
- * [head_dim]; eps at least 2^-126), the rotation of ccinfer_rotary_embedding, q to q_out [num_tokens]
+ * [head_dim]; eps at least 2^-126; a row whose sum of squares passes float32's largest number
+ * becomes zeros), the rotation of ccinfer_rotary_embedding, q to q_out [num_tokens]
  * [num_q_heads][head_dim], K and V to their slots of a bf16 cache, or, with k_scale and
  * v_scale, of an fp8 cache (layout and quantisation of ccinfer_write_kv_cache_fp8, straight
- * from the float32 rows; a NaN is stored as E4M3's). qkv rows lie qkv_token_stride elements
- * apart; q_out and the caches lie apart from them. Tokens whose slot is outside [0, max_slots) write no K/V; no two tokens may have the
- * same slot. */
+ * from the float32 rows; a NaN is stored as E4M3's NaN, which that call does not promise).
+ * qkv rows lie qkv_token_stride elements apart; q_out and the caches lie apart from them.
+ * Tokens whose slot is outside [0, max_slots) write no K/V; no two tokens may have the same
+ * slot. */
 int ccinfer_qkv_norm_rope(const void* qkv, int64_t qkv_token_stride, const void* q_norm_weight,
                           int q_norm_per_head, const void* k_norm_weight, int k_norm_per_head,
                           const int32_t* positions, const void* rope_cache,

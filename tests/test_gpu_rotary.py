@@ -632,3 +632,16 @@ def test_rows_whose_squares_are_under_the_smallest_normal_number(gpu):
             bound = np.abs(want) * R.BF16 + size * (R.F32 + share) * (1 + R.BF16) + 1e-38
             assert np.all(np.abs(got - want) <= bound), rotary
             assert np.abs(got).max(-1).min() > 2.0 ** -9  # (an answer of zeros is none)
+
+
+def test_rows_whose_sum_of_squares_passes_float32(gpu):
+    # stated: such a row comes out as zeros, its neighbours as they should
+    say("huge rows")
+    t, hq, hkv, d = 6, 2, 1, 64
+    s = make_norm(gpu, 16, t, hq, hkv, d, d, False)
+    s["qkv"][4] = (s["qkv"][4].float().abs() + 1).bfloat16() * 2.0 ** 64
+    q = run_norm(s, gpu, hq)
+    assert not q[4].any() and not s["k"][int(s["slot"][4])].any()
+    (wq, sq), _, _ = want_norm(s, hq, hkv, d, False, 1e-6, 0.0)
+    rest = [0, 1, 2, 3, 5]
+    R.assert_bf16(f64(q)[rest], wq[rest], sq[rest], "q")
