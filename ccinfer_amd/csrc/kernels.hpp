@@ -280,7 +280,6 @@ struct KvLayers {
     int64_t layer_stride = 0, scale_layer_stride = 0;
     int layers = 0, blocks = 0, heads = 0, block_size = 0;
     int64_t token_bytes = 0;  // of one token's heads
-    int64_t block_bytes() const { return token_bytes * block_size; }
 };
 
 // Blocks that the bitmap of free blocks covers at most.

@@ -124,8 +124,8 @@ __device__ __forceinline__ void copy_part(const KvLayers& kv, int part, int from
     c.finish(kv, from, to, tokens);
 }
 
-// The unit that every copy of these caches can move in: 16 bytes where every block starts at a
-// multiple of 16, else an element.
+// The unit that every copy of these caches can move in: 16 bytes where every token starts at a
+// multiple of 16 (an update's copies end behind a token), else an element.
 int copy_unit(const KvLayers& kv) {
     const uintptr_t all = reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v) |
                           static_cast<uintptr_t>(kv.layer_stride) |
