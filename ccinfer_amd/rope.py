@@ -33,6 +33,8 @@ def _frequencies(rotary_dim: int, theta: float, scaling: Optional[dict], op: str
         kind = ROPE_SCALINGS.index(scaling["type"])
         own = scaling.get("factors", ())
         _require(len(own) == (pairs if kind == 5 else 0), op)
+        if kind == 0 and "magnitude" in scaling:  # plain frequencies are linear ones over 1
+            scaling, kind = {"magnitude": scaling["magnitude"]}, 1
         params = (ctypes.c_double * (_PARAMS + len(own)))(
             scaling.get("factor", 1.0), scaling.get("original_max_position", 0.0),
             scaling.get("fast", 32.0 if kind == 3 else 4.0), scaling.get("slow", 1.0),

@@ -46,6 +46,21 @@ def test_plain_linear_ntk_and_factors():
     assert m == 1.25
 
 
+@pytest.mark.parametrize("kind", [{"type": "none"}, {"type": "linear", "factor": 2.0},
+                                  {"type": "ntk", "factor": 2.0},
+                                  {"type": "yarn", "factor": 2.0, "original_max_position": 4096},
+                                  {"type": "bands", "factor": 2.0, "original_max_position": 4096},
+                                  {"type": "factors", "factors": [1.5] * 16}])
+def test_a_magnitude_is_taken_with_every_scaling(kind):
+    f, own = cc.rope_frequencies(32, 1e4, kind)
+    got, m = cc.rope_frequencies(32, 1e4, {**kind, "magnitude": 1.25})
+    assert got == f and m == 1.25
+    assert cc.rope_frequencies(32, 1e4, {**kind, "magnitude": 0.0}) == (f, own)
+    for bad in (-1.0, NAN, INF):
+        with pytest.raises(cc.CcinferError):
+            cc.rope_frequencies(32, 1e4, {**kind, "magnitude": bad})
+
+
 def test_yarn_and_bands():
     r, theta, n, s = 128, 1e4, 4096, 16.0
     f = theta ** (-np.arange(0, r, 2) / r)
