@@ -242,30 +242,25 @@ def _size(query, *args) -> int:
     return _known_size(query, *args) if type(args[-1]) is int else query(*args)
 
 
-def _workspace_bytes(device, workspace: torch.Tensor) -> int:
-    """Bytes of a caller's workspace: contiguous (an expanded view has less memory than elements)
-    and on the device of the call's tensors."""
-    _require(workspace.is_cuda and workspace.get_device() == device.index
-             and workspace.is_contiguous(), "workspace")
-    return workspace.numel() * workspace.element_size()
-
-
-def _workspace(nbytes: int, device, workspace: Optional[torch.Tensor]):
+def _workspace(nbytes: int, device, workspace: Optional[torch.Tensor], least: int = 0):
+    """A workspace of nbytes and its size. A caller's is contiguous (an expanded view has less
+    memory than elements), on the device of the call's tensors and has at least nbytes, or
+    `least` bytes where that is given."""
     if nbytes == 0:
         return None, 0
-    if workspace is not None:
-        have = _workspace_bytes(device, workspace)
-        _require(have >= nbytes, "workspace")
-        return workspace, have
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+    if workspace is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+    have = workspace.numel() * workspace.element_size()
+    if have < (least or nbytes) or workspace.get_device() != device.index \
+            or not workspace.is_contiguous():
+        raise CcinferError(INVALID_ARGUMENT, "workspace")
+    return workspace, have
 
 
 def _prefill_workspace(nbytes: int, device, workspace: Optional[torch.Tensor]):
     """_workspace for the prefill calls, which also run in a workspace without the memory for
     split tiles that the size query counts in: the call itself refuses one that is too small."""
-    if nbytes == 0 or workspace is None:
-        return _workspace(nbytes, device, workspace)
-    return workspace, _workspace_bytes(device, workspace)
+    return _workspace(nbytes, device, workspace, least=1)
 
 
 def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

@@ -32,12 +32,11 @@ KV_INVALID_TABLE = 14  # status: a table row that the pool does not hold
 def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: str):
     """The cache arguments of the C ABI: pointers, layers, strides, blocks, heads, head_dim,
     block_size."""
-    _require(block_size > 0, op)
     fp8 = k_scale is not None
     dtype = torch.uint8 if fp8 else torch.bfloat16
     shape, stride = k_cache.shape, k_cache.stride()
     dims = len(shape)
-    _require(3 <= dims <= 5 and max(shape) < 2 ** 31 and k_cache.dtype is dtype
+    _require(3 <= dims <= 5 and 0 < block_size < 2 ** 31 and k_cache.dtype is dtype
              and v_cache.dtype is dtype and v_cache.shape == shape
              and k_cache.get_device() == dev and v_cache.get_device() == dev
              and fp8 == (v_scale is not None), op)
@@ -51,11 +50,12 @@ def _layers(k_cache, v_cache, k_scale, v_scale, block_size: int, dev: int, op: s
         _require((stride == vstride or layers == 1 or vstride[0] == stride[0])
                  and (stride[1:] == inner or k_cache[0].is_contiguous())
                  and (vstride[1:] == inner or v_cache[0].is_contiguous())
-                 and bs == block_size, op)
+                 and bs == block_size and layers < 2 ** 31 > nb and h < 2 ** 31 > d, op)
     else:
         nb, bs = (shape[0], shape[1]) if dims == 4 else (shape[0] // block_size, block_size)
         _require((dims == 4 or nb * bs == shape[0]) and k_cache.is_contiguous()
-                 and v_cache.is_contiguous() and bs == block_size, op)
+                 and v_cache.is_contiguous() and bs == block_size
+                 and nb < 2 ** 31 > h and d < 2 ** 31, op)
     ksp = vsp = None
     if fp8:
         need = nb * h * 16
@@ -140,9 +140,7 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
     _require(block_table.is_cuda, op)
     dev = current_device()
     shape, n, nb = block_table.shape, dst_rows.numel(), ref_counts.numel()
-    _require(len(shape) == 2 and max(shape) < 2 ** 31 and n < 2 ** 31 and nb < 2 ** 31
-             and 0 < cache_block_size < 2 ** 31
-             and block_table.dtype is _I32 and context_lens.dtype is _I32
+    _require(len(shape) == 2 and block_table.dtype is _I32 and context_lens.dtype is _I32
              and ref_counts.dtype is _I32 and dst_rows.dtype is _I32
              and block_table.get_device() == dev and context_lens.get_device() == dev
              and ref_counts.get_device() == dev and dst_rows.get_device() == dev
@@ -153,6 +151,7 @@ def update_block_tables(block_table: torch.Tensor, context_lens: torch.Tensor,
              and (lengths is None or _index(lengths, dev, op) == n)
              and (status is None or _index(status, dev, op) == 1), op)
     rows, width = shape
+    _require(rows < 2 ** 31 > width and n < 2 ** 31 > nb and 0 < cache_block_size < 2 ** 31, op)
     if status is None:
         status = torch.empty(1, dtype=_I32, device=block_table.device)
     copy_src = copy_dst = None
@@ -198,7 +197,9 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
     dev = current_device()
     _index(block_table, dev, op)
     _index(ref_counts, dev, op)
-    _require(block_table.dim() == 2 and max(block_table.shape) < 2 ** 31, op)
+    _require(block_table.dim() == 2, op)
+    rows, width = block_table.shape
+    _require(rows < 2 ** 31 > width, op)
     cache = _layers(k_cache, v_cache, k_scale, v_scale, cache_block_size, dev, op)
     nb = cache[7]
     _require(ref_counts.numel() == nb, op)
@@ -213,7 +214,6 @@ def compact_kv_blocks(block_table: torch.Tensor, ref_counts: torch.Tensor, k_cac
              and _index(remap, dev, op) == nb and _index(live, dev, op) == 1, op)
     ws, ws_bytes = _workspace(_known_size(compact_workspace_size, nb), block_table.device,
                               workspace)
-    rows, width = block_table.shape
     _check(_lib.load().ccinfer_compact_kv_blocks(
         block_table.data_ptr() or None, ref_counts.data_ptr(), rows, width, *cache,
         table.data_ptr() or None, refs.data_ptr(), remap.data_ptr(), live.data_ptr(),

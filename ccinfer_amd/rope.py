@@ -124,12 +124,12 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     dev = current_device()
     shape, qs, table = q.shape, q.stride(), rope_cache.shape
     _require(len(shape) == 3 == len(table) and table[2] == 2 and qs[2] == 1
-             and max(shape) < 2 ** 31 > table[0] and 2 * table[1] <= shape[2]
+             and shape[1] < 2 ** 31 > table[0] and 2 * table[1] <= shape[2] <= 1024
              and q.dtype is _BF16 and positions.dtype is _I32 and rope_cache.dtype is _F32
              and q.get_device() == dev and positions.get_device() == dev
              and rope_cache.get_device() == dev and positions.is_contiguous()
              and rope_cache.is_contiguous()
-             and positions.numel() == shape[0] > 0, op)
+             and 2 ** 31 > positions.numel() == shape[0] > 0, op)
     t, hq, d = shape
     if q_out is None:
         q_out = torch.empty(shape, dtype=_BF16, device=q.device)
