@@ -416,8 +416,9 @@ __global__ __launch_bounds__(kThreads) void update_plan_kernel(TableUpdate u, Kv
 // kThreads words, a word a lane, asked for at the start.
 // Bound by its chain of reads (plans and bitmap, source block, store): 48 beams of 8 layers 7.4
 // us, of which 25 MB of copies take 4.8, and 4 items 3.8; with the plan 11.3 and 7.3 in all. It
-// was 16.6 and 11.1 with a reduction for each sum and the copies' loads after the selection. A
-// step of 1024 rows that copies nothing takes 12.5.
+// was 16.6 and 11.1 with a reduction for each sum and the copies' loads after the selection. Rows
+// that grow by a token and copy nothing: 64 take 7.0 with the plan, 256 7.7, 1024 12.2, for under
+// 0.4 us of bytes.
 template <typename T, bool kSmall>
 __global__ __launch_bounds__(kThreads) void update_apply_kernel(TableUpdate u, KvLayers kv,
                                                                 int chunks, UpdateWorkspace ws) {

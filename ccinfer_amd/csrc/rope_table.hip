@@ -9,10 +9,15 @@
 //   r = n g - q        (one fused product and sum: rounded once, at most 1/2)
 // so r is off by the 2^-53 of g (3e-11 quarter turns at 10^6 positions) and goes to float32 with
 // 2^-24 of itself, into the Taylor series of sine and cosine on [-pi/4, pi/4], cut where the
-// next term is under 2e-9 ((pi/4)^11 / 11!).
+// next term is under 2e-9 ((pi/4)^11 / 11!). The series run in float32, and pi/2 and m are
+// rounded to it: an entry is off by 2.8e-8 of m in the mean (its nearest float32 by 2.0e-8), and
+// where m is no float32 itself by up to 2^-24 more, for all entries alike. With both constants in
+// two parts and m inside the series that was 2.6e-8 to 3.2e-8, and 42.8 to 44.3 us where this
+// takes 40.9 to 41.6: not kept.
 //
 // The table is only written, so the rate of plain stores bounds it: 2^20 positions x 32 pairs
-// (268 MB) take 40.8 us, 6.6 TB/s, where a fill of 2 GiB reaches 6.9. Two entries (16 bytes) a
+// (268 MB) take 40 to 45 us on different machines, 6.0 to 6.7 TB/s, where a fill of 2 GiB reaches
+// 6.9. Two entries (16 bytes) a
 // store, streamed; the reduction in three double operations keeps the arithmetic (about 27
 // operations an entry) under the stores' time.
 #include <hip/hip_runtime.h>

@@ -159,15 +159,24 @@ __global__ __launch_bounds__(kThreads) void rotary_rows_kernel(RotaryArgs a) {
 // (interleaved: eight), so there is nothing of this. Segments start at any even byte; the loads
 // and stores claim 2-byte alignment, which the hardware takes at full width.
 //
-// Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 38.4 us with the
-// norm and the cache write, 5.4 TB/s, and a copy of as many bytes 41.1; 8191 tokens x 40 heads
-// half rotated 31.0 us. What that took: eight wavefronts a SIMD (63 registers; at five, with two
+// Bound by memory: 12288 tokens of 16 q and 2 x 8 kv heads of 128 (208 MB) take 38.9 us with the
+// norm and the cache write, 5.3 TB/s, where a copy of as many bytes takes 40.2 and
+// ccinfer_qkv_prologue on the same rows, slots and positions 41.5 (three sets of inputs in turn;
+// one set again and again, which the last-level cache holds in part: 34.7, 29.3 and 34.7). Into
+// an fp8 cache 40.7, at the copy's rate 34.8; 8191 tokens x 40 heads half rotated 30.7. What that
+// took: eight wavefronts a SIMD (63 registers; at five, with two
 // rows a lane sharing (cos, sin) and weights, 46.8 us), stores with the streaming hint (41.5
 // without; a prefill that reads the rows afterwards takes the same time either way), and whole
 // lines a store (a lane's two segments side by side instead: 28 % more bytes written where they
-// are streamed). A half-layout row rotated in 50 or 120 of 128 elements takes nine lanes, so a
-// wavefront holds seven rows instead of eight, and loads in parts of lines: 40 us instead of 32
-// (one wavefront a row: 124).
+// are streamed).
+//
+// What is left. Half-layout widths that are no multiple of 16: segments that reach into one
+// another are stored twice in part and need a select an element in the sums. A row rotated in 50
+// or 120 of 128 elements also takes nine lanes, so a wavefront holds seven rows instead of eight:
+// 40 us instead of 32 (one wavefront a row: 124). With the norm, 12288 tokens of 16 q and 8 kv
+// heads: 120 of 128 65.0 us (128 of 128 38.9), all of 120 48.0. Few kv heads: a wavefront holds
+// rows of one section of one token, so with one kv head of 128 seven eighths of the K and V ones
+// are idle: 8 q and 1 kv heads run at 3.5 TB/s, 14 and 2 or 28 and 4 at 4.5.
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef f32x4 f32x4_a8 __attribute__((aligned(8)));
@@ -433,6 +442,8 @@ bool vec_plan(const RotaryArgs& a, bool interleaved, VecPlan& plan) {
     // wavefront. At nine chunks (7 rows or 4) the rotation of 8191 tokens x 40 heads takes 40 us
     // or 48, with norm and fp8 write 68 or 81; at five (12 or 8) a head of 64 rotated in 30 with
     // the norm 31 or 33; at six (10 or 8) the rotation 23.7 or 22.9, with the norm 28.1 or 25.9.
+    // At 17 to 21 (3 or 2) 4096 tokens x 40 heads of 272 to 336 take 38 to 42 or 44 to 47, with
+    // norm and write 54 to 59 or 66 to 69.
     plan.lanes = kWave / most * 2 >= kWave / power * 3 ? most : power;
     plan.power = plan.lanes == power;
     plan.whole = r % (interleaved ? kSegment : kChunkElems) == 0 && d % kChunkElems == 0;
