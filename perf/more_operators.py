@@ -296,7 +296,7 @@ def prepare(case, seed):
 
     if op in ("plan", "attn"):
         x["out"] = {"tree_mask": ints(x["total"], -(-x["nodes"] // 32)), "positions": ints(x["total"]),
-                    "slot_mapping": ints(x["total"]), "status": ints(1)}
+                    "slot_mapping": ints(x["total"]), "status": ints(c["rows"])}
     if op == "attn":
         x["mask"] = _plan_plain(x)[0]  # made once a step, for all layers
     elif op == "accept":
@@ -609,7 +609,7 @@ def _exact_ints(x, c, slot, ctx):
                 masks.append([np.uint32(bits >> 32 * w & 0xffffffff) for w in range(words)])
                 positions.append(before + len(path) - 1)
                 slots.append(slot(b, before + i))
-        return [_i32(np.array(masks, np.uint32).view(np.int32)), _i32(positions), _i32(slots), _i32([0])]
+        return [_i32(np.array(masks, np.uint32).view(np.int32)), _i32(positions), _i32(slots), _i32([0] * c["rows"])]
     draft, target = x["draft"].tolist(), x["target"].tolist()
     counts, nodes, tokens, lengths = [], [], [], []
     shape = (c["layers"], -1, c["hkv"])
