@@ -3,7 +3,8 @@
 The product is libccinfer_attn.so (built in-tree by ccinfer_amd.build). This package is the
 Python host side: a ctypes binding of the C ABI (`_lib`), torch-facing operators that mirror
 the reference's backend ops (`ops`), rotary positions (`rope`), pages of the cache (`pages`),
-and seeded synthetic workloads (`workloads`).
+trees of drafted tokens (`drafts`), decode over selected blocks (`sparse`), and seeded synthetic
+workloads (`workloads`).
 """
 from .ops import (  # noqa: F401
     ITEM_DECODE,
@@ -34,6 +35,19 @@ from .pages import (  # noqa: F401
     update_block_tables,
     update_tables_workspace_size,
 )
+from .drafts import (  # noqa: F401
+    accept_draft_tokens,
+    build_draft_tree,
+    tree_attention,
+    tree_attention_workspace_size,
+)
+from .sparse import (  # noqa: F401
+    score_kv_blocks,
+    select_kv_blocks,
+    sparse_decode_attention,
+    sparse_decode_workspace_size,
+    update_key_bounds,
+)
 from .rope import build_rope_cache, qkv_norm_rope, rope_frequencies, rotary_embedding  # noqa: F401
 
 __all__ = [
@@ -57,6 +71,8 @@ __all__ = [
     "fp8_scale_numel",
     "KV_EXHAUSTED",
     "KV_INVALID_TABLE",
+    "accept_draft_tokens",
+    "build_draft_tree",
     "build_rope_cache",
     "compact_kv_blocks",
     "compact_workspace_size",
@@ -64,6 +80,13 @@ __all__ = [
     "qkv_norm_rope",
     "rope_frequencies",
     "rotary_embedding",
+    "score_kv_blocks",
+    "select_kv_blocks",
+    "sparse_decode_attention",
+    "sparse_decode_workspace_size",
+    "tree_attention",
+    "tree_attention_workspace_size",
     "update_block_tables",
+    "update_key_bounds",
     "update_tables_workspace_size",
 ]

@@ -82,6 +82,21 @@ SIGNATURES = {
         [_vp, _vp, _c_int, _c_int] + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
         + [_vp] * 5 + [_c_size, _vp],
     ),
+    "ccinfer_build_draft_tree": (_c_int, [_vp] * 4 + [_c_int] * 6 + [_vp] * 5),
+    "ccinfer_tree_attention_workspace_size": (_c_size, [_c_int] * 8),
+    "ccinfer_tree_attention": (
+        _c_int, [_vp] * 10 + [_c_int] * 8 + [_vp, _c_size, _vp]),
+    "ccinfer_accept_draft_tokens": (
+        _c_int,
+        [_vp] * 6 + [_c_int] * 3 + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
+        + [_vp] * 5,
+    ),
+    "ccinfer_update_key_bounds": (_c_int, [_vp] * 6 + [_c_int] * 5 + [_vp]),
+    "ccinfer_score_kv_blocks": (_c_int, [_vp] * 5 + [_c_int] * 6 + [_vp]),
+    "ccinfer_select_kv_blocks": (_c_int, [_vp] * 2 + [_c_int] * 7 + [_vp, _vp]),
+    "ccinfer_sparse_decode_workspace_size": (_c_size, [_c_int] * 6),
+    "ccinfer_sparse_decode_attention": (
+        _c_int, [_vp] * 9 + [_c_int] * 7 + [_vp, _c_size, _vp]),
     "ccinfer_error_message": (ctypes.c_char_p, [_c_int]),
     "ccinfer_version": (ctypes.c_char_p, []),
 }

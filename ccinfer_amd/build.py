@@ -50,14 +50,19 @@ SOURCES = [
     CSRC / "rope_table.hip",
     CSRC / "rotary.hip",
     CSRC / "kv_pages.hip",
+    CSRC / "draft_tree.hip",
+    CSRC / "tree_attn.hip",
+    CSRC / "kv_select.hip",
+    CSRC / "sparse_attn.hip",
     CSRC / "capi.cpp",
     CSRC / "dropin" / "launchers.cpp",
     CSRC / "dropin" / "hip_backend.cpp",
 ]
 
-# Sources that do rely on NaN semantics: a NaN in a row reaches the fp8 cache as a NaN, and a
-# NaN parameter of the frequencies is refused.
-HONOR_NANS = {"rotary.hip", "rope_table.hip"}
+# Sources that do rely on NaN semantics: a NaN in a row reaches the fp8 cache as a NaN, a NaN
+# parameter of the frequencies is refused, and a NaN among keys, bounds or scores puts its block
+# before the others.
+HONOR_NANS = {"rotary.hip", "rope_table.hip", "kv_select.hip"}
 
 
 def _compile(src: Path) -> Path:

@@ -307,6 +307,36 @@ bool kv_layers_of(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
     return true;
 }
 
+// Shapes of the calls on drafted tokens: blocks of 16 tokens.
+bool drafts_ok(int batch_size, int total_tokens, int max_blocks_per_req, int cache_block_size) {
+    return batch_size > 0 && total_tokens > 0 && max_blocks_per_req > 0 &&
+           cache_block_size == 16 && fits_int(static_cast<int64_t>(max_blocks_per_req) * 16);
+}
+
+// `rows` tokens of q: head dims in pieces of eight elements.
+bool heads_ok(int rows, int num_q_heads, int num_kv_heads, int head_dim) {
+    return num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 &&
+           head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256 &&
+           fits_int(static_cast<int64_t>(rows) * num_q_heads);
+}
+
+// Shapes of the calls on bounds, scores and selected blocks.
+bool blocks_ok(int batch_size, int max_blocks_per_req, int num_q_heads, int num_kv_heads,
+               int head_dim, int cache_block_size) {
+    return batch_size > 0 && drafts_ok(batch_size, 1, max_blocks_per_req, cache_block_size) &&
+           heads_ok(batch_size, num_q_heads, num_kv_heads, head_dim) &&
+           fits_int(static_cast<int64_t>(batch_size) * num_kv_heads *
+                    ((max_blocks_per_req + int64_t{255}) / 256));
+}
+
+// The entries of a selection, and the workgroups of its attention, have 32-bit numbers.
+bool sparse_fits(int batch_size, int num_q_heads, int num_kv_heads, int num_selected) {
+    const int64_t items = static_cast<int64_t>(batch_size) * num_kv_heads *
+                          ((num_q_heads / num_kv_heads + 15) / 16);
+    return fits_int(static_cast<int64_t>(batch_size) * num_kv_heads * num_selected) &&
+           fits_int(items * (num_selected / 16 + int64_t{1}));
+}
+
 // Tables and counts alone, without the caches that they speak of.
 bool kv_pool_of(int num_blocks, int cache_block_size, KvLayers& kv) {
     if (num_blocks <= 0 || cache_block_size <= 0 ||
@@ -907,6 +937,228 @@ int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_cou
     return map_hip_error(compact_kv_blocks(
         block_table, ref_counts, static_cast<int64_t>(num_rows) * max_blocks_per_req, kv,
         block_table_out, ref_counts_out, remap, num_live, workspace, as_stream(stream)));
+}
+
+int ccinfer_build_draft_tree(const int32_t* parents, const int32_t* query_start_loc,
+                             const int32_t* context_lens, const int32_t* block_table,
+                             int batch_size, int total_tokens, int max_blocks_per_req,
+                             int max_nodes, int mask_words, int cache_block_size,
+                             int32_t* tree_mask, int32_t* positions, int32_t* slot_mapping,
+                             int32_t* status, void* stream) {
+    if (!parents || !query_start_loc || !context_lens || !block_table || !tree_mask ||
+        !positions || !slot_mapping || !status)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!drafts_ok(batch_size, total_tokens, max_blocks_per_req, cache_block_size) ||
+        max_nodes <= 0 || mask_words <= 0 || mask_words < (max_nodes - 1) / 32 + 1)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (batch_size > kTreeMaxRequests || max_nodes > kTreeMaxNodes ||
+        mask_words > kTreeMaxNodes / 32)
+        return CCINFER_ERR_UNSUPPORTED;
+    return map_hip_error(build_draft_tree(parents, query_start_loc, context_lens, block_table,
+                                          batch_size, total_tokens, max_blocks_per_req, mask_words,
+                                          max_nodes, tree_mask, positions, slot_mapping, status,
+                                          as_stream(stream)));
+}
+
+size_t ccinfer_tree_attention_workspace_size(int batch_size, int total_query_tokens,
+                                             int max_blocks_per_req, int mask_words,
+                                             int num_q_heads, int num_kv_heads, int head_dim,
+                                             int cache_block_size) {
+    if (!drafts_ok(batch_size, total_query_tokens, max_blocks_per_req, cache_block_size) ||
+        !heads_ok(total_query_tokens, num_q_heads, num_kv_heads, head_dim) || mask_words <= 0 ||
+        mask_words > kTreeMaxNodes / 32 ||
+        !tree_attention_supported(batch_size, total_query_tokens, max_blocks_per_req, num_q_heads,
+                                  num_kv_heads, head_dim, false))
+        return 0;
+    return tree_attention_workspace_bytes(total_query_tokens, num_q_heads, num_kv_heads, head_dim);
+}
+
+int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cache,
+                           const float* k_scale, const float* v_scale, const int32_t* block_table,
+                           const int32_t* query_start_loc, const int32_t* context_lens,
+                           const int32_t* tree_mask, void* output, int batch_size,
+                           int total_query_tokens, int max_blocks_per_req, int mask_words,
+                           int num_q_heads, int num_kv_heads, int head_dim, int cache_block_size,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k_cache || !v_cache || !block_table || !query_start_loc || !context_lens ||
+        !tree_mask || !output || (k_scale == nullptr) != (v_scale == nullptr))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!drafts_ok(batch_size, total_query_tokens, max_blocks_per_req, cache_block_size) ||
+        !heads_ok(total_query_tokens, num_q_heads, num_kv_heads, head_dim) || mask_words <= 0)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    const bool fp8 = k_scale != nullptr;
+    if (mask_words > kTreeMaxNodes / 32 ||
+        !tree_attention_supported(batch_size, total_query_tokens, max_blocks_per_req, num_q_heads,
+                                  num_kv_heads, head_dim, fp8))
+        return CCINFER_ERR_UNSUPPORTED;
+    if (!fast_aligned(q, k_cache, v_cache, output) || !aligned16(k_scale) || !aligned16(v_scale))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    const size_t need =
+        tree_attention_workspace_bytes(total_query_tokens, num_q_heads, num_kv_heads, head_dim);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    TreeAttention t;
+    t.q = q;
+    t.k = k_cache;
+    t.v = v_cache;
+    t.k_scale = k_scale;
+    t.v_scale = v_scale;
+    t.table = block_table;
+    t.qsl = query_start_loc;
+    t.ctx = context_lens;
+    t.mask = tree_mask;
+    t.out = output;
+    t.batch = batch_size;
+    t.total = total_query_tokens;
+    t.mbpr = max_blocks_per_req;
+    t.hq = num_q_heads;
+    t.hkv = num_kv_heads;
+    t.head_dim = head_dim;
+    t.words = mask_words;
+    return map_hip_error(tree_attention(t, workspace, as_stream(stream)));
+}
+
+int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
+                                const int32_t* parents, const int32_t* query_start_loc,
+                                const int32_t* context_lens, const int32_t* block_table,
+                                int batch_size, int total_tokens, int max_blocks_per_req,
+                                void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                                int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
+                                int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
+                                int32_t* context_lens_out, void* stream) {
+    if (!draft_tokens || !target_tokens || !parents || !query_start_loc || !context_lens ||
+        !block_table || !accepted || !accepted_nodes || !tokens || !context_lens_out)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    KvLayers kv;
+    const bool bare = !k_cache && !v_cache && !k_scale && !v_scale && num_layers == 0;
+    if (!bare && !kv_layers_of(k_cache, v_cache, k_scale, v_scale, num_layers, layer_stride,
+                               scale_layer_stride, num_blocks, n_kv_heads, head_dim,
+                               cache_block_size, kv))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (batch_size <= 0 || total_tokens <= 0 || max_blocks_per_req <= 0 || cache_block_size <= 0 ||
+        !fits_int(static_cast<int64_t>(max_blocks_per_req) * cache_block_size))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (batch_size > kTreeMaxRequests) return CCINFER_ERR_UNSUPPORTED;
+    AcceptDrafts a;
+    a.draft = draft_tokens;
+    a.target = target_tokens;
+    a.parents = parents;
+    a.qsl = query_start_loc;
+    a.ctx = context_lens;
+    a.table = block_table;
+    a.batch = batch_size;
+    a.total = total_tokens;
+    a.mbpr = max_blocks_per_req;
+    a.accepted = accepted;
+    a.nodes = accepted_nodes;
+    a.tokens = tokens;
+    a.lengths = context_lens_out;
+    return map_hip_error(accept_draft_tokens(a, kv, as_stream(stream)));
+}
+
+int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* key_bounds,
+                              const int32_t* block_table, const int32_t* context_lens,
+                              const int32_t* query_start_loc, int batch_size,
+                              int max_blocks_per_req, int num_kv_heads, int head_dim,
+                              int cache_block_size, void* stream) {
+    if (!k_cache || !key_bounds || !block_table || !context_lens)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!blocks_ok(batch_size, max_blocks_per_req, num_kv_heads, num_kv_heads, head_dim,
+                   cache_block_size))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (batch_size > kBoundsMaxRequests) return CCINFER_ERR_UNSUPPORTED;
+    const uintptr_t piece = k_scale != nullptr ? 8 : 16;  // of a key row, eight elements
+    if (reinterpret_cast<uintptr_t>(k_cache) % piece != 0 || !aligned16(key_bounds) ||
+        reinterpret_cast<uintptr_t>(k_scale) % 4 != 0)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    return map_hip_error(update_key_bounds(k_cache, k_scale, key_bounds, block_table, context_lens,
+                                           query_start_loc, batch_size, max_blocks_per_req,
+                                           num_kv_heads, head_dim, as_stream(stream)));
+}
+
+int ccinfer_score_kv_blocks(const void* q, const void* key_bounds, const int32_t* block_table,
+                            const int32_t* context_lens, float* scores, int batch_size,
+                            int max_blocks_per_req, int num_q_heads, int num_kv_heads,
+                            int head_dim, int cache_block_size, void* stream) {
+    if (!q || !key_bounds || !block_table || !context_lens || !scores)
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!blocks_ok(batch_size, max_blocks_per_req, num_q_heads, num_kv_heads, head_dim,
+                   cache_block_size))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned16(q) || !aligned16(key_bounds)) return CCINFER_ERR_INVALID_ARGUMENT;
+    return map_hip_error(score_kv_blocks(q, key_bounds, block_table, context_lens, scores,
+                                         batch_size, max_blocks_per_req, num_q_heads,
+                                         num_kv_heads, head_dim, as_stream(stream)));
+}
+
+int ccinfer_select_kv_blocks(const float* scores, const int32_t* context_lens, int batch_size,
+                             int max_blocks_per_req, int num_kv_heads, int num_selected,
+                             int first_blocks, int last_blocks, int cache_block_size,
+                             int32_t* selected, void* stream) {
+    if (!scores || !context_lens || !selected) return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!blocks_ok(batch_size, max_blocks_per_req, num_kv_heads, num_kv_heads, 8,
+                   cache_block_size))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (first_blocks < 0 || last_blocks < 0 || num_selected <= 0 ||
+        num_selected < static_cast<int64_t>(first_blocks) + last_blocks ||
+        !fits_int(static_cast<int64_t>(batch_size) * num_kv_heads * num_selected))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (max_blocks_per_req > kSelectMaxBlocks) return CCINFER_ERR_UNSUPPORTED;
+    return map_hip_error(select_kv_blocks(scores, context_lens, selected, batch_size,
+                                          max_blocks_per_req, num_kv_heads, num_selected,
+                                          first_blocks, last_blocks, as_stream(stream)));
+}
+
+size_t ccinfer_sparse_decode_workspace_size(int batch_size, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int num_selected, int cache_block_size) {
+    if (!blocks_ok(batch_size, 1, num_q_heads, num_kv_heads, head_dim, cache_block_size) ||
+        num_selected <= 0 ||
+        !sparse_fits(batch_size, num_q_heads, num_kv_heads, num_selected))
+        return 0;
+    return sparse_decode_workspace_bytes(batch_size, num_q_heads, num_kv_heads, head_dim,
+                                         num_selected);
+}
+
+int ccinfer_sparse_decode_attention(const void* q, const void* k_cache, const void* v_cache,
+                                    const float* k_scale, const float* v_scale,
+                                    const int32_t* block_table, const int32_t* context_lens,
+                                    const int32_t* selected, void* output, int batch_size,
+                                    int max_blocks_per_req, int num_q_heads, int num_kv_heads,
+                                    int head_dim, int num_selected, int cache_block_size,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k_cache || !v_cache || !block_table || !context_lens || !selected || !output ||
+        (k_scale == nullptr) != (v_scale == nullptr))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (!blocks_ok(batch_size, max_blocks_per_req, num_q_heads, num_kv_heads, head_dim,
+                   cache_block_size) ||
+        num_selected <= 0 ||
+        !sparse_fits(batch_size, num_q_heads, num_kv_heads, num_selected))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    if (k_scale != nullptr && head_dim != 64 && head_dim != 128) return CCINFER_ERR_UNSUPPORTED;
+    if (!fast_aligned(q, k_cache, v_cache, output) || !aligned16(k_scale) || !aligned16(v_scale))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    const size_t need = sparse_decode_workspace_bytes(batch_size, num_q_heads, num_kv_heads,
+                                                      head_dim, num_selected);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return CCINFER_ERR_INVALID_ARGUMENT;
+    SparseDecode s;
+    s.q = q;
+    s.k = k_cache;
+    s.v = v_cache;
+    s.k_scale = k_scale;
+    s.v_scale = v_scale;
+    s.table = block_table;
+    s.ctx = context_lens;
+    s.selected = selected;
+    s.out = output;
+    s.batch = batch_size;
+    s.mbpr = max_blocks_per_req;
+    s.hq = num_q_heads;
+    s.hkv = num_kv_heads;
+    s.head_dim = head_dim;
+    s.take = num_selected;
+    return map_hip_error(sparse_decode(s, workspace, as_stream(stream)));
 }
 
 const char* ccinfer_error_message(int code) {

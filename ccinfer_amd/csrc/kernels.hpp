@@ -315,4 +315,81 @@ hipError_t compact_kv_blocks(const int32_t* table, const int32_t* refs, int64_t 
                              int32_t* remap, int32_t* num_live, void* workspace,
                              hipStream_t stream);
 
+// ---- drafted tokens -------------------------------------------------------------
+// Requests of a call, and nodes (drafted tokens) of a request, at most.
+constexpr int kTreeMaxRequests = 2048;
+constexpr int kTreeMaxNodes = 2048;
+
+struct TreeAttention {
+    const void* q = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    const float* k_scale = nullptr;  // fp8 cache
+    const float* v_scale = nullptr;
+    const int32_t* table = nullptr;
+    const int32_t* qsl = nullptr;
+    const int32_t* ctx = nullptr;
+    const int32_t* mask = nullptr;  // [total][words]
+    void* out = nullptr;
+    int batch = 0, total = 0, mbpr = 0, hq = 0, hkv = 0, head_dim = 0, words = 0;
+};
+
+bool tree_attention_supported(int batch, int total, int mbpr, int hq, int hkv, int head_dim,
+                              bool fp8);
+size_t tree_attention_workspace_bytes(int total, int hq, int hkv, int head_dim);
+hipError_t tree_attention(const TreeAttention& t, void* workspace, hipStream_t stream);
+
+hipError_t build_draft_tree(const int32_t* parents, const int32_t* qsl, const int32_t* ctx,
+                            const int32_t* table, int batch, int total, int mbpr, int words,
+                            int max_nodes, int32_t* mask, int32_t* positions, int32_t* slots,
+                            int32_t* status, hipStream_t stream);
+
+struct AcceptDrafts {
+    const int32_t* draft = nullptr;
+    const int32_t* target = nullptr;
+    const int32_t* parents = nullptr;
+    const int32_t* qsl = nullptr;
+    const int32_t* ctx = nullptr;
+    const int32_t* table = nullptr;
+    int batch = 0, total = 0, mbpr = 0;
+    int32_t* accepted = nullptr;
+    int32_t* nodes = nullptr;
+    int32_t* tokens = nullptr;
+    int32_t* lengths = nullptr;
+};
+
+// kv.layers 0: no cache.
+hipError_t accept_draft_tokens(const AcceptDrafts& a, const KvLayers& kv, hipStream_t stream);
+
+// ---- decode over selected blocks ---------------------------------------------------
+constexpr int kBoundsMaxRequests = 2048;
+constexpr int kSelectMaxBlocks = 1 << 16;  // of a table row
+
+hipError_t update_key_bounds(const void* k, const float* k_scale, void* bounds,
+                             const int32_t* table, const int32_t* ctx, const int32_t* qsl,
+                             int batch, int mbpr, int hkv, int head_dim, hipStream_t stream);
+
+hipError_t score_kv_blocks(const void* q, const void* bounds, const int32_t* table,
+                           const int32_t* ctx, float* scores, int batch, int mbpr, int hq, int hkv,
+                           int head_dim, hipStream_t stream);
+
+hipError_t select_kv_blocks(const float* scores, const int32_t* ctx, int32_t* selected, int batch,
+                            int mbpr, int hkv, int take, int first, int last, hipStream_t stream);
+
+struct SparseDecode {
+    const void* q = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    const float* k_scale = nullptr;  // fp8 cache
+    const float* v_scale = nullptr;
+    const int32_t* table = nullptr;
+    const int32_t* ctx = nullptr;
+    const int32_t* selected = nullptr;  // [batch][hkv][take]
+    void* out = nullptr;
+    int batch = 0, mbpr = 0, hq = 0, hkv = 0, head_dim = 0, take = 0;
+};
+
+size_t sparse_decode_workspace_bytes(int batch, int hq, int hkv, int head_dim, int take);
+hipError_t sparse_decode(const SparseDecode& s, void* workspace, hipStream_t stream);
+
 }  // namespace ccinfer::hipk

@@ -453,6 +453,131 @@ int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_cou
                               int32_t* num_live, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* ---- drafted tokens ---------------------------------------------------------------------
+ * A step that checks several drafted tokens a request at once. Request b has n = query_start_loc
+ * [b + 1] - query_start_loc[b] nodes; context_lens[b] counts them, as prefill does its new tokens:
+ * node i lies at position context_lens[b] - n + i of the cache, whatever its depth in the tree.
+ * parents[t] is the request's node from which node t goes on (lower than its own number), -1 for
+ * one that goes on from the committed context. At most 2048 requests a call and 2048 nodes a
+ * request. The reference decodes one token a request and step (src/backend/params.h:148-211). */
+
+/* From parents [total_tokens]: tree_mask [total_tokens][mask_words] (bit j of a row, bit j % 32 of
+ * word j / 32: the node sees the request's node j; its ancestors and itself), positions
+ * [total_tokens] (of rotary embeddings: committed tokens + depth) and slot_mapping [total_tokens]
+ * (cache slot of each node, blocks of 16 tokens). mask_words at least max_nodes / 32, rounded up.
+ * status [batch_size]: CCINFER_OK, or CCINFER_ERR_INVALID_ARGUMENT for a request with more than
+ * max_nodes nodes, fewer context tokens than nodes, or nodes outside [0, total_tokens) (its rows
+ * then get no mask, position -1 and slot -1), with a parent out of range (taken as -1) or without
+ * a block for a node (slot -1). */
+int ccinfer_build_draft_tree(const int32_t* parents, const int32_t* query_start_loc,
+                             const int32_t* context_lens, const int32_t* block_table,
+                             int batch_size, int total_tokens, int max_blocks_per_req,
+                             int max_nodes, int mask_words, int cache_block_size,
+                             int32_t* tree_mask, int32_t* positions, int32_t* slot_mapping,
+                             int32_t* status, void* stream);
+
+/* Workspace bytes of ccinfer_tree_attention (0 for an invalid or unsupported shape). */
+size_t ccinfer_tree_attention_workspace_size(int batch_size, int total_query_tokens,
+                                             int max_blocks_per_req, int mask_words,
+                                             int num_q_heads, int num_kv_heads, int head_dim,
+                                             int cache_block_size);
+
+/* ccinfer_prefill_attention with a mask among the new tokens in place of their order: row i of
+ * request b sees the positions before its request's nodes and node j where bit j of tree_mask
+ * [query_start_loc[b] + i] is set (any mask, also one without itself; a node past the mask's words
+ * is seen by none). Rows that see nothing become zeros; rows of no request, and of requests whose
+ * context is shorter than their nodes, are left as they are. A node's K and V that a row does not
+ * see do not reach it, infinities and NaN included. k_scale / v_scale NULL: a bf16 cache, head_dim
+ * a multiple of 8 up to 256; else an fp8 cache (ccinfer_write_kv_cache_fp8), head_dim 64 or 128;
+ * CCINFER_ERR_UNSUPPORTED for others, for more than 2048 requests or 64 mask words, and for batches
+ * whose rows and tables together pass 2^30 units of work. q, caches, scales and output 16-byte
+ * aligned. The workspace needs no initialisation. */
+int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cache,
+                           const float* k_scale, const float* v_scale, const int32_t* block_table,
+                           const int32_t* query_start_loc, const int32_t* context_lens,
+                           const int32_t* tree_mask, void* output, int batch_size,
+                           int total_query_tokens, int max_blocks_per_req, int mask_words,
+                           int num_q_heads, int num_kv_heads, int head_dim, int cache_block_size,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the model confirms of the trees. target_tokens[t] is the token that the model says after
+ * node t. The path of a request starts at node 0 (the token the last step ended with, always
+ * taken) and goes on to the lowest child whose draft_tokens entry equals its parent's target.
+ * accepted [batch_size]: its length; accepted_nodes [total_tokens]: its nodes, from the request's
+ * first row on, -1 behind them; tokens [total_tokens]: the new tokens, target_tokens of those
+ * nodes, -1 behind them (the last one is the next step's node 0); context_lens_out [batch_size]:
+ * the context without the nodes that were not taken. K and V (and scales) of the k-th node of the
+ * path move to the position behind the committed tokens that k counts, in every layer of the
+ * caches (as in the calls on pages; caches NULL with num_layers 0: none, and a later call with the
+ * same arguments for each layer moves them). Blocks that hold nodes belong to one request alone.
+ * A row without a block in the pool is not moved. A request without nodes, with more than 2048,
+ * with fewer context tokens than nodes or with nodes outside [0, total_tokens): accepted 0, its
+ * context as it is. context_lens_out may not be context_lens where the call is made again. */
+int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
+                                const int32_t* parents, const int32_t* query_start_loc,
+                                const int32_t* context_lens, const int32_t* block_table,
+                                int batch_size, int total_tokens, int max_blocks_per_req,
+                                void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                                int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
+                                int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
+                                int32_t* context_lens_out, void* stream);
+
+/* ---- decode over selected blocks of the context ----------------------------------------
+ * Decode that reads the blocks in which a query's weight can lie. Beside each layer's K lie
+ * key_bounds, bf16 [num_blocks][num_kv_heads][2][head_dim]: the smallest and the largest of each
+ * block's keys, element by element (1/16 of the cache's bytes). Blocks of 16 tokens. Several
+ * query tokens of one request are rows of their own, with the same table row. */
+
+/* The bounds of the blocks that hold the newest tokens of each row, query_start_loc[b + 1] -
+ * query_start_loc[b] of them (query_start_loc NULL: one; no fewer than were written or moved since
+ * the last call), over all their positions below context_lens[b]. A key that is NaN makes both
+ * bounds of its element NaN. With k_scale: an fp8 cache; bounds are rounded to bf16 where a scale is no power of two. Blocks that
+ * are shared by rows are whole (other sharings: the last one written stays). At most 2048 rows
+ * (CCINFER_ERR_UNSUPPORTED). head_dim a multiple of 8 up to 256. */
+int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* key_bounds,
+                              const int32_t* block_table, const int32_t* context_lens,
+                              const int32_t* query_start_loc, int batch_size,
+                              int max_blocks_per_req, int num_kv_heads, int head_dim,
+                              int cache_block_size, void* stream);
+
+/* scores [batch_size][num_kv_heads][max_blocks_per_req] float: for block j of the row the largest,
+ * over the query heads of the kv head, of sum_d max(q_d lo_d, q_d hi_d) / sqrt(head_dim): no key
+ * of the block gives a larger logit. -infinity past the context, for negative table entries, and
+ * for rows whose context the table does not hold; NaN where a bound or q is NaN or a bound is
+ * infinite. */
+int ccinfer_score_kv_blocks(const void* q, const void* key_bounds, const int32_t* block_table,
+                            const int32_t* context_lens, float* scores, int batch_size,
+                            int max_blocks_per_req, int num_q_heads, int num_kv_heads,
+                            int head_dim, int cache_block_size, void* stream);
+
+/* selected [batch_size][num_kv_heads][num_selected]: the row's first `first_blocks` and last
+ * `last_blocks` blocks, and of the others those with the highest scores (NaN before all, equal
+ * ones by the lower number), in ascending order; all of them where they are no more than
+ * num_selected; -1 behind them. num_selected at least first_blocks + last_blocks; at most 2^16
+ * blocks a row (CCINFER_ERR_UNSUPPORTED). */
+int ccinfer_select_kv_blocks(const float* scores, const int32_t* context_lens, int batch_size,
+                             int max_blocks_per_req, int num_kv_heads, int num_selected,
+                             int first_blocks, int last_blocks, int cache_block_size,
+                             int32_t* selected, void* stream);
+
+/* Workspace bytes of ccinfer_sparse_decode_attention (0: none needed, or an invalid shape). */
+size_t ccinfer_sparse_decode_workspace_size(int batch_size, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int num_selected, int cache_block_size);
+
+/* Decode attention of each (row, kv head) over the positions below context_lens[b] that lie in its
+ * blocks selected [batch_size][num_kv_heads][num_selected] (numbers within the row; ones outside
+ * the context, and of negative table entries, are passed over; one that is named twice counts
+ * twice). Zeros for a row that sees nothing or whose context the table does not hold. Caches, head
+ * dims and alignment as in ccinfer_tree_attention. */
+int ccinfer_sparse_decode_attention(const void* q, const void* k_cache, const void* v_cache,
+                                    const float* k_scale, const float* v_scale,
+                                    const int32_t* block_table, const int32_t* context_lens,
+                                    const int32_t* selected, void* output, int batch_size,
+                                    int max_blocks_per_req, int num_q_heads, int num_kv_heads,
+                                    int head_dim, int num_selected, int cache_block_size,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* Human-readable text for a status code (the reference's error_message()). */
 const char* ccinfer_error_message(int code);
 
