@@ -37,15 +37,18 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int32_t* unwr
     return (const __attribute__((address_space(4))) int32_t*)(reinterpret_cast<uintptr_t>(p));
 }
 
-// One layer's cache. dr <= D dims a row, a multiple of 8 (the rest of D counts as zeros).
-template <bool F8>
+// One layer's cache of rows of D dims, or, padded, of dr < D, a multiple of 8 (the rest of D counts
+// as zeros).
+template <int D, bool F8, bool Pad>
 struct Cache {
+    static constexpr bool kF8 = F8;
     const std::conditional_t<F8, uint8_t, __bf16>* k;
     const std::conditional_t<F8, uint8_t, __bf16>* v;
     const float* ks;
     const float* vs;
     int hkv;
     int dr;
+    __device__ __forceinline__ int dims() const { return Pad ? dr : D; }
 };
 
 // One chunk: two blocks, wave-uniform. Tokens [0, lim) of a block that is `on` are there; what
@@ -94,25 +97,39 @@ __device__ __forceinline__ int q_dim(int kk, int g) {
     return F8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : (kk * 4 + g) * 8;
 }
 
-template <int D, bool F8>
-__device__ __forceinline__ void load_k(KRegs<D, F8>& r, const Cache<F8>& c, const Pair& p, int h,
-                                       int lane) {
+// A block's first row of head h, wave-uniform: loads take it from scalar registers and a 32-bit
+// offset a lane (a block has at most 2^30 bytes).
+template <class Elem, class C>
+__device__ __forceinline__ const Elem* block_rows(const Elem* base, const C& c, int pb, int h) {
+    return base + (static_cast<int64_t>(pb) * kBlock * c.hkv + h) * c.dims();
+}
+
+template <class C>
+__device__ __forceinline__ u32x4 load_scales(const float* base, const C& c, int pb, int h, int g) {
+    return load16(base + (static_cast<int64_t>(pb) * c.hkv + h) * kBlock +
+                  static_cast<uint32_t>(4 * g));
+}
+
+template <int D, bool F8, bool Pad>
+__device__ __forceinline__ void load_k(KRegs<D, F8>& r, const Cache<D, F8, Pad>& c, const Pair& p,
+                                       int h, int lane) {
     const int i = lane & 15, g = lane >> 4;
+    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims();
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const int64_t slot = static_cast<int64_t>(p.pb[b]) * kBlock + min(i, p.lim[b] - 1);
-        const auto* row = c.k + (slot * c.hkv + h) * c.dr;
+        const auto* blk = block_rows(c.k, c, p.pb[b], h);
+        const uint32_t row = static_cast<uint32_t>(min(i, p.lim[b] - 1)) * stride;
         if constexpr (F8) {
 #pragma unroll
             for (int s = 0; s < Shape<D>::kSteps / 2; ++s)
-                r.k[b][s] = load16(row + 64 * s + 16 * g);
-            r.s[b] = load16(c.ks + (static_cast<int64_t>(p.pb[b]) * c.hkv + h) * kBlock + 4 * g);
+                r.k[b][s] = load16(blk + (row + 64 * s + 16 * g));
+            r.s[b] = load_scales(c.ks, c, p.pb[b], h, g);
         } else {
 #pragma unroll
             for (int kk = 0; kk < Shape<D>::kSteps; ++kk) {
                 const int dim = q_dim<false>(kk, g);
-                const bool ok = dim < c.dr;
-                r.k[b][kk] = load16(row + (ok ? dim : 0));
+                const bool ok = !Pad || dim < c.dr;
+                r.k[b][kk] = load16(blk + (row + (ok ? dim : 0)));
                 // a dim past the row meets q's zero, but 0 x inf is none
                 if (!ok) r.k[b][kk] = u32x4{0u, 0u, 0u, 0u};
             }
@@ -120,27 +137,28 @@ __device__ __forceinline__ void load_k(KRegs<D, F8>& r, const Cache<F8>& c, cons
     }
 }
 
-template <int D, bool F8>
-__device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<F8>& c, const Pair& p, int h,
-                                       int lane) {
+template <int D, bool F8, bool Pad>
+__device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<D, F8, Pad>& c, const Pair& p,
+                                       int h, int lane) {
     constexpr int NV = Shape<D>::kNV;
     const int i = lane & 15, g = lane >> 4;
+    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims();
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int b = e >> 2;
-        const int64_t slot =
-            static_cast<int64_t>(p.pb[b]) * kBlock + min(4 * g + (e & 3), p.lim[b] - 1);
-        const auto* row = c.v + (slot * c.hkv + h) * c.dr;
+        const auto* blk = block_rows(c.v, c, p.pb[b], h);
+        const uint32_t row = static_cast<uint32_t>(min(4 * g + (e & 3), p.lim[b] - 1)) * stride;
         if constexpr (F8) {
             if constexpr (NV == 8) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(row + i * NV);
+                const u32x2 w = *reinterpret_cast<const u32x2*>(blk + (row + i * NV));
                 r.v[e][0] = w[0];
                 r.v[e][1] = w[1];
             } else {
-                r.v[e][0] = *reinterpret_cast<const uint32_t*>(row + i * NV);
+                r.v[e][0] = *reinterpret_cast<const uint32_t*>(blk + (row + i * NV));
             }
         } else if constexpr (NV == 4) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(row + (i * NV < c.dr ? i * NV : 0));
+            const u32x2 w =
+                *reinterpret_cast<const u32x2*>(blk + (row + (!Pad || i * NV < c.dr ? i * NV : 0)));
             r.v[e][0] = w[0];
             r.v[e][1] = w[1];
         } else {
@@ -148,7 +166,7 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<F8>& c, cons
 #pragma unroll
             for (int x = 0; x < NV / 8; ++x) {
                 const int dim = i * NV + 8 * x;
-                const u32x4 w = load16(row + (dim < c.dr ? dim : 0));
+                const u32x4 w = load16(blk + (row + (!Pad || dim < c.dr ? dim : 0)));
 #pragma unroll
                 for (int y = 0; y < 4; ++y) r.v[e][4 * x + y] = w[y];
             }
@@ -156,8 +174,7 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<F8>& c, cons
     }
     if constexpr (F8) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-            r.s[b] = load16(c.vs + (static_cast<int64_t>(p.pb[b]) * c.hkv + h) * kBlock + 4 * g);
+        for (int b = 0; b < 2; ++b) r.s[b] = load_scales(c.vs, c, p.pb[b], h, g);
     }
 }
 
@@ -188,72 +205,53 @@ __device__ __forceinline__ uint32_t v_word(const VRegs<D, F8>& r, int e, int w) 
     }
 }
 
-// Whether an infinity or a NaN lies among this lane's V.
+// Zeros in place of the infinities and NaN of this lane's V; whether there were any. (An exponent
+// of all ones plus one, or an fp8 NaN's seven ones plus one, carries into the sign's place.)
 template <int D, bool F8>
-__device__ __forceinline__ bool v_unbounded(const VRegs<D, F8>& r) {
-    bool bad = false;
+__device__ __forceinline__ bool clear_unbounded(VRegs<D, F8>& r) {
+    constexpr uint32_t kExp = F8 ? 0x7f7f7f7fu : 0x7f807f80u;
+    constexpr uint32_t kOne = F8 ? 0x01010101u : 0x00800080u;
+    constexpr uint32_t kSign = F8 ? 0x80808080u : 0x80008000u;
+    uint32_t any = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int w = 0; w < Shape<D>::kVWords; ++w) {
-            const uint32_t x = v_word<D, F8>(r, e, w);
-            bad |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-        }
-    return bad;
-}
-
-// The second product of a chunk in which some rows do not see a token whose V is unbounded: token
-// by token, so that only rows that see it meet it (p is -0 where they do not). Lane (i, g) holds dims NV i .. of tokens
-// T(g, e); lane (j, g) needs dims NV (4 g + r) .. of every token.
-template <int D, bool F8, int NT>
-__device__ __forceinline__ void pv_by_token(State<D, NT>& st, const VRegs<D, F8>& v,
-                                                      const float (&p)[NT][8], int lane) {
-    constexpr int NV = Shape<D>::kNV;
-    const int j = lane & 15, g = lane >> 4;
-#pragma unroll 1
-    for (int from = 0; from < 4; ++from)
+        for (auto& w : r.v[e]) any |= ((w & kExp) + kOne) & kSign;
+    const bool found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+    if (found) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float pe[NT];
+        for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) pe[t] = __shfl(p[t][e], from * 16 + j);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int w = 0; w < NV / 2; ++w) {
-                    const uint32_t x = static_cast<uint32_t>(
-                        __shfl(static_cast<int>(v_word<D, F8>(v, e, w)), from * 16 + 4 * g + r));
-                    const float lo = __uint_as_float(x << 16);
-                    const float hi = __uint_as_float(x & 0xffff0000u);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const bool sees = __float_as_uint(pe[t]) != 0x80000000u;
-                        st.acc[t][2 * w][r] += sees ? pe[t] * lo : 0.f;
-                        st.acc[t][2 * w + 1][r] += sees ? pe[t] * hi : 0.f;
-                    }
-                }
-        }
+            for (auto& w : r.v[e]) {
+                const uint32_t bad = ((w & kExp) + kOne) & kSign;
+                w &= ~((bad >> (F8 ? 7 : 15)) * (F8 ? 0xffu : 0xffffu));
+            }
+    }
+    return found;
 }
 
 // Chunks first, first + stride, ... below last of the rows. chunk(c): the Pair of chunk c (asked
 // for two chunks ahead: the ids' way to the scalar registers is hidden behind a chunk's work).
 // seen(c, t, bits): false where every row of tile t sees all that is there of the chunk, else
-// bits has a bit for each of its 32 tokens that this lane's row sees.
-template <int D, bool F8, int NT, class Chunks, class Seen>
-__device__ __forceinline__ void attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
-                                       const Cache<F8>& cache, int h, int first, int last,
+// bits has a bit for each of its 32 tokens that this lane's row sees. In such chunks the matrix
+// product leaves out infinities and NaN of V, which would reach rows that do not see their token
+// (0 x inf); true if there were any: add_unbounded then brings them to the rows that do.
+template <int D, bool F8, bool Pad, int NT, class Chunks, class Seen>
+__device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
+                                       const Cache<D, F8, Pad>& cache, int h, int first, int last,
                                        int stride, float scale_log2, int lane, Chunks chunk,
                                        Seen seen) {
     constexpr int S = Shape<D>::kSteps;
     constexpr int NV = Shape<D>::kNV;
-    if (first >= last) return;
+    if (first >= last) return false;
+    bool left_out = false;
     const int g = lane >> 4;
     KRegs<D, F8> k;
     VRegs<D, F8> v;
     Pair cur = chunk(first);
     Pair next = chunk(min(first + stride, last - 1));
-    load_k<D, F8>(k, cache, cur, h, lane);
-    load_v<D, F8>(v, cache, cur, h, lane);
+    load_k(k, cache, cur, h, lane);
+    load_v(v, cache, cur, h, lane);
     for (int c = first;; c += stride) {
         const bool more = c + stride < last;
         const Pair after = chunk(min(c + 2 * stride, last - 1));
@@ -289,7 +287,7 @@ __device__ __forceinline__ void attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
                     sc[t][4 * b + r] = s4[t][r] * f;
                 }
         }
-        if (more) load_k<D, F8>(k, cache, next, h, lane);
+        if (more) load_k(k, cache, next, h, lane);
         if (cur.any()) {
             bool hidden = false;  // wave-uniform: some score is masked
 #pragma unroll
@@ -348,45 +346,87 @@ __device__ __forceinline__ void attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
 #pragma unroll
                     for (int n = 0; n < NV; ++n) st.acc[t][n] = st.acc[t][n] * alpha[t];
             }
-            if (hidden && __builtin_amdgcn_ballot_w64(v_unbounded<D, F8>(v)) != 0) {
+            if (hidden) left_out |= clear_unbounded<D, F8>(v);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                u32x4 vw;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1),
+                                        v_word<D, F8>(v, 2 * x + 1, n >> 1), n & 1);
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[t][e] = sc[t][e] == kNegInf ? -0.f : p[t][e];
-                pv_by_token<D, F8, NT>(st, v, p, lane);
-            } else {
-#pragma unroll
-                for (int n = 0; n < NV; ++n) {
-                    u32x4 vw;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1),
-                                            v_word<D, F8>(v, 2 * x + 1, n >> 1), n & 1);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        st.acc[t][n] =
-                            mfma16x16x32(__builtin_bit_cast(bf16x8, vw), pop[t], st.acc[t][n]);
-                }
+                    st.acc[t][n] =
+                        mfma16x16x32(__builtin_bit_cast(bf16x8, vw), pop[t], st.acc[t][n]);
             }
         }
         if (!more) break;
-        load_v<D, F8>(v, cache, next, h, lane);
+        load_v(v, cache, next, h, lane);
         cur = next;
         next = after;
+    }
+    return left_out;
+}
+
+// The infinities and NaN of V that attend left out, added to the rows that see their tokens (a
+// sum with one in it is one, whatever its weight). Rare, and written for few registers: element
+// by element.
+template <int D, bool F8, bool Pad, int NT, class Chunks, class Seen>
+__device__ __forceinline__ void add_unbounded(State<D, NT>& st, const Cache<D, F8, Pad>& cache,
+                                              int h, int first, int last, int stride, int lane,
+                                              Chunks chunk, Seen seen) {
+    constexpr int NV = Shape<D>::kNV;
+    for (int c = first; c < last; c += stride) {
+        uint32_t bits[NT];
+        bool some = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            bits[t] = 0;
+            some |= seen(c, t, bits[t]);
+        }
+        if (!some) continue;
+        const Pair p = chunk(c);
+#pragma unroll 1
+        for (int key = 0; key < kChunk; ++key) {
+            const int b = key >> 4;
+            if (!p.on[b] || (key & 15) >= p.lim[b]) continue;
+            const int64_t slot = static_cast<int64_t>(p.pb[b]) * kBlock + (key & 15);
+            const auto* row = cache.v + (slot * cache.hkv + h) * cache.dims();
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int n = 0; n < NV; ++n) {
+                    const int dim = NV * (4 * (lane >> 4) + r) + n;
+                    uint32_t f = 0;
+                    if (!Pad || dim < cache.dr) {
+                        if constexpr (F8)
+                            f = (row[dim] & 0x7f) == 0x7f ? 0x7fc00000u : 0u;
+                        else
+                            f = static_cast<uint32_t>(
+                                    reinterpret_cast<const uint16_t*>(row)[dim]) << 16;
+                    }
+                    const bool bad = (f & 0x7f800000u) == 0x7f800000u;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        if (bad && ((bits[t] >> key) & 1u) != 0)
+                            st.acc[t][n][r] += __uint_as_float(f);
+                }
+        }
     }
 }
 
 // The q operand of a tile: lane (j, g) holds the dims q_dim(kk, g) .. + 8 of its row, zeros for
 // a row that is not there and dims past the row's end.
-template <int D, bool F8>
+template <int D, bool F8, bool Pad>
 __device__ __forceinline__ void load_q(bf16x8 (&q)[Shape<D>::kSteps], const __bf16* row, bool live,
                                        int dr, int lane) {
 #pragma unroll
     for (int kk = 0; kk < Shape<D>::kSteps; ++kk) {
         const int dim = q_dim<F8>(kk, lane >> 4);
-        const bool ok = live && dim < dr;
-        u32x4 w = {0u, 0u, 0u, 0u};
-        if (ok) w = load16(row + dim);
+        // (a row that is not there points at one that is)
+        const bool ok = live && (!Pad || dim < dr);
+        u32x4 w = load16(row + (!Pad || dim < dr ? dim : 0));
+        if (!ok) w = u32x4{0u, 0u, 0u, 0u};
         q[kk] = __builtin_bit_cast(bf16x8, w);
     }
 }

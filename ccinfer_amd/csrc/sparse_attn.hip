@@ -21,10 +21,10 @@ using namespace rows;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTile = 16;  // query heads of a workgroup
 
-template <bool F8>
+template <int D, bool F8, bool Pad>
 struct SparseArgs {
     const __bf16* q;
-    Cache<F8> cache;
+    Cache<D, F8, Pad> cache;
     const int32_t* table;
     const int32_t* ctx;
     const int32_t* selected;
@@ -40,12 +40,12 @@ __device__ __forceinline__ int decode_ctx(int c, int mbpr) {
     return c > 0 && (static_cast<int64_t>(c) + kBlock - 1) / kBlock <= mbpr ? c : 0;
 }
 
-template <int D, bool F8>
-__global__ __launch_bounds__(kThreads, 2) void sparse_decode_kernel(SparseArgs<F8> a) {
+template <int D, bool F8, bool Pad>
+__global__ __launch_bounds__(kThreads, 2) void sparse_decode_kernel(SparseArgs<D, F8, Pad> a) {
     __shared__ Parts<D, 1> parts;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hkv = a.cache.hkv, dr = a.cache.dr;
+    const int hkv = a.cache.hkv, dr = a.cache.dims();
     const int G = a.hq / hkv;
     const int split = blockIdx.x % a.splits;
     const int item = blockIdx.x / a.splits;  // ((b * hkv) + h) * tiles + tile
@@ -72,10 +72,10 @@ __global__ __launch_bounds__(kThreads, 2) void sparse_decode_kernel(SparseArgs<F
     st.clear();
     bf16x8 q[1][Shape<D>::kSteps];
     const int row = lane & 15;
-    load_q<D, F8>(q[0],
-                  a.q + (static_cast<int64_t>(b) * a.hq + head0 + min(row, heads - 1)) * dr,
-                  row < heads, dr, lane);
-    attend<D, F8, 1>(
+    load_q<D, F8, Pad>(q[0],
+                       a.q + (static_cast<int64_t>(b) * a.hq + head0 + min(row, heads - 1)) * dr,
+                       row < heads, dr, lane);
+    attend(
         st, q, a.cache, h, first, chunks, stride, a.scale_log2, lane,
         [&](int c) {
             const int k = __builtin_amdgcn_readfirstlane(2 * ((c - first) / stride));
@@ -157,9 +157,9 @@ int64_t part_rows(int batch, int hq, int hkv, int take) {
     return static_cast<int64_t>(batch) * hkv * tiles * splits_of(batch, hq, hkv, take) * kTile;
 }
 
-template <int D, bool F8>
+template <int D, bool F8, bool Pad>
 hipError_t launch(const SparseDecode& s, void* workspace, hipStream_t stream) {
-    SparseArgs<F8> a;
+    SparseArgs<D, F8, Pad> a;
     a.q = static_cast<const __bf16*>(s.q);
     using Elem = std::conditional_t<F8, uint8_t, __bf16>;
     a.cache = {static_cast<const Elem*>(s.k), static_cast<const Elem*>(s.v), s.k_scale, s.v_scale,
@@ -183,7 +183,7 @@ hipError_t launch(const SparseDecode& s, void* workspace, hipStream_t stream) {
     }
     const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.hkv * a.tiles *
                                                 a.splits);
-    hipLaunchKernelGGL((sparse_decode_kernel<D, F8>), dim3(grid), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((sparse_decode_kernel<D, F8, Pad>), dim3(grid), dim3(kThreads), 0, stream, a);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess || a.splits == 1) return err;
     const int64_t rows = static_cast<int64_t>(s.batch) * s.hq;
     hipLaunchKernelGGL((sparse_merge_kernel<D>),
@@ -203,15 +203,19 @@ size_t sparse_decode_workspace_bytes(int batch, int hq, int hkv, int head_dim, i
 
 hipError_t sparse_decode(const SparseDecode& s, void* workspace, hipStream_t stream) {
     const bool fp8 = s.k_scale != nullptr;
-    switch (mfma_dim(s.head_dim)) {
+    const int d = s.head_dim;
+    switch (mfma_dim(d)) {
         case 64:
-            return fp8 ? launch<64, true>(s, workspace, stream)
-                       : launch<64, false>(s, workspace, stream);
+            return fp8 ? launch<64, true, false>(s, workspace, stream)
+                   : d == 64 ? launch<64, false, false>(s, workspace, stream)
+                             : launch<64, false, true>(s, workspace, stream);
         case 128:
-            return fp8 ? launch<128, true>(s, workspace, stream)
-                       : launch<128, false>(s, workspace, stream);
+            return fp8 ? launch<128, true, false>(s, workspace, stream)
+                   : d == 128 ? launch<128, false, false>(s, workspace, stream)
+                              : launch<128, false, true>(s, workspace, stream);
         default:
-            return launch<256, false>(s, workspace, stream);
+            return d == 256 ? launch<256, false, false>(s, workspace, stream)
+                            : launch<256, false, true>(s, workspace, stream);
     }
 }
 

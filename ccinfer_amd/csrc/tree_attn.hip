@@ -47,10 +47,10 @@ struct SlotDesc {
     int last_slot;
 };
 
-template <bool F8>
+template <int D, bool F8, bool Pad>
 struct TreeArgs {
     const __bf16* q;
-    Cache<F8> cache;
+    Cache<D, F8, Pad> cache;
     const int32_t* table;
     const int32_t* qsl;
     const int32_t* ctx;
@@ -110,8 +110,8 @@ __device__ __forceinline__ int request_units(const Request& r, int G) {
     return chunks * (4 * full + chunk_units<R>(rows - full * 4 * R));
 }
 
-template <int D, bool F8>
-__global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<F8> a) {
+template <int D, bool F8, bool Pad>
+__global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D, F8, Pad> a) {
     constexpr int NT = kTiles<D>;
     constexpr int R = 16 * NT;
     __shared__ Parts<D, NT> parts;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<F8
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hkv = a.cache.hkv;
-    const int G = a.hq / hkv;
+    const int G = a.hq / hkv, dr = a.cache.dims();
     const int h = blockIdx.x % hkv, slot = blockIdx.x / hkv;
     SlotDesc* desc = a.desc + static_cast<int64_t>(h) * a.slots + slot;
 
@@ -213,36 +213,35 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<F8
                 const int r = row0 + (live ? row : 0);
                 const int node = r / G;
                 const int64_t token = req.first + node;
-                load_q<D, F8>(q[t],
-                              a.q + (token * a.hq + h * G + (r - node * G)) * a.cache.dr, live,
-                              a.cache.dr, lane);
+                load_q<D, F8, Pad>(q[t], a.q + (token * a.hq + h * G + (r - node * G)) * dr, live,
+                                   dr, lane);
                 mask_row[t] = a.mask + token * a.words;
             }
             const auto table = unwritten(a.table) + static_cast<int64_t>(b) * a.mbpr;
-            attend<D, F8, NT>(
-                st, q, a.cache, h, c0 + part, c1, share, a.scale_log2, lane,
-                [&](int c) {
-                    const int cb = c * kChunk;
-                    const int blk = 2 * c;
-                    const int pb0 = table[blk];
-                    const int pb1 = cb + kBlock < req.end ? table[blk + 1] : -1;
-                    return make_pair(pb0, req.end - cb, pb1, req.end - cb - kBlock);
-                },
-                [&](int c, int t, uint32_t& bits) {
-                    const int o = c * kChunk - req.before;  // tree node of the chunk's first token
-                    if (o <= -kChunk) return false;
-                    const uint32_t* m = mask_row[t];
-                    if (o < 0) {
-                        bits = (m[0] << -o) | ((1u << -o) - 1u);
-                    } else {
-                        const int w = o >> 5;
-                        const uint32_t lo = w < a.words ? m[w] : 0u;
-                        const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
-                        bits = static_cast<uint32_t>(
-                            ((static_cast<uint64_t>(hi) << 32) | lo) >> (o & 31));
-                    }
-                    return true;
-                });
+            auto chunk = [&](int c) {
+                const int cb = c * kChunk;
+                const int pb0 = table[2 * c];
+                const int pb1 = cb + kBlock < req.end ? table[2 * c + 1] : -1;
+                return make_pair(pb0, req.end - cb, pb1, req.end - cb - kBlock);
+            };
+            auto seen = [&](int c, int t, uint32_t& bits) {
+                const int o = c * kChunk - req.before;  // tree node of the chunk's first token
+                if (o <= -kChunk) return false;
+                const uint32_t* m = mask_row[t];
+                if (o < 0) {
+                    bits = (m[0] << -o) | ((1u << -o) - 1u);
+                } else {
+                    const int w = o >> 5;
+                    const uint32_t lo = w < a.words ? m[w] : 0u;
+                    const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
+                    bits = static_cast<uint32_t>(((static_cast<uint64_t>(hi) << 32) | lo) >>
+                                                 (o & 31));
+                }
+                return true;
+            };
+            if (attend(st, q, a.cache, h, c0 + part, c1, share, a.scale_log2, lane,
+                                  chunk, seen))
+                add_unbounded(st, a.cache, h, c0 + part, c1, share, lane, chunk, seen);
         }
 
         const int64_t piece = (static_cast<int64_t>(h) * a.slots + slot) * 2 + which;
@@ -257,8 +256,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<F8
                 const int r = row0 + row;
                 const int node = r / G;
                 const int64_t token = req.first + node;
-                store_bf16_row<D>(a.out + (token * a.hq + h * G + (r - node * G)) * a.cache.dr, x,
-                                  inverse_sum(l), a.cache.dr, lane);
+                store_bf16_row<D>(a.out + (token * a.hq + h * G + (r - node * G)) * dr, x,
+                                  inverse_sum(l), dr, lane);
             } else {
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y)
@@ -341,11 +340,11 @@ TreeWorkspace workspace_of(int total, int hq, int hkv, int D) {
     return w;
 }
 
-template <int D, bool F8>
+template <int D, bool F8, bool Pad>
 hipError_t launch(const TreeAttention& t, void* workspace, hipStream_t stream) {
     const TreeWorkspace w = workspace_of(t.total, t.hq, t.hkv, D);
     char* ws = static_cast<char*>(workspace);
-    TreeArgs<F8> a;
+    TreeArgs<D, F8, Pad> a;
     a.q = static_cast<const __bf16*>(t.q);
     using Elem = std::conditional_t<F8, uint8_t, __bf16>;
     a.cache = {static_cast<const Elem*>(t.k), static_cast<const Elem*>(t.v), t.k_scale, t.v_scale,
@@ -368,7 +367,7 @@ hipError_t launch(const TreeAttention& t, void* workspace, hipStream_t stream) {
     a.part_ml = reinterpret_cast<float2*>(ws + w.ml);
     a.part_acc = reinterpret_cast<float*>(ws + w.acc);
     const unsigned grid = static_cast<unsigned>(a.slots) * t.hkv;
-    hipLaunchKernelGGL((tree_attention_kernel<D, F8>), dim3(grid), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((tree_attention_kernel<D, F8, Pad>), dim3(grid), dim3(kThreads), 0, stream, a);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     hipLaunchKernelGGL((tree_merge_kernel<D>), dim3(grid, kMergeSplit), dim3(kThreads), 0, stream,
                        a.desc, a.part_acc, a.part_ml, a.out, a.slots, a.row_cap, t.hq, t.hkv,
@@ -399,15 +398,19 @@ size_t tree_attention_workspace_bytes(int total, int hq, int hkv, int head_dim) 
 
 hipError_t tree_attention(const TreeAttention& t, void* workspace, hipStream_t stream) {
     const bool fp8 = t.k_scale != nullptr;
-    switch (mfma_dim(t.head_dim)) {
+    const int d = t.head_dim;
+    switch (mfma_dim(d)) {
         case 64:
-            return fp8 ? launch<64, true>(t, workspace, stream)
-                       : launch<64, false>(t, workspace, stream);
+            return fp8 ? launch<64, true, false>(t, workspace, stream)
+                   : d == 64 ? launch<64, false, false>(t, workspace, stream)
+                             : launch<64, false, true>(t, workspace, stream);
         case 128:
-            return fp8 ? launch<128, true>(t, workspace, stream)
-                       : launch<128, false>(t, workspace, stream);
+            return fp8 ? launch<128, true, false>(t, workspace, stream)
+                   : d == 128 ? launch<128, false, false>(t, workspace, stream)
+                              : launch<128, false, true>(t, workspace, stream);
         default:
-            return launch<256, false>(t, workspace, stream);
+            return d == 256 ? launch<256, false, false>(t, workspace, stream)
+                            : launch<256, false, true>(t, workspace, stream);
     }
 }
 
