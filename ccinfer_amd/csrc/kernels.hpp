@@ -316,8 +316,9 @@ hipError_t compact_kv_blocks(const int32_t* table, const int32_t* refs, int64_t 
                              hipStream_t stream);
 
 // ---- drafted tokens -------------------------------------------------------------
-// Requests of a call, and nodes (drafted tokens) of a request, at most.
+// Requests of a call (of an attention call), and nodes (drafted tokens) of a request, at most.
 constexpr int kTreeMaxRequests = 2048;
+constexpr int kTreeMaxBatch = 1024;
 constexpr int kTreeMaxNodes = 2048;
 
 struct TreeAttention {

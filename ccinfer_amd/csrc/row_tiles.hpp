@@ -7,12 +7,17 @@
 // (j = lane & 15, g = lane >> 4) holds row j of a tile; its eight scores of a chunk are those of
 // tokens T(g, e) = 16 (e / 4) + 4 g + e % 4, and acc[t][n][r] is O[16 t + j][NV (4 g + r) + n].
 //
-// K and V of a chunk have one set of registers each: K of the next chunk is asked for when the
-// scores are done, V when the second product is, so a chunk and a half is in flight on the
-// average while the register file holds one, and two tiles of rows fit beside it at two
-// wavefronts a SIMD.
+// Two ways of the chunks. One wavefront by itself (attend) loads K and V into registers, one set
+// each: K of the next chunk is asked for when the scores are done, V when the second product is, so
+// a chunk and a half is in flight on the average. Wavefronts with different rows and the same
+// chunks (attend_shared) copy each chunk once into a ring in LDS: the first product wants 16 rows
+// of K in 16 neighbouring lanes, in memory a read of 16 lines at once, of which the address unit
+// takes one a cycle, and every wavefront by itself would ask for them again (48 trees whose
+// wavefronts read each chunk three to four times: 383 us, the address unit busy for all of it;
+// through the ring %TIME%).
 #pragma once
 
+#include <cstddef>
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -21,7 +26,7 @@ namespace ccinfer::hipk::rows {
 
 constexpr int kBlock = 16;
 constexpr int kChunk = 32;
-constexpr int kWaves = 4;  // wavefronts of a workgroup
+constexpr int64_t kMaxTokenBytes = (1 << 24) - 1;  // of one token's heads, K or V
 
 template <int D>
 struct Shape {
@@ -78,17 +83,34 @@ __device__ __forceinline__ Pair make_pair(int pb0, int lim0, int pb1, int lim1) 
     return p;
 }
 
+// A chunk's K and V in registers. K: lane (i, g) has of token i of each block the dims q_dim(kk, g)
+// .. + 8 of every step (fp8: 16 bytes hold two steps'). V: dims NV i .. of tokens T(g, e). The
+// scales of an fp8 chunk: of tokens 4 g .. of each block.
 template <int D, bool F8>
 struct KRegs {
-    // fp8: 16 bytes of a row hold two steps' dims 64 s + 16 g .. + 16 (q_dim says the same)
     u32x4 k[2][F8 ? Shape<D>::kSteps / 2 : Shape<D>::kSteps];
     u32x4 s[F8 ? 2 : 1];
 };
-
 template <int D, bool F8>
 struct VRegs {
     uint32_t v[8][F8 ? (Shape<D>::kNV + 3) / 4 : Shape<D>::kVWords];
     u32x4 s[F8 ? 2 : 1];
+};
+
+// A chunk's K and V in LDS: 32 rows of kPieces 16-byte pieces each. Piece x of row r of K lies at
+// place x ^ swizzle(r) of its row: the 16 rows that lanes read at once then lie in different
+// banks. V is read row by row, and lies as it is.
+template <int D, bool F8>
+struct Tile {
+    static constexpr int kPieces = D * (F8 ? 1 : 2) / 16;
+    static constexpr int kBytes = kChunk * kPieces * 16;
+    static constexpr int kLoads = kBytes / (64 * 16);  // of K, and of V: a wavefront moves 1 KB
+    static __device__ __forceinline__ int swizzle(int row) {
+        constexpr int kRowsPerLine = kPieces >= 16 ? 1 : 16 / kPieces;  // a line of 256 bytes
+        return (row / kRowsPerLine) & ((kPieces < 16 ? kPieces : 16) - 1);
+    }
+    char kv[2][kBytes];
+    float scales[F8 ? 2 : 1][F8 ? kChunk : 4];  // of K, of V
 };
 
 // First of the eight dims that lane group g holds in step kk.
@@ -97,28 +119,30 @@ __device__ __forceinline__ int q_dim(int kk, int g) {
     return F8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : (kk * 4 + g) * 8;
 }
 
-// A block's first row of head h, wave-uniform: loads take it from scalar registers and a 32-bit
-// offset a lane (a block has at most 2^30 bytes).
+// A block's first row of head h, wave-uniform: loads take it from scalar registers and an offset
+// in bytes a lane (rows are less than 2^24 bytes apart: kMaxTokenBytes).
 template <class Elem, class C>
-__device__ __forceinline__ const Elem* block_rows(const Elem* base, const C& c, int pb, int h) {
-    return base + (static_cast<int64_t>(pb) * kBlock * c.hkv + h) * c.dims();
+__device__ __forceinline__ const char* block_rows(const Elem* base, const C& c, int pb, int h) {
+    return reinterpret_cast<const char*>(
+        base + (static_cast<int64_t>(pb) * kBlock * c.hkv + h) * c.dims());
 }
 
 template <class C>
 __device__ __forceinline__ u32x4 load_scales(const float* base, const C& c, int pb, int h, int g) {
-    return load16(base + (static_cast<int64_t>(pb) * c.hkv + h) * kBlock +
-                  static_cast<uint32_t>(4 * g));
+    return load16(reinterpret_cast<const char*>(
+                      base + (static_cast<int64_t>(pb) * c.hkv + h) * kBlock) +
+                  static_cast<uint32_t>(16 * g));
 }
 
 template <int D, bool F8, bool Pad>
 __device__ __forceinline__ void load_k(KRegs<D, F8>& r, const Cache<D, F8, Pad>& c, const Pair& p,
                                        int h, int lane) {
     const int i = lane & 15, g = lane >> 4;
-    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims();
+    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims() * (F8 ? 1 : 2);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const auto* blk = block_rows(c.k, c, p.pb[b], h);
-        const uint32_t row = static_cast<uint32_t>(min(i, p.lim[b] - 1)) * stride;
+        const char* blk = block_rows(c.k, c, p.pb[b], h);
+        const uint32_t row = __umul24(min(i, p.lim[b] - 1), stride);
         if constexpr (F8) {
 #pragma unroll
             for (int s = 0; s < Shape<D>::kSteps / 2; ++s)
@@ -129,7 +153,7 @@ __device__ __forceinline__ void load_k(KRegs<D, F8>& r, const Cache<D, F8, Pad>&
             for (int kk = 0; kk < Shape<D>::kSteps; ++kk) {
                 const int dim = q_dim<false>(kk, g);
                 const bool ok = !Pad || dim < c.dr;
-                r.k[b][kk] = load16(blk + (row + (ok ? dim : 0)));
+                r.k[b][kk] = load16(blk + (row + (ok ? 2 * dim : 0)));
                 // a dim past the row meets q's zero, but 0 x inf is none
                 if (!ok) r.k[b][kk] = u32x4{0u, 0u, 0u, 0u};
             }
@@ -142,12 +166,12 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<D, F8, Pad>&
                                        int h, int lane) {
     constexpr int NV = Shape<D>::kNV;
     const int i = lane & 15, g = lane >> 4;
-    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims();
+    const uint32_t stride = static_cast<uint32_t>(c.hkv) * c.dims() * (F8 ? 1 : 2);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int b = e >> 2;
-        const auto* blk = block_rows(c.v, c, p.pb[b], h);
-        const uint32_t row = static_cast<uint32_t>(min(4 * g + (e & 3), p.lim[b] - 1)) * stride;
+        const char* blk = block_rows(c.v, c, p.pb[b], h);
+        const uint32_t row = __umul24(min(4 * g + (e & 3), p.lim[b] - 1), stride);
         if constexpr (F8) {
             if constexpr (NV == 8) {
                 const u32x2 w = *reinterpret_cast<const u32x2*>(blk + (row + i * NV));
@@ -157,8 +181,8 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<D, F8, Pad>&
                 r.v[e][0] = *reinterpret_cast<const uint32_t*>(blk + (row + i * NV));
             }
         } else if constexpr (NV == 4) {
-            const u32x2 w =
-                *reinterpret_cast<const u32x2*>(blk + (row + (!Pad || i * NV < c.dr ? i * NV : 0)));
+            const u32x2 w = *reinterpret_cast<const u32x2*>(
+                blk + (row + (!Pad || i * NV < c.dr ? 2 * i * NV : 0)));
             r.v[e][0] = w[0];
             r.v[e][1] = w[1];
         } else {
@@ -166,7 +190,7 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<D, F8, Pad>&
 #pragma unroll
             for (int x = 0; x < NV / 8; ++x) {
                 const int dim = i * NV + 8 * x;
-                const u32x4 w = load16(blk + (row + (!Pad || dim < c.dr ? dim : 0)));
+                const u32x4 w = load16(blk + (row + (!Pad || dim < c.dr ? 2 * dim : 0)));
 #pragma unroll
                 for (int y = 0; y < 4; ++y) r.v[e][4 * x + y] = w[y];
             }
@@ -178,10 +202,173 @@ __device__ __forceinline__ void load_v(VRegs<D, F8>& r, const Cache<D, F8, Pad>&
     }
 }
 
+__device__ const uint32_t kZeros[4] = {0u, 0u, 0u, 0u};
+
+// Where copies go: `ring` by the name of another variable. Taken as writes to the ring, each would
+// make the compiler wait for all of them before the next read of any tile; the loop's own waits
+// and meetings order them.
+struct LdsCopy {
+    using Byte = __attribute__((address_space(3))) char;
+    Byte* name;
+    uint32_t ring;  // bytes from there
+    __device__ __forceinline__ LdsCopy(void* other, const void* ring_)
+        : name((Byte*)other),
+          ring(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Byte*)const_cast<void*>(ring_))) -
+               static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Byte*)other))) {}
+    __device__ __forceinline__ __attribute__((address_space(3))) void* at(uint32_t off) const {
+        uint32_t o = ring + off;
+        asm("" : "+s"(o));
+        return (__attribute__((address_space(3))) void*)(name + o);
+    }
+};
+
+// Copies chunks into tiles. Instruction z of K, or of V, moves the 64 pieces from row z kRows on;
+// of all of them wavefront r of Of asks for its part (the same number for each: where there are
+// fewer than wavefronts, some ask for the same again). The part of one of several lies in K or in
+// V, that of one of four or more in one of the blocks.
+template <int Of, int D, bool F8, bool Pad>
+struct Copier {
+    using T = Tile<D, F8>;
+    static constexpr int kRows = 64 / T::kPieces;
+    static constexpr int kEach = 2 * T::kLoads >= Of ? 2 * T::kLoads / Of : 1;
+    static constexpr int kAsked = kEach + (F8 ? 1 : 0);
+    static_assert(Of <= 2 || Of % 4 == 0);
+    static_assert(2 * T::kLoads % Of == 0 || Of % (2 * T::kLoads) == 0);
+    const Cache<D, F8, Pad>& cache;
+    int h, lane, x0;
+    uint32_t stride;  // bytes of a token's heads
+    LdsCopy to;
+    __device__ __forceinline__ Copier(const Cache<D, F8, Pad>& c, int h_, int r, int lane_,
+                                      const LdsCopy& to_)
+        : cache(c), h(h_), lane(lane_), to(to_) {
+        x0 = Of == 1 ? 0 : r % (2 * T::kLoads / kEach) * kEach;
+        stride = static_cast<uint32_t>(c.hkv) * c.dims() * (F8 ? 1 : 2);
+    }
+    // Instruction z of K (of_v false) or V, of a tile at byte `tile` of the ring.
+    __device__ __forceinline__ void one(uint32_t tile, const Pair& p, bool of_v, int z) const {
+        const bool second = z >= T::kLoads / 2;
+        const int pb = second ? p.pb[1] : p.pb[0], lim = second ? p.lim[1] : p.lim[0];
+        const int row0 = z * kRows & (kBlock - 1);  // wave-uniform
+        const int row = lane / T::kPieces;
+        // swizzle(row0 + row): the bits of the two do not meet
+        int piece = lane % T::kPieces;
+        if (!of_v) piece ^= T::swizzle(row) ^ T::swizzle(row0);
+        const char* blk = reinterpret_cast<const char*>(
+            of_v ? block_rows(cache.v, cache, pb, h) : block_rows(cache.k, cache, pb, h));
+        const bool past = Pad && 8 * piece >= cache.dr;
+        // rows past the last are copies of it
+        const char* src = blk + (__umul24(min(row0 + row, lim - 1), stride) +
+                                 static_cast<uint32_t>(past ? 0 : 16 * piece));
+        // a dim of K past the row meets q's zero, but 0 x inf is none; one of V goes to columns
+        // that are not stored
+        if (past && !of_v) src = reinterpret_cast<const char*>(kZeros);
+        __builtin_amdgcn_global_load_lds(
+            src, to.at(tile + ((of_v ? T::kLoads : 0) + z) * 64 * 16), 16, 0, 0);
+    }
+    // The scales of K, of V, or of both.
+    __device__ __forceinline__ void scales(uint32_t tile, const Pair& p, bool of_k,
+                                           bool of_v) const {
+        const float* scale = lane < kChunk ? cache.ks : cache.vs;
+        const int pb = (lane & kBlock) != 0 ? p.pb[1] : p.pb[0];
+        const float* src = scale + (static_cast<int64_t>(pb) * cache.hkv + h) * kBlock +
+                           (lane & (kBlock - 1));
+        if (lane < kChunk ? of_k : of_v)
+            __builtin_amdgcn_global_load_lds(src, to.at(tile + offsetof(T, scales)), 4, 0, 0);
+    }
+    // This wavefront's part of a chunk, into tile `slot` of the ring.
+    __device__ __forceinline__ void ask(int slot, const Pair& p) const {
+        const uint32_t tile = static_cast<uint32_t>(slot) * sizeof(T);
+#pragma unroll
+        for (int y = 0; y < kEach; ++y)
+            one(tile, p, x0 >= T::kLoads, x0 % T::kLoads + y);
+        if constexpr (F8) scales(tile, p, true, true);
+    }
+    // All of a chunk's K, or V (Of = 1, one tile).
+    __device__ __forceinline__ void ask_half(const Pair& p, bool of_v) const {
+#pragma unroll
+        for (int z = 0; z < T::kLoads; ++z) one(0, p, of_v, z);
+        if constexpr (F8) scales(0, p, !of_v, of_v);
+    }
+};
+
+template <int D, bool F8>
+__device__ __forceinline__ void read_k(KRegs<D, F8>& r, const Tile<D, F8>& tile, int lane) {
+    using T = Tile<D, F8>;
+    constexpr int kEach = sizeof(r.k[0]) / 16;
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int row = 16 * b + i;
+            r.k[b][x] = *reinterpret_cast<const u32x4*>(
+                tile.kv[0] + (row * T::kPieces + ((4 * x + g) ^ T::swizzle(row))) * 16);
+        }
+        if constexpr (F8) r.s[b] = *reinterpret_cast<const u32x4*>(&tile.scales[0][16 * b + 4 * g]);
+    }
+}
+
+template <int D, bool F8>
+__device__ __forceinline__ void read_v(VRegs<D, F8>& r, const Tile<D, F8>& tile, int lane) {
+    constexpr int kWords = sizeof(r.v[0]) / 4;
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const char* from = tile.kv[1] +
+                           (16 * (e >> 2) + 4 * g + (e & 3)) * Tile<D, F8>::kPieces * 16 +
+                           i * kWords * 4;
+        if constexpr (kWords == 1) {
+            r.v[e][0] = *reinterpret_cast<const uint32_t*>(from);
+        } else if constexpr (kWords == 2) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(from);
+            r.v[e][0] = w[0];
+            r.v[e][1] = w[1];
+        } else {
+#pragma unroll
+            for (int x = 0; x < kWords; x += 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(from + 4 * x);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) r.v[e][x + y] = w[y];
+            }
+        }
+    }
+    if constexpr (F8) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            r.s[b] = *reinterpret_cast<const u32x4*>(&tile.scales[F8 ? 1 : 0][16 * b + 4 * g]);
+    }
+}
+
+// Until all but the newest n loads of this wavefront have landed, and all its LDS reads.
+template <int n>
+__device__ __forceinline__ void wait_loads_but() {
+    static_assert(n < 64);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | ((n >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Until this wavefront's LDS reads have arrived: what they read may be written again.
+__device__ __forceinline__ void wait_reads() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The workgroup's wavefronts meet; what they copied into LDS before may be read after.
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
 template <int D, int NT>
 struct State {
     f32x4 acc[NT][Shape<D>::kNV];
-    float m[NT];  // running maximum, base 2, the same in a row's four lanes
+    float m[NT];  // what the exponents are taken from, base 2, the same in a row's four lanes
     float l[NT];  // this lane's part of the sum
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -230,140 +417,299 @@ __device__ __forceinline__ bool clear_unbounded(VRegs<D, F8>& r) {
     return found;
 }
 
-// Chunks first, first + stride, ... below last of the rows. chunk(c): the Pair of chunk c (asked
-// for two chunks ahead: the ids' way to the scalar registers is hidden behind a chunk's work).
-// seen(c, t, bits): false where every row of tile t sees all that is there of the chunk, else
-// bits has a bit for each of its 32 tokens that this lane's row sees. In such chunks the matrix
-// product leaves out infinities and NaN of V, which would reach rows that do not see their token
-// (0 x inf); true if there were any: add_unbounded then brings them to the rows that do.
-template <int D, bool F8, bool Pad, int NT, class Chunks, class Seen>
-__device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
-                                       const Cache<D, F8, Pad>& cache, int h, int first, int last,
-                                       int stride, float scale_log2, int lane, Chunks chunk,
-                                       Seen seen) {
-    constexpr int S = Shape<D>::kSteps;
-    constexpr int NV = Shape<D>::kNV;
-    if (first >= last) return false;
-    bool left_out = false;
-    const int g = lane >> 4;
-    KRegs<D, F8> k;
-    VRegs<D, F8> v;
-    Pair cur = chunk(first);
-    Pair next = chunk(min(first + stride, last - 1));
-    load_k(k, cache, cur, h, lane);
-    load_v(v, cache, cur, h, lane);
-    for (int c = first;; c += stride) {
-        const bool more = c + stride < last;
-        const Pair after = chunk(min(c + 2 * stride, last - 1));
-        float sc[NT][8];
+// Products of q with K: sc[t][e] of row j and token T(g, e), times the token's scale in an fp8
+// cache; the logits' factor follows in the exponent.
+template <int D, bool F8, int NT>
+__device__ __forceinline__ void first_product(float (&sc)[NT][8],
+                                              const bf16x8 (&q)[NT][Shape<D>::kSteps],
+                                              const KRegs<D, F8>& k) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            f32x4 s4[NT];
+    for (int b = 0; b < 2; ++b) {
+        f32x4 s4[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) s4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kk = 0; kk < S; ++kk) {
-                u32x4 w;
-                if constexpr (F8) {
+        for (int kk = 0; kk < Shape<D>::kSteps; ++kk) {
+            u32x4 w;
+            if constexpr (F8) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t bytes = k.k[b][kk >> 1][2 * (kk & 1) + x];
-                        w[2 * x] = e4m3x2_to_bf16x2<false>(bytes);
-                        w[2 * x + 1] = e4m3x2_to_bf16x2<true>(bytes);
-                    }
-                } else {
-                    w = k.k[b][kk];
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t bytes = k.k[b][kk >> 1][2 * (kk & 1) + x];
+                    w[2 * x] = e4m3x2_to_bf16x2<false>(bytes);
+                    w[2 * x + 1] = e4m3x2_to_bf16x2<true>(bytes);
                 }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    s4[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, w), q[t][kk], s4[t]);
+            } else {
+                w = k.k[b][kk];
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float f =
-                        F8 ? scale_log2 * __uint_as_float(k.s[F8 ? b : 0][r]) : scale_log2;
-                    sc[t][4 * b + r] = s4[t][r] * f;
-                }
+                s4[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, w), q[t][kk], s4[t]);
         }
-        if (more) load_k(k, cache, next, h, lane);
-        if (cur.any()) {
-            bool hidden = false;  // wave-uniform: some score is masked
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                uint32_t bits = 0xffffffffu;
-                const bool some = seen(c, t, bits);
-                if (some || !cur.whole()) {
-                    hidden |= some;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int b = e >> 2, key = 4 * g + (e & 3);
-                        const bool ok = cur.on[b] && key < cur.lim[b] &&
-                                        ((bits >> (16 * b + key)) & 1u) != 0;
-                        sc[t][e] = ok ? sc[t][e] : kNegInf;
-                    }
-                }
+            for (int r = 0; r < 4; ++r)
+                sc[t][4 * b + r] =
+                    F8 ? s4[t][r] * __uint_as_float(k.s[F8 ? b : 0][r]) : s4[t][r];
+    }
+}
+
+// Masks the scores of a chunk that some row does not see whole. seen(c, t, bits): false where
+// every row of tile t sees all that is there of the chunk, else bits has a bit for each of its 32
+// tokens that this lane's row sees. Returns whether `seen` hid any (wave-uniform).
+template <int NT, class Seen>
+__device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, int c, int lane,
+                                            Seen seen) {
+    uint32_t bits[NT];
+    bool hidden = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        bits[t] = 0xffffffffu;
+        hidden |= seen(c, t, bits[t]);
+    }
+    if (hidden || !p.whole()) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int b = e >> 2, key = 4 * (lane >> 4) + (e & 3);
+                const bool ok =
+                    p.on[b] && key < p.lim[b] && ((bits[t] >> (16 * b + key)) & 1u) != 0;
+                sc[t][e] = ok ? sc[t][e] : kNegInf;
             }
-            float p[NT][8];
-            bf16x8 pop[NT];
-            float alpha[NT];
-            bool grew = false;
+    }
+    return hidden;
+}
+
+// The reference that the exponents are taken from follows the maximum only when a score passes it
+// by 2^8: probabilities up to 256 are as good in floating point, and without a new one nothing is
+// compared across lanes and no sum is scaled.
+template <int D, int NT>
+__device__ __forceinline__ void follow_maximum(State<D, NT>& st, const float (&sc)[NT][8],
+                                               float scale_log2) {
+    float top[NT];
+    bool passed = false;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float top = fmaxf(fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])),
-                                  fmaxf(fmaxf(sc[t][4], sc[t][5]), fmaxf(sc[t][6], sc[t][7])));
-                top = fmaxf(st.m[t], wave_max_xor16_32(top));
-                const float use = top == kNegInf ? 0.f : top;  // nothing seen yet: exp2(-inf)
-                alpha[t] = __builtin_amdgcn_exp2f(st.m[t] - use);
-                grew |= top != st.m[t];
-                st.m[t] = top;
-                float sum = 0.f;
+    for (int t = 0; t < NT; ++t) {
+        top[t] = fmaxf(fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])),
+                       fmaxf(fmaxf(sc[t][4], sc[t][5]), fmaxf(sc[t][6], sc[t][7]))) *
+                 scale_log2;
+        passed |= top[t] > st.m[t] + 8.f;
+    }
+    if (__builtin_amdgcn_ballot_w64(passed) != 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[t][e] = __builtin_amdgcn_exp2f(sc[t][e] - use);
-                    sum += p[t][e];
-                }
-                st.l[t] = st.l[t] * alpha[t] + sum;
-                if constexpr (F8) {
+        for (int t = 0; t < NT; ++t) {
+            const float m = fmaxf(st.m[t], wave_max_xor16_32(top[t]));
+            // (nothing seen yet: sums of zeros)
+            const float f = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(st.m[t] - m);
+            st.m[t] = m;
+            st.l[t] *= f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        // a masked token's scale may be anything; a NaN stays one
-                        p[t][e] = __float_as_uint(p[t][e]) != 0u
-                                      ? p[t][e] * __uint_as_float(v.s[F8 ? e >> 2 : 0][e & 3])
-                                      : 0.f;
-                }
-                u32x4 pw;
-                // probabilities in bf16 (2^-8 of each, and the matrix unit takes no wider ones); the
-                // sum is of the unrounded ones
-#pragma unroll
-                for (int x = 0; x < 4; ++x) pw[x] = pack_bf16x2(p[t][2 * x], p[t][2 * x + 1]);
-                pop[t] = __builtin_bit_cast(bf16x8, pw);
-            }
-            if (__builtin_amdgcn_ballot_w64(grew) != 0) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int n = 0; n < NV; ++n) st.acc[t][n] = st.acc[t][n] * alpha[t];
-            }
-            if (hidden) left_out |= clear_unbounded<D, F8>(v);
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                u32x4 vw;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1),
-                                        v_word<D, F8>(v, 2 * x + 1, n >> 1), n & 1);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    st.acc[t][n] =
-                        mfma16x16x32(__builtin_bit_cast(bf16x8, vw), pop[t], st.acc[t][n]);
-            }
+            for (int n = 0; n < Shape<D>::kNV; ++n) st.acc[t][n] = st.acc[t][n] * f;
         }
-        if (!more) break;
-        load_v(v, cache, next, h, lane);
-        cur = next;
-        next = after;
+    }
+}
+
+// Probabilities and the second product. `clear`: V's infinities and NaN are left out (see
+// add_unbounded); returns whether there were any.
+template <int D, bool F8, int NT>
+__device__ __forceinline__ bool second_product(State<D, NT>& st, const float (&sc)[NT][8],
+                                               VRegs<D, F8>& v, float scale_log2, bool clear) {
+    const bool found = clear && clear_unbounded<D, F8>(v);
+    bf16x8 pop[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float from = st.m[t] == kNegInf ? 0.f : st.m[t];
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], scale_log2, -from));
+            st.l[t] += p[e];
+        }
+        if constexpr (F8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                // a masked token's scale may be anything; a NaN stays one
+                p[e] = __float_as_uint(p[e]) != 0u
+                           ? p[e] * __uint_as_float(v.s[F8 ? e >> 2 : 0][e & 3])
+                           : 0.f;
+        }
+        u32x4 pw;
+        // probabilities in bf16 (2^-8 of each, and the matrix unit takes no wider ones); the sum
+        // is of the unrounded ones
+#pragma unroll
+        for (int x = 0; x < 4; ++x) pw[x] = pack_bf16x2(p[2 * x], p[2 * x + 1]);
+        pop[t] = __builtin_bit_cast(bf16x8, pw);
+    }
+#pragma unroll
+    for (int n = 0; n < Shape<D>::kNV; ++n) {
+        u32x4 vw;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1), v_word<D, F8>(v, 2 * x + 1, n >> 1),
+                                n & 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            st.acc[t][n] = mfma16x16x32(__builtin_bit_cast(bf16x8, vw), pop[t], st.acc[t][n]);
+    }
+    return found;
+}
+
+// Chunks first, first + stride, ... below last of the rows of one wavefront. next(): their Pairs,
+// one after the other (the last one again behind it), from ids that lie in the wavefront's lanes:
+// a scalar load a chunk would make every wait for LDS wait for it too. Chunks that `seen` hides a
+// part of (mask_scores) are multiplied without the infinities and NaN of V, which would reach rows
+// that do not see their token (0 x inf); true if there were any: add_unbounded then brings them
+// to the rows that do.
+template <int D, bool F8, bool Pad, int NT, class Next, class Seen>
+__device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
+                                       const Cache<D, F8, Pad>& cache, int h, int first, int last,
+                                       int stride, float scale_log2, int lane, Next& next,
+                                       Seen seen) {
+    if (first >= last) return false;
+    bool left_out = false;
+    KRegs<D, F8> k;
+    VRegs<D, F8> v;
+    Pair cur = next();
+    load_k(k, cache, cur, h, lane);
+    // K before V here as in the loop: the waits count loads in their order
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(v, cache, cur, h, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    int c = first;
+    // One chunk; with More, K and V of the next one are asked for on the way.
+    auto step = [&](auto more) {
+        constexpr bool More = decltype(more)::value;
+        Pair after = cur;
+        if constexpr (More) after = next();
+        float sc[NT][8];
+        first_product<D, F8, NT>(sc, q, k);
+        if constexpr (More) load_k(k, cache, after, h, lane);
+        const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
+        follow_maximum<D, NT>(st, sc, scale_log2);
+        // (a chunk that is off was read from the pool's first block, whatever that holds)
+        const bool found =
+            second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !cur.any());
+        left_out |= found && hidden;
+        if constexpr (More) {
+            load_v(v, cache, after, h, lane);
+            cur = after;
+            c += stride;
+        }
+    };
+    while (c + stride < last) step(std::true_type{});
+    step(std::false_type{});
+    return left_out;
+}
+
+// The same through a tile in LDS of the wavefront's own, with few registers: K and V of the next
+// chunk are asked for as soon as this one's have been read from their place.
+template <int D, bool F8, bool Pad, int NT, class Next, class Seen>
+__device__ __forceinline__ bool attend_alone(State<D, NT>& st,
+                                             const bf16x8 (&q)[NT][Shape<D>::kSteps],
+                                             const Cache<D, F8, Pad>& cache,
+                                             const Tile<D, F8>& tile, const LdsCopy& copies,
+                                             int h, int first, int last, int stride,
+                                             float scale_log2, int lane, Next& next, Seen seen) {
+    if (first >= last) return false;
+    constexpr int kHalf = Tile<D, F8>::kLoads + (F8 ? 1 : 0);
+    const Copier<1, D, F8, Pad> copier(cache, h, 0, lane, copies);
+    bool left_out = false;
+    Pair cur = next();
+    copier.ask_half(cur, false);
+    copier.ask_half(cur, true);
+    for (int c = first; c < last; c += stride) {
+        const bool more = c + stride < last;
+        Pair after = cur;
+        if (more) after = next();
+        wait_loads_but<kHalf>();  // K is there
+        float sc[NT][8];
+        {
+            KRegs<D, F8> k;
+            read_k<D, F8>(k, tile, lane);
+            if (more) {
+                wait_reads();
+                copier.ask_half(after, false);
+            }
+            first_product<D, F8, NT>(sc, q, k);
+        }
+        const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
+        follow_maximum<D, NT>(st, sc, scale_log2);
+        if (more)
+            wait_loads_but<kHalf>();  // V is there
+        else
+            wait_loads_but<0>();
+        VRegs<D, F8> v;
+        read_v<D, F8>(v, tile, lane);
+        if (more) {
+            wait_reads();
+            copier.ask_half(after, true);
+        }
+        const bool found = second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !cur.any());
+        left_out |= found && hidden;
+        cur = after;
+    }
+    return left_out;
+}
+
+// The same for Of wavefronts of a workgroup that take the chunks first, first + stride, ... below
+// last together, each with rows of its own; all wavefronts of the workgroup call it with the same
+// number of steps, those whose chunks end earlier with nothing to do in the last one. ring: the
+// Depth tiles of these wavefronts (copies: the same place for the copies). They meet every Group
+// steps; a tile is asked for Depth - Group steps before it is read, when all have left the steps
+// that read its place, one a step: requests are under way all the time.
+template <int Of, int Depth, int D, bool F8, bool Pad, int NT, class Next, class Seen>
+__device__ __forceinline__ bool attend_shared(State<D, NT>& st,
+                                              const bf16x8 (&q)[NT][Shape<D>::kSteps],
+                                              const Cache<D, F8, Pad>& cache,
+                                              const Tile<D, F8>* ring, const LdsCopy& copies,
+                                              int r, int h, int first, int last, int stride,
+                                              int steps, bool busy, float scale_log2, int lane,
+                                              Next& next, Seen seen) {
+    constexpr int Group = Depth >= 8 ? 2 : 1;
+    constexpr int kAhead = Depth - Group;
+    const Copier<Of, D, F8, Pad> copier(cache, h, r, lane, copies);
+    constexpr int kAsked = Copier<Of, D, F8, Pad>::kAsked;
+    bool left_out = false;
+    uint32_t on = 0;  // two bits a tile that was asked for and is to be read: its blocks are there
+    int asked = 0;    // how many those are
+    auto ask = [&](int s) {
+        const Pair p = next();
+        on |= (static_cast<uint32_t>(p.on[0]) | static_cast<uint32_t>(p.on[1]) << 1) << (2 * asked);
+        ++asked;
+        copier.ask(s % Depth, p);
+    };
+    for (int x = 0; x < min(kAhead, steps); ++x) ask(x);
+    for (int s = 0; s < steps; s += Group) {
+        // this wavefront's part of the next Group tiles; newer ones may be under way
+        if (s + kAhead <= steps)
+            wait_loads_but<(kAhead - Group) * kAsked>();
+        else
+            wait_loads_but<0>();
+        meet();
+#pragma unroll
+        for (int x = 0; x < Group; ++x) {
+            if (s + kAhead + x < steps) ask(s + kAhead + x);
+            const int c = first + (s + x) * stride;
+            const Pair pair = next.read(c, (on & 1u) != 0, (on & 2u) != 0);
+            on >>= 2;
+            --asked;
+            if (!busy || s + x >= steps || c >= last) continue;
+            const Tile<D, F8>& tile = ring[(s + x) % Depth];
+            float sc[NT][8];
+            {
+                KRegs<D, F8> k;
+                read_k<D, F8>(k, tile, lane);
+                first_product<D, F8, NT>(sc, q, k);
+            }
+            VRegs<D, F8> v;
+            read_v<D, F8>(v, tile, lane);
+            const bool hidden = mask_scores<NT>(sc, pair, c, lane, seen);
+            follow_maximum<D, NT>(st, sc, scale_log2);
+            const bool found =
+                second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !pair.any());
+            left_out |= found && hidden;
+        }
     }
     return left_out;
 }
@@ -431,10 +777,95 @@ __device__ __forceinline__ void load_q(bf16x8 (&q)[Shape<D>::kSteps], const __bf
     }
 }
 
-// A row's columns of this lane in the merges: D / 64 next to one another.
+// What a row's sums are multiplied by: 0 where it saw nothing. (By its bits: sources that do not
+// honour NaNs would take a NaN sum for none.)
+__device__ __forceinline__ float inverse_sum(float l) {
+    return __float_as_uint(l) != 0u ? 1.f / l : 0.f;
+}
+
+// Place for half a workgroup's sums, lane by lane.
+template <int D, int NT, int Waves>
+struct Exchange {
+    f32x4 acc[Waves / 2][NT * Shape<D>::kNV][64];
+    float m[Waves / 2][NT][64];
+    float l[Waves / 2][NT][64];
+};
+
+// Adds up the sums of the `parts` (a power of two) wavefronts that took different chunks of the
+// same rows into those of part 0: in each round the upper half hands its own over. A workgroup's
+// wavefronts are `part * groups + group`; all of them call it.
+template <int D, int NT, int Waves>
+__device__ __forceinline__ void add_parts(Exchange<D, NT, Waves>& x, State<D, NT>& st, int part,
+                                          int parts, int group, int groups, int lane) {
+    constexpr int NV = Shape<D>::kNV;
+    for (int half = parts / 2; half >= 1; half /= 2) {
+        if (part >= half && part < 2 * half) {
+            const int at = (part - half) * groups + group;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int n = 0; n < NV; ++n) x.acc[at][t * NV + n][lane] = st.acc[t][n];
+                x.m[at][t][lane] = st.m[t];
+                x.l[at][t][lane] = st.l[t];
+            }
+        }
+        __syncthreads();
+        if (part < half) {
+            const int at = part * groups + group;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float mo = x.m[at][t][lane];
+                const float m = fmaxf(st.m[t], mo);
+                // a part that saw nothing, or only NaN, has -inf, and zeros or NaN
+                const float use = m == kNegInf ? 0.f : m;
+                const float f = __builtin_amdgcn_exp2f(st.m[t] - use);
+                const float fo = __builtin_amdgcn_exp2f(mo - use);
+                st.m[t] = m;
+                st.l[t] = st.l[t] * f + x.l[at][t][lane] * fo;
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+                    st.acc[t][n] = st.acc[t][n] * f + x.acc[at][t * NV + n][lane] * fo;
+            }
+        }
+        if (half > 1) __syncthreads();
+    }
+}
+
+// Row j of tile t, finished, to `row` (bf16, dr elements).
+template <int D, bool Pad, int NT>
+__device__ __forceinline__ void store_row(const State<D, NT>& st, int t, float l, __bf16* row,
+                                          int dr, int lane) {
+    constexpr int NV = Shape<D>::kNV;
+    const float inv = inverse_sum(l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NV; n += 4) {
+            const int dim = NV * (4 * (lane >> 4) + r) + n;
+            const u32x2 w = {pack_bf16x2(st.acc[t][n][r] * inv, st.acc[t][n + 1][r] * inv),
+                             pack_bf16x2(st.acc[t][n + 2][r] * inv, st.acc[t][n + 3][r] * inv)};
+            if (!Pad || dim < dr) *reinterpret_cast<u32x2*>(row + dim) = w;
+        }
+}
+
+// The same as it is, to D floats.
+template <int D, int NT>
+__device__ __forceinline__ void store_part(const State<D, NT>& st, int t, float* row, int lane) {
+    constexpr int NV = Shape<D>::kNV;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NV; n += 4) {
+            const f32x4 w = {st.acc[t][n][r], st.acc[t][n + 1][r], st.acc[t][n + 2][r],
+                             st.acc[t][n + 3][r]};
+            *reinterpret_cast<f32x4*>(row + NV * (4 * (lane >> 4) + r) + n) = w;
+        }
+}
+
+// A merge's lane has D / 64 columns of a row next to one another.
 template <int D>
-__device__ __forceinline__ void store_bf16_row(__bf16* out, const float (&x)[D / 64], float inv,
-                                               int dr, int lane) {
+__device__ __forceinline__ void store_columns(__bf16* out, const float (&x)[D / 64], float inv,
+                                              int dr, int lane) {
     constexpr int P = D / 64;
     if (lane * P >= dr) return;
     if constexpr (P == 1) {
@@ -447,68 +878,11 @@ __device__ __forceinline__ void store_bf16_row(__bf16* out, const float (&x)[D /
     }
 }
 
-// What a row's sums are multiplied by: 0 where it saw nothing. (By its bits: sources that do not
-// honour NaNs would take a NaN sum for none.)
-__device__ __forceinline__ float inverse_sum(float l) {
-    return __float_as_uint(l) != 0u ? 1.f / l : 0.f;
-}
-
-// LDS of a workgroup's partial rows: rows are 4 floats longer than D, so that the 16 rows that
-// lanes write at once lie in different banks.
-template <int D, int NT>
-struct Parts {
-    static constexpr int kRows = 16 * NT;
-    static constexpr int kStride = D + 4;
-    float acc[kWaves][kRows][kStride];
-    float m[kWaves][kRows];
-    float l[kWaves][kRows];
+// A workgroup's LDS: chunks, and, when all wavefronts are done with them, their sums.
+template <int D, bool F8, int NT, int Waves, int Tiles>
+union Shared {
+    Exchange<D, NT, Waves> sums;
+    Tile<D, F8> tiles[Tiles];
 };
-
-// A wavefront's rows into LDS.
-template <int D, int NT>
-__device__ __forceinline__ void put_part(Parts<D, NT>& parts, const State<D, NT>& st, int wave,
-                                         int lane) {
-    constexpr int NV = Shape<D>::kNV;
-    const int j = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float l = wave_sum_xor16_32(st.l[t]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int n = 0; n < NV; n += 4) {
-                const f32x4 w = {st.acc[t][n][r], st.acc[t][n + 1][r], st.acc[t][n + 2][r],
-                                 st.acc[t][n + 3][r]};
-                *reinterpret_cast<f32x4*>(&parts.acc[wave][16 * t + j][NV * (4 * g + r) + n]) = w;
-            }
-        if (g == 0) {
-            parts.m[wave][16 * t + j] = st.m[t];
-            parts.l[wave][16 * t + j] = l;
-        }
-    }
-}
-
-// Row `row` of the parts of wavefronts from, from + step, ... (`count` of them): this lane's
-// columns of the sum over them, with the row's maximum and sum.
-template <int D, int NT>
-__device__ __forceinline__ void sum_parts(const Parts<D, NT>& parts, int row, int from, int step,
-                                          int count, int lane, float (&x)[D / 64], float& m,
-                                          float& l) {
-    constexpr int P = D / 64;
-    m = kNegInf;
-    for (int w = 0; w < count; ++w) m = fmaxf(m, parts.m[from + w * step][row]);
-    l = 0.f;
-#pragma unroll
-    for (int y = 0; y < P; ++y) x[y] = 0.f;
-    // a part that saw nothing, or only NaN, has maximum -inf, and zeros or NaN
-    const float use = m == kNegInf ? 0.f : m;
-    for (int w = 0; w < count; ++w) {
-        const int at = from + w * step;
-        const float f = __builtin_amdgcn_exp2f(parts.m[at][row] - use);
-        l += parts.l[at][row] * f;
-#pragma unroll
-        for (int y = 0; y < P; ++y) x[y] += parts.acc[at][row][lane * P + y] * f;
-    }
-}
 
 }  // namespace ccinfer::hipk::rows

@@ -18,6 +18,7 @@ namespace {
 
 using namespace rows;
 
+constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTile = 16;  // query heads of a workgroup
 
@@ -41,8 +42,8 @@ __device__ __forceinline__ int decode_ctx(int c, int mbpr) {
 }
 
 template <int D, bool F8, bool Pad>
-__global__ __launch_bounds__(kThreads, 2) void sparse_decode_kernel(SparseArgs<D, F8, Pad> a) {
-    __shared__ Parts<D, 1> parts;
+__global__ __launch_bounds__(kThreads, D <= 128 ? 3 : 1) void sparse_decode_kernel(SparseArgs<D, F8, Pad> a) {
+    __shared__ Exchange<D, 1, kWaves> sums;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hkv = a.cache.hkv, dr = a.cache.dims();
@@ -75,29 +76,28 @@ __global__ __launch_bounds__(kThreads, 2) void sparse_decode_kernel(SparseArgs<D
     load_q<D, F8, Pad>(q[0],
                        a.q + (static_cast<int64_t>(b) * a.hq + head0 + min(row, heads - 1)) * dr,
                        row < heads, dr, lane);
-    attend(
-        st, q, a.cache, h, first, chunks, stride, a.scale_log2, lane,
-        [&](int c) {
-            const int k = __builtin_amdgcn_readfirstlane(2 * ((c - first) / stride));
-            return make_pair(__builtin_amdgcn_readlane(block, k), __builtin_amdgcn_readlane(lim, k),
-                             __builtin_amdgcn_readlane(block, k + 1),
-                             __builtin_amdgcn_readlane(lim, k + 1));
-        },
-        [](int, int, uint32_t&) { return false; });
-    put_part<D, 1>(parts, st, wave, lane);
-    __syncthreads();
-    for (int r = wave; r < heads; r += kWaves) {
-        float x[D / 64], m, l;
-        sum_parts<D, 1>(parts, r, 0, 1, kWaves, lane, x, m, l);
-        if (a.splits == 1) {
-            store_bf16_row<D>(a.out + (static_cast<int64_t>(b) * a.hq + head0 + r) * dr, x,
-                              inverse_sum(l), dr, lane);
-        } else {
-            const int64_t at = static_cast<int64_t>(blockIdx.x) * kTile + r;
-#pragma unroll
-            for (int y = 0; y < D / 64; ++y) a.part_acc[at * D + lane * (D / 64) + y] = x[y];
-            if (lane == 0) a.part_ml[at] = float2{m, l};
-        }
+    int k = 0;
+    const int last_k = 2 * ((chunks - 1 - first) / stride);
+    auto next = [&] {
+        const Pair p = make_pair(__builtin_amdgcn_readlane(block, k), __builtin_amdgcn_readlane(lim, k),
+                                 __builtin_amdgcn_readlane(block, k + 1),
+                                 __builtin_amdgcn_readlane(lim, k + 1));
+        k = min(k + 2, last_k);
+        return p;
+    };
+    attend(st, q, a.cache, h, first, chunks, stride, a.scale_log2, lane, next,
+           [](int, int, uint32_t&) { return false; });
+    add_parts(sums, st, wave, kWaves, 0, 1, lane);
+    if (wave != 0) return;
+    const float l = wave_sum_xor16_32(st.l[0]);
+    if (row >= heads) return;
+    if (a.splits == 1) {
+        store_row<D, Pad, 1>(st, 0, l, a.out + (static_cast<int64_t>(b) * a.hq + head0 + row) * dr,
+                             dr, lane);
+    } else {
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * kTile + row;
+        store_part<D, 1>(st, 0, a.part_acc + at * D, lane);
+        if (lane < 16) a.part_ml[at] = float2{st.m[0], l};
     }
 }
 
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void sparse_merge_kernel(const float* par
         for (int y = 0; y < P; ++y) x[y] = x[y] * f + part_acc[at * D + lane * P + y] * fs;
         m = top;
     }
-    store_bf16_row<D>(out + row * dr, x, inverse_sum(l), dr, lane);
+    store_columns<D>(out + row * dr, x, inverse_sum(l), dr, lane);
 }
 
 // Workgroups that keep the chip busy, and chunks a wavefront at least where a list is cut (a part

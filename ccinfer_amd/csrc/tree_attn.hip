@@ -7,12 +7,12 @@
 //   Row i sees position p if p < context_lens[b] - n, or if bit p - (context_lens[b] - n) of its
 //   mask is set. o = sum softmax(q k / sqrt d) v; zeros for a row that sees nothing.
 //
-// The G query heads of a kv head and the nodes make one matrix of n G rows, so a tree of 16
-// nodes at G = 4 fills 64 rows and K and V are read once for all of them. Rows are worked in
-// blocks of up to four wavefronts' tiles (kRows each). Up to kRows rows all four wavefronts take
-// different chunks of the same rows, up to 2 kRows two by two, beyond that every wavefront has
-// rows of its own and the same chunks as the others, at about the same time: what one asks of
-// HBM the others find in L1 or L2.
+// The G query heads of a kv head and the nodes make one matrix of n G rows, so a tree of 64 nodes
+// at G = 4 fills the 256 rows of a workgroup, and K and V are read once for all of them. Rows are
+// worked in blocks of up to eight wavefronts' (32 each, 16 at head dims over 128). In a block of
+// few rows, wavefronts share the chunks instead: up to a wavefront's rows each of the eight takes
+// chunks of its own, up to two wavefronts' four pairs do, and so on; what they found is added up
+// in LDS.
 //
 // Work is cut without knowing the lengths on the host: the (request, row block) items of a kv
 // head, laid end to end in units of their cost, are cut into `slots` equal ranges, one for each
@@ -29,14 +29,18 @@ namespace {
 
 using namespace rows;
 
-constexpr int kThreads = kWaves * 64;
-constexpr int kMaxRequests = kTreeMaxRequests;
-constexpr int kPerThread = kMaxRequests / kThreads;
-constexpr int kMergeSplit = 8;  // workgroups of the merge a slot: 16 of at most 128 rows each
+constexpr int kMaxRequests = kTreeMaxBatch;
+constexpr int kMergeWaves = 4;
+constexpr int kMergeSplit = 16;  // workgroups of the merge a slot: 16 of at most 256 rows each
 
-// Two tiles of 16 rows a wavefront, one at head dims over 128 (two would need 320 registers).
+// Wavefronts of a workgroup, and tiles of 16 rows of each. One workgroup a CU: the ring fills its
+// LDS. At head dims over 128 a wavefront needs the registers of two.
+template <int D>
+constexpr int kWaves = D <= 128 ? 8 : 4;
 template <int D>
 constexpr int kTiles = D <= 128 ? 2 : 1;
+template <int D>
+constexpr int kBlockRows = kWaves<D> * 16 * kTiles<D>;
 
 // The cut item that begins in a slot: its rows, and the last slot that holds a piece of it
 // (rows 0: none).
@@ -76,12 +80,9 @@ struct Request {
     int end;     // tokens that the table row holds
 };
 
-template <class Ptr>
-__device__ __forceinline__ Request request_of(Ptr qsl, Ptr ctx, int b, int total, int mbpr) {
+__device__ __forceinline__ Request request_of(int from, int to, int c, int total, int mbpr) {
     Request r;
-    r.first = qsl[b];
-    const int to = qsl[b + 1];
-    const int c = ctx[b];
+    r.first = from;
     r.n = to - r.first;
     r.before = c - r.n;
     r.nodes = min(to, total) - r.first;
@@ -93,36 +94,106 @@ __device__ __forceinline__ Request request_of(Ptr qsl, Ptr ctx, int b, int total
 // Units of all requests together stay below this (the host refuses other shapes).
 constexpr int kMaxUnits = 1 << 30;
 
-// Cost of a chunk for a block of this many rows. A block of one wavefront's rows reads as many
-// bytes as one of four and computes a quarter.
+// Wavefronts of a block of this many rows that have rows of their own.
 template <int R>
+__device__ __forceinline__ int row_groups(int rows) {
+    return rows <= R ? 1 : (rows <= 2 * R ? 2 : (rows <= 4 * R ? 4 : 8));
+}
+
+// Cost of a chunk for a block. Its bytes take about as long as the products of all wavefronts;
+// fewer rows are bound by the bytes.
+constexpr int kFullUnits = 5;
+template <int D>
 __device__ __forceinline__ int chunk_units(int rows) {
-    return rows <= R ? 2 : (rows <= 2 * R ? 3 : 4);
+    return 2 * rows <= kBlockRows<D> ? 4 : kFullUnits;
 }
 
 // Units of a request's row blocks.
-template <int R>
+template <int D>
 __device__ __forceinline__ int request_units(const Request& r, int G) {
     if (r.nodes <= 0) return 0;
     const int rows = r.nodes * G;
-    const int full = (rows - 1) / (4 * R);
+    const int full = (rows - 1) / kBlockRows<D>;
     const int chunks = (r.end + kChunk - 1) / kChunk;
-    return chunks * (4 * full + chunk_units<R>(rows - full * 4 * R));
+    return chunks * (kFullUnits * full + chunk_units<D>(rows - full * kBlockRows<D>));
+}
+
+// The blocks of chunks first, first + stride, ... below last of a table row, one chunk after the
+// other (the last one again behind them), 64 chunks at a time in the wavefront's lanes: lane 2 k
+// + x of `ids[w]` holds block x of chunk 32 w + k.
+struct BlockIds {
+    const int32_t* table;
+    int end, stride, last, lane;
+    int c;  // of the next Pair
+    int k;  // its place
+    int ids[2];
+    __device__ __forceinline__ BlockIds(const int32_t* t, int first, int last_, int stride_,
+                                        int end_, int lane_)
+        : table(t), end(end_), stride(stride_), last(last_), lane(lane_), c(first), k(0) {
+        load();
+    }
+    __device__ __forceinline__ void load() {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int chunk = c + (32 * w + (lane >> 1)) * stride;
+            const int block = 2 * chunk + (lane & 1);
+            ids[w] = chunk < last && block * kBlock < end ? table[block] : -1;
+        }
+        // here, where it is rare: a load that may be under way at a use makes the compiler wait
+        // for the copies into LDS there too
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+    __device__ __forceinline__ Pair operator()() {
+        const int w = k >= 64 ? ids[1] : ids[0];
+        const int left = end - c * kChunk;
+        const Pair p = make_pair(__builtin_amdgcn_readlane(w, k & 63), left,
+                                 __builtin_amdgcn_readlane(w, (k & 63) + 1), left - kBlock);
+        if (c + stride < last) {
+            c += stride;
+            k += 2;
+            if (k == 128) {
+                k = 0;
+                load();
+            }
+        }
+        return p;
+    }
+    // Of chunk c, whose blocks are there (on0, on1) or not: what its scores are masked by.
+    __device__ __forceinline__ Pair read(int c_, bool on0, bool on1) const {
+        const int left = end - c_ * kChunk;
+        return make_pair(on0 ? 0 : -1, left, on1 ? 0 : -1, left - kBlock);
+    }
+};
+
+// Workgroups go to the eight XCDs in turn. Here those of one XCD take neighbouring places: slots
+// next to one another, whose row blocks read the same chunks, with all heads of each, which lie
+// side by side in memory (an XCD with one head reads 256 bytes of every 2 KB, of which few of its
+// L2's channels hold anything: %TIME%).
+__device__ __forceinline__ int place_on_chip(int i, int n) {
+    const int xcd = i & 7, each = n >> 3, more = n & 7;
+    return xcd * each + min(xcd, more) + (i >> 3);
 }
 
 template <int D, bool F8, bool Pad>
-__global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D, F8, Pad> a) {
+__global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_kernel(
+    TreeArgs<D, F8, Pad> a) {
     constexpr int NT = kTiles<D>;
     constexpr int R = 16 * NT;
-    __shared__ Parts<D, NT> parts;
+    constexpr int W = kWaves<D>;
+    constexpr int kThreads = W * 64;
+    constexpr int kPerThread = kMaxRequests / kThreads;  // requests of a thread
+    __shared__ __align__(16) Shared<D, F8, NT, W, W> shared;
+    __shared__ __align__(16) uint32_t lds_copy[4];
     __shared__ int starts[kMaxRequests + 1];
-    __shared__ int64_t wave_sum[kWaves];
+    __shared__ int froms[kMaxRequests], tos[kMaxRequests], ctxs[kMaxRequests];
+    __shared__ int64_t wave_sum[W];
     __shared__ int first_request;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hkv = a.cache.hkv;
     const int G = a.hq / hkv, dr = a.cache.dims();
-    const int h = blockIdx.x % hkv, slot = blockIdx.x / hkv;
+    const int at_chip = place_on_chip(blockIdx.x, gridDim.x);
+    const int h = at_chip % hkv, slot = at_chip / hkv;
     SlotDesc* desc = a.desc + static_cast<int64_t>(h) * a.slots + slot;
 
     // Where each request's units start.
@@ -132,9 +203,14 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D,
 #pragma unroll
     for (int x = 0; x < kPerThread; ++x) {
         const int b = tid * per + x;
-        units[x] = x < per && b < a.batch
-                       ? request_units<R>(request_of(a.qsl, a.ctx, b, a.total, a.mbpr), G)
-                       : 0;
+        units[x] = 0;
+        if (x < per && b < a.batch) {
+            const int from = a.qsl[b], to = a.qsl[b + 1], c = a.ctx[b];
+            froms[b] = from;
+            tos[b] = to;
+            ctxs[b] = c;
+            units[x] = request_units<D>(request_of(from, to, c, a.total, a.mbpr), G);
+        }
         sum += units[x];
     }
     int64_t incl = sum;
@@ -147,7 +223,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D,
     __syncthreads();
     int64_t before = incl - sum, total_units = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
         before += w < wave ? wave_sum[w] : 0;
         total_units += wave_sum[w];
     }
@@ -177,17 +253,19 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D,
     for (int u = __builtin_amdgcn_readfirstlane(u0); u < u1;) {
         while (starts[b + 1] <= u) ++b;
         b = __builtin_amdgcn_readfirstlane(b);
-        const Request req = request_of(unwritten(a.qsl), unwritten(a.ctx), b, a.total, a.mbpr);
+        const Request req = request_of(__builtin_amdgcn_readfirstlane(froms[b]),
+                                       __builtin_amdgcn_readfirstlane(tos[b]),
+                                       __builtin_amdgcn_readfirstlane(ctxs[b]), a.total, a.mbpr);
         const int all_rows = req.nodes * G;
         const int chunks = (req.end + kChunk - 1) / kChunk;
-        const int full = (all_rows - 1) / (4 * R);
+        const int full = (all_rows - 1) / kBlockRows<D>;
         const int local = u - __builtin_amdgcn_readfirstlane(starts[b]);
-        const int rb = min(local / (4 * chunks), full);
-        const int row0 = rb * 4 * R;
-        const int block_rows = min(all_rows - row0, 4 * R);
-        const int weight = chunk_units<R>(block_rows);
+        const int rb = min(local / (kFullUnits * chunks), full);
+        const int row0 = rb * kBlockRows<D>;
+        const int block_rows = min(all_rows - row0, kBlockRows<D>);
+        const int weight = chunk_units<D>(block_rows);
         const int item = chunks * weight;
-        const int from = local - rb * 4 * chunks;
+        const int from = local - rb * kFullUnits * chunks;
         const int to = min(item, from + (u1 - u));
         // a chunk belongs to the slot that its first unit lies in
         const int c0 = (from + weight - 1) / weight, c1 = (to + weight - 1) / weight;
@@ -197,72 +275,94 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D,
             own = SlotDesc{req.first, row0, block_rows, (u - from + item - 1) / quota};
 
         // Wavefronts by rows, and those of the same rows by chunks.
-        const int groups = block_rows <= R ? 1 : (block_rows <= 2 * R ? 2 : 4);
-        const int share = kWaves / groups;
+        const int groups = row_groups<R>(block_rows);
+        const int share = W / groups;
         const int group = wave % groups, part = wave / groups;
         State<D, NT> st;
         st.clear();
         const bool busy = group * R < block_rows;
-        if (busy) {
-            bf16x8 q[NT][Shape<D>::kSteps];
-            const uint32_t* mask_row[NT];
+        bf16x8 q[NT][Shape<D>::kSteps];
+        const uint32_t* mask_row[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int row = group * R + 16 * t + (lane & 15);
+            const bool live = row < block_rows;
+            const int r = row0 + (live ? row : 0);
+            const int node = r / G;
+            const int64_t token = req.first + node;
+            load_q<D, F8, Pad>(q[t], a.q + (token * a.hq + h * G + (r - node * G)) * dr, live, dr,
+                               lane);
+            mask_row[t] = a.mask + token * a.words;
+        }
+        const int32_t* table = a.table + static_cast<int64_t>(b) * a.mbpr;
+        BlockIds ids(table, c0 + part, c1, share, req.end, lane);
+        auto chunk = [&](int c) {
+            const int cb = c * kChunk;
+            return make_pair(table[2 * c], req.end - cb,
+                             cb + kBlock < req.end ? table[2 * c + 1] : -1, req.end - cb - kBlock);
+        };
+        auto seen = [&](int c, int t, uint32_t& bits) {
+            const int o = c * kChunk - req.before;  // tree node of the chunk's first token
+            if (o <= -kChunk) return false;
+            const uint32_t* m = mask_row[t];
+            if (o < 0) {
+                bits = (m[0] << -o) | ((1u << -o) - 1u);
+            } else {
+                const int w = o >> 5;
+                const uint32_t lo = w < a.words ? m[w] : 0u;
+                const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
+                bits = static_cast<uint32_t>(((static_cast<uint64_t>(hi) << 32) | lo) >> (o & 31));
+            }
+            return true;
+        };
+        const int steps = (c1 - c0 + share - 1) / share;
+        bool left_out;
+        if (c0 >= c1)
+            left_out = false;
+        else if (groups == 1)
+            left_out = attend_alone(st, q, a.cache, shared.tiles[wave],
+                                    LdsCopy(lds_copy, shared.tiles + wave), h, c0 + part, c1,
+                                    share, a.scale_log2, lane, ids, seen);
+        else if (groups == 2)
+            left_out = attend_shared<2, 2>(st, q, a.cache, shared.tiles + 2 * part, LdsCopy(lds_copy, shared.tiles + 2 * part),
+                                           group, h,
+                                           c0 + part, c1, share, steps, busy, a.scale_log2, lane,
+                                           ids, seen);
+        else if (groups == 4)
+            left_out = attend_shared<4, 4>(st, q, a.cache, shared.tiles + 4 * part, LdsCopy(lds_copy, shared.tiles + 4 * part),
+                                           group, h,
+                                           c0 + part, c1, share, steps, busy, a.scale_log2, lane,
+                                           ids, seen);
+        else if constexpr (W == 8)
+            left_out = attend_shared<8, 8>(st, q, a.cache, shared.tiles, LdsCopy(lds_copy, shared.tiles),
+                                           group, h, c0, c1, 1,
+                                           steps, busy, a.scale_log2, lane, ids, seen);
+        else
+            left_out = false;
+        if (left_out)
+            add_unbounded(st, a.cache, h, c0 + part, c1, share, lane, chunk, seen);
+
+        __syncthreads();  // the tiles' place is the sums' now
+        add_parts(shared.sums, st, part, share, group, groups, lane);
+        if (part == 0) {
+            const int64_t piece = (static_cast<int64_t>(h) * a.slots + slot) * 2 + which;
+            float* pa = a.part_acc + piece * a.row_cap * D;
+            float2* pm = a.part_ml + piece * a.row_cap;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int row = group * R + 16 * t + (lane & 15);
-                const bool live = row < block_rows;
-                const int r = row0 + (live ? row : 0);
-                const int node = r / G;
-                const int64_t token = req.first + node;
-                load_q<D, F8, Pad>(q[t], a.q + (token * a.hq + h * G + (r - node * G)) * dr, live,
-                                   dr, lane);
-                mask_row[t] = a.mask + token * a.words;
-            }
-            const auto table = unwritten(a.table) + static_cast<int64_t>(b) * a.mbpr;
-            auto chunk = [&](int c) {
-                const int cb = c * kChunk;
-                const int pb0 = table[2 * c];
-                const int pb1 = cb + kBlock < req.end ? table[2 * c + 1] : -1;
-                return make_pair(pb0, req.end - cb, pb1, req.end - cb - kBlock);
-            };
-            auto seen = [&](int c, int t, uint32_t& bits) {
-                const int o = c * kChunk - req.before;  // tree node of the chunk's first token
-                if (o <= -kChunk) return false;
-                const uint32_t* m = mask_row[t];
-                if (o < 0) {
-                    bits = (m[0] << -o) | ((1u << -o) - 1u);
+                const float l = wave_sum_xor16_32(st.l[t]);
+                if (row >= block_rows) continue;
+                if (whole) {
+                    const int r = row0 + row;
+                    const int node = r / G;
+                    const int64_t token = req.first + node;
+                    store_row<D, Pad, NT>(
+                        st, t, l, a.out + (token * a.hq + h * G + (r - node * G)) * dr, dr, lane);
                 } else {
-                    const int w = o >> 5;
-                    const uint32_t lo = w < a.words ? m[w] : 0u;
-                    const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
-                    bits = static_cast<uint32_t>(((static_cast<uint64_t>(hi) << 32) | lo) >>
-                                                 (o & 31));
+                    store_part<D, NT>(st, t, pa + static_cast<int64_t>(row) * D, lane);
+                    if (lane < 16) pm[row] = float2{st.m[t], l};
                 }
-                return true;
-            };
-            if (attend(st, q, a.cache, h, c0 + part, c1, share, a.scale_log2, lane,
-                                  chunk, seen))
-                add_unbounded(st, a.cache, h, c0 + part, c1, share, lane, chunk, seen);
-        }
-
-        const int64_t piece = (static_cast<int64_t>(h) * a.slots + slot) * 2 + which;
-        float* pa = a.part_acc + piece * a.row_cap * D;
-        float2* pm = a.part_ml + piece * a.row_cap;
-        put_part<D, NT>(parts, st, wave, lane);
-        __syncthreads();
-        for (int row = wave; row < block_rows; row += kWaves) {
-            float x[D / 64], m, l;
-            sum_parts<D, NT>(parts, row % R, row / R, groups, share, lane, x, m, l);
-            if (whole) {
-                const int r = row0 + row;
-                const int node = r / G;
-                const int64_t token = req.first + node;
-                store_bf16_row<D>(a.out + (token * a.hq + h * G + (r - node * G)) * dr, x,
-                                  inverse_sum(l), dr, lane);
-            } else {
-#pragma unroll
-                for (int y = 0; y < D / 64; ++y)
-                    pa[static_cast<int64_t>(row) * D + lane * (D / 64) + y] = x[y];
-                if (lane == 0) pm[row] = float2{m, l};
             }
         }
         __syncthreads();
@@ -274,7 +374,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attention_kernel(TreeArgs<D,
 // Rows of the cut items, a wavefront each in turn: the pieces of slots [slot, last_slot], the
 // first of them the slot's item that begins in it, the others those that begin before them.
 template <int D>
-__global__ __launch_bounds__(kThreads) void tree_merge_kernel(
+__global__ __launch_bounds__(kMergeWaves * 64) void tree_merge_kernel(
     const SlotDesc* desc, const float* part_acc, const float2* part_ml, __bf16* out, int slots,
     int row_cap, int hq, int hkv, int dr) {
     constexpr int P = D / 64;
@@ -284,7 +384,8 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(
     const int G = hq / hkv;
     const SlotDesc d = desc[static_cast<int64_t>(h) * slots + slot];
     const int64_t base = (static_cast<int64_t>(h) * slots + slot) * 2;
-    for (int row = blockIdx.y * kWaves + wave; row < d.rows; row += kMergeSplit * kWaves) {
+    for (int row = blockIdx.y * kMergeWaves + wave; row < d.rows;
+         row += kMergeSplit * kMergeWaves) {
         float m = kNegInf, l = 0.f, x[P];
 #pragma unroll
         for (int y = 0; y < P; ++y) x[y] = 0.f;
@@ -303,25 +404,24 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(
         }
         const int r = d.first_row + row;
         const int node = r / G;
-        store_bf16_row<D>(
+        store_columns<D>(
             out + ((static_cast<int64_t>(d.first_token) + node) * hq + h * G + (r - node * G)) * dr,
             x, inverse_sum(l), dr, lane);
     }
 }
 
-// Workgroups that the chip holds at once, two for each of 256 CUs.
-constexpr int kResident = 512;
-// Units of a slot at least: four chunks for a wavefront of a small block.
-constexpr int kMinUnits = 32;
+// Workgroups that the chip holds at once: one for each of 256 CUs.
+constexpr int kResident = 256;
+// Units of a slot at least: what two to sixteen chunks cost.
+constexpr int kMinUnits = 64;
 
 int slots_of(int hkv) { return std::max(1, kResident / hkv); }
 
 int mfma_dim(int head_dim) { return head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256); }
 
 int row_cap_of(int total, int hq, int hkv, int D) {
-    const int wave_rows = D <= 128 ? 32 : 16;
     const int64_t rows = static_cast<int64_t>(total) * (hq / hkv);
-    return static_cast<int>(std::min<int64_t>(rows, 4 * wave_rows));
+    return static_cast<int>(std::min<int64_t>(rows, D <= 128 ? kBlockRows<128> : kBlockRows<256>));
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -367,9 +467,10 @@ hipError_t launch(const TreeAttention& t, void* workspace, hipStream_t stream) {
     a.part_ml = reinterpret_cast<float2*>(ws + w.ml);
     a.part_acc = reinterpret_cast<float*>(ws + w.acc);
     const unsigned grid = static_cast<unsigned>(a.slots) * t.hkv;
-    hipLaunchKernelGGL((tree_attention_kernel<D, F8, Pad>), dim3(grid), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((tree_attention_kernel<D, F8, Pad>), dim3(grid), dim3(kWaves<D> * 64), 0, stream, a);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-    hipLaunchKernelGGL((tree_merge_kernel<D>), dim3(grid, kMergeSplit), dim3(kThreads), 0, stream,
+    hipLaunchKernelGGL((tree_merge_kernel<D>), dim3(grid, kMergeSplit), dim3(kMergeWaves * 64), 0,
+                       stream,
                        a.desc, a.part_acc, a.part_ml, a.out, a.slots, a.row_cap, t.hq, t.hkv,
                        t.head_dim);
     return hipGetLastError();
@@ -379,13 +480,12 @@ hipError_t launch(const TreeAttention& t, void* workspace, hipStream_t stream) {
 
 bool tree_attention_supported(int batch, int total, int mbpr, int hq, int hkv, int head_dim,
                               bool fp8) {
-    if (batch > kTreeMaxRequests || head_dim > 256 || head_dim % 8 != 0) return false;
+    if (batch > kTreeMaxBatch || head_dim > 256 || head_dim % 8 != 0) return false;
     if (fp8 && head_dim != 64 && head_dim != 128) return false;
-    // units: 4 a chunk and row block
-    const int D = mfma_dim(head_dim);
-    const int64_t block = D <= 128 ? 128 : 64;
+    // units: at most kFullUnits a chunk and row block
+    const int64_t block = head_dim <= 128 ? kBlockRows<128> : kBlockRows<256>;
     const int64_t blocks = static_cast<int64_t>(total) * (hq / hkv) / block + batch;
-    const int64_t units = 4 * (static_cast<int64_t>(mbpr) / 2 + 1);
+    const int64_t units = kFullUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
     // below 2^28 row blocks the product keeps 64 bits; a request's and all requests' units, and
     // the ends of the slots, keep 32
     return blocks < (int64_t{1} << 28) && units * blocks < kMaxUnits &&

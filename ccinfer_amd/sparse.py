@@ -86,7 +86,8 @@ def score_kv_blocks(q: torch.Tensor, key_bounds: torch.Tensor, block_table: torc
     """float32 [rows, kv heads, max_blocks_per_req]: the largest logit that any key within a
     block's bounds could have with any query head of the kv head, sum_d max(q_d lo_d, q_d hi_d) /
     sqrt(head_dim). -inf past the context, for negative table entries, and for rows whose context
-    the table does not hold; NaN for NaN or infinite bounds. q [rows, q heads, head_dim]."""
+    the table does not hold; NaN for NaN bounds, NaN or an infinity for infinite ones. q [rows, q
+    heads, head_dim]."""
     op = "score_kv_blocks"
     _require(q.is_cuda, op)
     dev = current_device()

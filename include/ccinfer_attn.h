@@ -544,8 +544,8 @@ int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* k
 /* scores [batch_size][num_kv_heads][max_blocks_per_req] float: for block j of the row the largest,
  * over the query heads of the kv head, of sum_d max(q_d lo_d, q_d hi_d) / sqrt(head_dim): no key
  * of the block gives a larger logit. -infinity past the context, for negative table entries, and
- * for rows whose context the table does not hold; NaN where a bound or q is NaN or a bound is
- * infinite. */
+ * for rows whose context the table does not hold; NaN where a bound or q is NaN, NaN or an
+ * infinity where a bound is infinite. */
 int ccinfer_score_kv_blocks(const void* q, const void* key_bounds, const int32_t* block_table,
                             const int32_t* context_lens, float* scores, int batch_size,
                             int max_blocks_per_req, int num_q_heads, int num_kv_heads,

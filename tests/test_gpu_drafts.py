@@ -13,6 +13,11 @@ pytestmark = pytest.mark.gpu
 NAN = float("nan")
 
 
+@pytest.fixture(autouse=True)
+def seed():
+    torch.manual_seed(1234)
+
+
 def i32(a, dev):
     return torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)
 

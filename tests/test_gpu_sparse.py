@@ -13,6 +13,11 @@ pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
 
 
+@pytest.fixture(autouse=True)
+def seed():
+    torch.manual_seed(1234)
+
+
 def i32(a, dev):
     return torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)
 
@@ -123,7 +128,9 @@ def test_scores_of_nan(gpu):
     q = torch.randn(2, 4, 64).bfloat16()
     q[1, 2, 7] = NAN
     got = cc.score_kv_blocks(q.to(gpu), bounds.to(gpu), i32(table, gpu), i32(ctx, gpu)).cpu().numpy()
-    assert np.isnan(got[0, 0, [3, 4]]).all() and np.isfinite(got[0, 0, [0, 1, 2, 5, 6]]).all()
+    # 0 x inf in the part of the other sign, or inf
+    assert np.isnan(got[0, 0, 3]) and got[0, 0, 4] != -INF and not np.isfinite(got[0, 0, 4])
+    assert np.isfinite(got[0, 0, [0, 1, 2, 5, 6]]).all()
     assert np.isnan(got[1, 0, :7]).all() and np.isneginf(got[:, 0, 7:]).all()
 
 
