@@ -5,7 +5,8 @@
 // Layout of the products (as in decode_core.hpp): S^T = K . Q^T and O^T = V^T . P^T, so that the
 // probabilities leave the first product in the lanes that the second one takes them from. Lane
 // (j = lane & 15, g = lane >> 4) holds row j of a tile; its eight scores of a chunk are those of
-// tokens T(g, e) = 16 (e / 4) + 4 g + e % 4, and acc[t][n][r] is O[16 t + j][NV (4 g + r) + n].
+// tokens T(g, e) = 16 (e / 4) + 4 g + e % 4, and acc[t][n][r] is O[16 t + j][NV (4 g + r) + n],
+// or [16 n + 4 g + r] where V comes out of LDS transposed (Tr).
 //
 // Two ways of the chunks. One wavefront by itself (attend) loads K and V into registers, one set
 // each: K of the next chunk is asked for when the scores are done, V when the second product is, so
@@ -17,7 +18,6 @@
 // through the ring %TIME%).
 #pragma once
 
-#include <cstddef>
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -63,45 +63,56 @@ struct Cache {
 struct Pair {
     int pb[2];
     int lim[2];
-    bool on[2];
-    __device__ __forceinline__ bool any() const { return on[0] || on[1]; }
+    uint32_t on;  // a bit a block
+    __device__ __forceinline__ bool is_on(int b) const { return ((on >> b) & 1u) != 0; }
     __device__ __forceinline__ bool whole() const {
-        return on[0] && on[1] && lim[0] == kBlock && lim[1] == kBlock;
+        return on == 3u && lim[0] + lim[1] == 2 * kBlock;
     }
 };
 
 // pb < 0 or lim <= 0: the block is not there.
 __device__ __forceinline__ Pair make_pair(int pb0, int lim0, int pb1, int lim1) {
+    if ((pb0 | pb1) >= 0 && min(lim0, lim1) >= kBlock)  // nearly always
+        return Pair{{pb0, pb1}, {kBlock, kBlock}, 3u};
     Pair p;
-    p.on[0] = pb0 >= 0 && lim0 > 0;
-    p.on[1] = pb1 >= 0 && lim1 > 0;
+    const bool on0 = pb0 >= 0 && lim0 > 0, on1 = pb1 >= 0 && lim1 > 0;
     const int l0 = min(lim0, kBlock), l1 = min(lim1, kBlock);
-    p.pb[0] = p.on[0] ? pb0 : (p.on[1] ? pb1 : 0);
-    p.lim[0] = p.on[0] ? l0 : (p.on[1] ? l1 : 1);
-    p.pb[1] = p.on[1] ? pb1 : p.pb[0];
-    p.lim[1] = p.on[1] ? l1 : p.lim[0];
+    p.on = (on0 ? 1u : 0u) | (on1 ? 2u : 0u);
+    p.pb[0] = on0 ? pb0 : (on1 ? pb1 : 0);
+    p.lim[0] = on0 ? l0 : (on1 ? l1 : 1);
+    p.pb[1] = on1 ? pb1 : p.pb[0];
+    p.lim[1] = on1 ? l1 : p.lim[0];
     return p;
 }
 
 // A chunk's K and V in registers. K: lane (i, g) has of token i of each block the dims q_dim(kk, g)
-// .. + 8 of every step (fp8: 16 bytes hold two steps'). V: dims NV i .. of tokens T(g, e). The
-// scales of an fp8 chunk: of tokens 4 g .. of each block.
+// .. + 8 of every step (fp8: 16 bytes hold two steps'). V: dims NV i .. of tokens T(g, e), or (Tr)
+// dim 16 n + i of tokens T(g, 0..7), the operands as they are. The scales of an fp8 chunk: of
+// tokens 4 g .. of each block.
 template <int D, bool F8>
 struct KRegs {
     u32x4 k[2][F8 ? Shape<D>::kSteps / 2 : Shape<D>::kSteps];
     u32x4 s[F8 ? 2 : 1];
 };
-template <int D, bool F8>
+template <int D, bool F8, bool Tr = false>
 struct VRegs {
-    uint32_t v[8][F8 ? (Shape<D>::kNV + 3) / 4 : Shape<D>::kVWords];
+    static_assert(!Tr || !F8);
+    static constexpr int kRows = Tr ? Shape<D>::kNV : 8;
+    static constexpr int kWords = Tr ? 4 : (F8 ? (Shape<D>::kNV + 3) / 4 : Shape<D>::kVWords);
+    uint32_t v[kRows][kWords];
     u32x4 s[F8 ? 2 : 1];
 };
 
-// A chunk's K and V in LDS: 32 rows of kPieces 16-byte pieces each. Piece x of row r of K lies at
-// place x ^ swizzle(r) of its row: the 16 rows that lanes read at once then lie in different
-// banks. V is read row by row, and lies as it is.
+// A chunk's K and V in LDS: 32 rows of kPieces 16-byte pieces each. Piece x of row r lies at place
+// x ^ swizzle(r) of its row: the 16 rows that lanes read at once then lie in different banks.
+template <bool F8>
+struct TileScales {};
+template <>
+struct TileScales<true> {
+    float scales[2][kChunk];  // of K, of V
+};
 template <int D, bool F8>
-struct Tile {
+struct Tile : TileScales<F8> {
     static constexpr int kPieces = D * (F8 ? 1 : 2) / 16;
     static constexpr int kBytes = kChunk * kPieces * 16;
     static constexpr int kLoads = kBytes / (64 * 16);  // of K, and of V: a wavefront moves 1 KB
@@ -109,9 +120,12 @@ struct Tile {
         constexpr int kRowsPerLine = kPieces >= 16 ? 1 : 16 / kPieces;  // a line of 256 bytes
         return (row / kRowsPerLine) & ((kPieces < 16 ? kPieces : 16) - 1);
     }
-    char kv[2][kBytes];
-    float scales[F8 ? 2 : 1][F8 ? kChunk : 4];  // of K, of V
+    static constexpr int kRowBytes = 16 * kPieces;
+    static constexpr uint32_t kKvAt = F8 ? sizeof(TileScales<true>) : 0;
+    alignas(256) char kv[2][kBytes];
 };
+static_assert(sizeof(TileScales<true>) == 256 && sizeof(Tile<64, true>) == 256 + 2 * 2048 &&
+              sizeof(Tile<64, false>) == 2 * 4096);
 
 // First of the eight dims that lane group g holds in step kk.
 template <bool F8>
@@ -244,17 +258,19 @@ struct Copier {
         x0 = Of == 1 ? 0 : r % (2 * T::kLoads / kEach) * kEach;
         stride = static_cast<uint32_t>(c.hkv) * c.dims() * (F8 ? 1 : 2);
     }
+    // Head h of a block's first token, of K or V.
+    __device__ __forceinline__ const char* block(bool of_v, int pb) const {
+        return reinterpret_cast<const char*>((of_v ? cache.v : cache.k) +
+                                             static_cast<int64_t>(h) * cache.dims()) +
+               static_cast<uint64_t>(static_cast<uint32_t>(pb)) * (stride * kBlock);
+    }
     // Instruction z of K (of_v false) or V, of a tile at byte `tile` of the ring.
-    __device__ __forceinline__ void one(uint32_t tile, const Pair& p, bool of_v, int z) const {
-        const bool second = z >= T::kLoads / 2;
-        const int pb = second ? p.pb[1] : p.pb[0], lim = second ? p.lim[1] : p.lim[0];
+    __device__ __forceinline__ void one(uint32_t tile, const char* blk, int lim, bool of_v,
+                                        int z) const {
         const int row0 = z * kRows & (kBlock - 1);  // wave-uniform
         const int row = lane / T::kPieces;
         // swizzle(row0 + row): the bits of the two do not meet
-        int piece = lane % T::kPieces;
-        if (!of_v) piece ^= T::swizzle(row) ^ T::swizzle(row0);
-        const char* blk = reinterpret_cast<const char*>(
-            of_v ? block_rows(cache.v, cache, pb, h) : block_rows(cache.k, cache, pb, h));
+        const int piece = lane % T::kPieces ^ T::swizzle(row) ^ T::swizzle(row0);
         const bool past = Pad && 8 * piece >= cache.dr;
         // rows past the last are copies of it
         const char* src = blk + (__umul24(min(row0 + row, lim - 1), stride) +
@@ -263,7 +279,7 @@ struct Copier {
         // that are not stored
         if (past && !of_v) src = reinterpret_cast<const char*>(kZeros);
         __builtin_amdgcn_global_load_lds(
-            src, to.at(tile + ((of_v ? T::kLoads : 0) + z) * 64 * 16), 16, 0, 0);
+            src, to.at(tile + T::kKvAt + ((of_v ? T::kLoads : 0) + z) * 64 * 16), 16, 0, 0);
     }
     // The scales of K, of V, or of both.
     __device__ __forceinline__ void scales(uint32_t tile, const Pair& p, bool of_k,
@@ -272,21 +288,39 @@ struct Copier {
         const int pb = (lane & kBlock) != 0 ? p.pb[1] : p.pb[0];
         const float* src = scale + (static_cast<int64_t>(pb) * cache.hkv + h) * kBlock +
                            (lane & (kBlock - 1));
+        // (scales come first in a tile)
         if (lane < kChunk ? of_k : of_v)
-            __builtin_amdgcn_global_load_lds(src, to.at(tile + offsetof(T, scales)), 4, 0, 0);
+            __builtin_amdgcn_global_load_lds(src, to.at(tile), 4, 0, 0);
     }
     // This wavefront's part of a chunk, into tile `slot` of the ring.
     __device__ __forceinline__ void ask(int slot, const Pair& p) const {
         const uint32_t tile = static_cast<uint32_t>(slot) * sizeof(T);
+        const bool of_v = x0 >= T::kLoads;
+        const int z0 = x0 % T::kLoads;
+        if constexpr (Of >= 4) {
+            const bool second = z0 >= T::kLoads / 2;
+            const int lim = second ? p.lim[1] : p.lim[0];
+            const char* blk = block(of_v, second ? p.pb[1] : p.pb[0]);
 #pragma unroll
-        for (int y = 0; y < kEach; ++y)
-            one(tile, p, x0 >= T::kLoads, x0 % T::kLoads + y);
+            for (int y = 0; y < kEach; ++y) one(tile, blk, lim, of_v, z0 + y);
+        } else {
+            half(tile, p, of_v);
+        }
         if constexpr (F8) scales(tile, p, true, true);
     }
-    // All of a chunk's K, or V (Of = 1, one tile).
-    __device__ __forceinline__ void ask_half(const Pair& p, bool of_v) const {
+    // All of a chunk's K, or V.
+    __device__ __forceinline__ void half(uint32_t tile, const Pair& p, bool of_v) const {
 #pragma unroll
-        for (int z = 0; z < T::kLoads; ++z) one(0, p, of_v, z);
+        for (int b = 0; b < 2; ++b) {
+            const char* blk = block(of_v, p.pb[b]);
+#pragma unroll
+            for (int y = 0; y < T::kLoads / 2; ++y)
+                one(tile, blk, p.lim[b], of_v, b * (T::kLoads / 2) + y);
+        }
+    }
+    // The same of a wavefront by itself (Of = 1), with the scales.
+    __device__ __forceinline__ void ask_half(const Pair& p, bool of_v) const {
+        half(0, p, of_v);
         if constexpr (F8) scales(0, p, !of_v, of_v);
     }
 };
@@ -308,34 +342,54 @@ __device__ __forceinline__ void read_k(KRegs<D, F8>& r, const Tile<D, F8>& tile,
     }
 }
 
-template <int D, bool F8>
-__device__ __forceinline__ void read_v(VRegs<D, F8>& r, const Tile<D, F8>& tile, int lane) {
-    constexpr int kWords = sizeof(r.v[0]) / 4;
+// fp8: the lane's dims of each token.
+template <int D>
+__device__ __forceinline__ void read_v(VRegs<D, true>& r, const Tile<D, true>& tile, int lane) {
+    using T = Tile<D, true>;
+    constexpr int kWords = VRegs<D, true>::kWords;
     const int i = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const char* from = tile.kv[1] +
-                           (16 * (e >> 2) + 4 * g + (e & 3)) * Tile<D, F8>::kPieces * 16 +
-                           i * kWords * 4;
+        const int row = 16 * (e >> 2) + 4 * g + (e & 3);
+        const int byte = i * kWords * 4;
+        const char* from = tile.kv[1] + row * T::kRowBytes +
+                           ((byte / 16 ^ T::swizzle(row)) * 16 + byte % 16);
         if constexpr (kWords == 1) {
             r.v[e][0] = *reinterpret_cast<const uint32_t*>(from);
-        } else if constexpr (kWords == 2) {
+        } else {
             const u32x2 w = *reinterpret_cast<const u32x2*>(from);
             r.v[e][0] = w[0];
             r.v[e][1] = w[1];
-        } else {
-#pragma unroll
-            for (int x = 0; x < kWords; x += 4) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(from + 4 * x);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) r.v[e][x + y] = w[y];
-            }
         }
     }
-    if constexpr (F8) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-            r.s[b] = *reinterpret_cast<const u32x4*>(&tile.scales[F8 ? 1 : 0][16 * b + 4 * g]);
+    for (int b = 0; b < 2; ++b)
+        r.s[b] = *reinterpret_cast<const u32x4*>(&tile.scales[1][16 * b + 4 * g]);
+}
+
+// bf16: LDS hands each 16 lanes four tokens' 16 dims transposed, a lane's being one dim of them;
+// lane s gives the place of four dims, 4 (s % 4) .., of token s / 4.
+template <int D>
+__device__ __forceinline__ void read_v(VRegs<D, false, true>& r, const Tile<D, false>& tile,
+                                       int lane) {
+    using T = Tile<D, false>;
+    using Four = short __attribute__((ext_vector_type(4)));
+    using InLds = __attribute__((address_space(3))) Four*;
+    const int row = lane >> 2;
+    // of dims 4 (s % 4) ..; those of 16 n + .. lie at `at` ^ 32 n
+    int at = row * T::kRowBytes + (((lane & 3) / 2 ^ T::swizzle(row)) * 16 + (lane & 1) * 8);
+    asm("" : "+v"(at));  // one register, not one for each n through the loop
+#pragma unroll
+    for (int n = 0; n < Shape<D>::kNV; ++n) {
+        const char* from = tile.kv[1] + (at ^ 32 * n);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const u32x2 w = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (InLds)const_cast<char*>(from + b * kBlock * T::kRowBytes)));
+            r.v[n][2 * b] = w[0];
+            r.v[n][2 * b + 1] = w[1];
+        }
     }
 }
 
@@ -365,8 +419,9 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
-template <int D, int NT>
+template <int D, int NT, bool Tr = false>
 struct State {
+    static constexpr bool kTr = Tr;
     f32x4 acc[NT][Shape<D>::kNV];
     float m[NT];  // what the exponents are taken from, base 2, the same in a row's four lanes
     float l[NT];  // this lane's part of the sum
@@ -378,6 +433,22 @@ struct State {
             m[t] = kNegInf;
             l[t] = 0.f;
         }
+    }
+    // The dim of acc[.][n][r] in lane group g.
+    static __device__ __forceinline__ int dim(int n, int r, int g) {
+        return Tr ? 16 * n + 4 * g + r : Shape<D>::kNV * (4 * g + r) + n;
+    }
+    // Four neighbouring dims of a row, set x of kNV, from dim four_dim(x, g) on.
+    __device__ __forceinline__ f32x4 four(int t, int x) const {
+        if constexpr (Tr) {
+            return acc[t][x];
+        } else {
+            const int r = x % 4, n = x / 4 * 4;
+            return f32x4{acc[t][n][r], acc[t][n + 1][r], acc[t][n + 2][r], acc[t][n + 3][r]};
+        }
+    }
+    static __device__ __forceinline__ int four_dim(int x, int g) {
+        return Tr ? dim(x, 0, g) : dim(x / 4 * 4, x % 4, g);
     }
 };
 
@@ -394,22 +465,22 @@ __device__ __forceinline__ uint32_t v_word(const VRegs<D, F8>& r, int e, int w) 
 
 // Zeros in place of the infinities and NaN of this lane's V; whether there were any. (An exponent
 // of all ones plus one, or an fp8 NaN's seven ones plus one, carries into the sign's place.)
-template <int D, bool F8>
-__device__ __forceinline__ bool clear_unbounded(VRegs<D, F8>& r) {
+template <int D, bool F8, bool Tr>
+__device__ __forceinline__ bool clear_unbounded(VRegs<D, F8, Tr>& r) {
     constexpr uint32_t kExp = F8 ? 0x7f7f7f7fu : 0x7f807f80u;
     constexpr uint32_t kOne = F8 ? 0x01010101u : 0x00800080u;
     constexpr uint32_t kSign = F8 ? 0x80808080u : 0x80008000u;
     uint32_t any = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (auto& row : r.v)
 #pragma unroll
-        for (auto& w : r.v[e]) any |= ((w & kExp) + kOne) & kSign;
+        for (auto& w : row) any |= ((w & kExp) + kOne) & kSign;
     const bool found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
     if (found) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (auto& row : r.v)
 #pragma unroll
-            for (auto& w : r.v[e]) {
+            for (auto& w : row) {
                 const uint32_t bad = ((w & kExp) + kOne) & kSign;
                 w &= ~((bad >> (F8 ? 7 : 15)) * (F8 ? 0xffu : 0xffffu));
             }
@@ -474,7 +545,7 @@ __device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, i
             for (int e = 0; e < 8; ++e) {
                 const int b = e >> 2, key = 4 * (lane >> 4) + (e & 3);
                 const bool ok =
-                    p.on[b] && key < p.lim[b] && ((bits[t] >> (16 * b + key)) & 1u) != 0;
+                    p.is_on(b) && key < p.lim[b] && ((bits[t] >> (16 * b + key)) & 1u) != 0;
                 sc[t][e] = ok ? sc[t][e] : kNegInf;
             }
     }
@@ -484,8 +555,8 @@ __device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, i
 // The reference that the exponents are taken from follows the maximum only when a score passes it
 // by 2^8: probabilities up to 256 are as good in floating point, and without a new one nothing is
 // compared across lanes and no sum is scaled.
-template <int D, int NT>
-__device__ __forceinline__ void follow_maximum(State<D, NT>& st, const float (&sc)[NT][8],
+template <int D, int NT, bool Tr>
+__device__ __forceinline__ void follow_maximum(State<D, NT, Tr>& st, const float (&sc)[NT][8],
                                                float scale_log2) {
     float top[NT];
     bool passed = false;
@@ -512,10 +583,11 @@ __device__ __forceinline__ void follow_maximum(State<D, NT>& st, const float (&s
 
 // Probabilities and the second product. `clear`: V's infinities and NaN are left out (see
 // add_unbounded); returns whether there were any.
-template <int D, bool F8, int NT>
-__device__ __forceinline__ bool second_product(State<D, NT>& st, const float (&sc)[NT][8],
-                                               VRegs<D, F8>& v, float scale_log2, bool clear) {
-    const bool found = clear && clear_unbounded<D, F8>(v);
+template <int D, bool F8, int NT, bool Tr>
+__device__ __forceinline__ bool second_product(State<D, NT, Tr>& st, const float (&sc)[NT][8],
+                                               VRegs<D, F8, Tr>& v, float scale_log2,
+                                               bool clear) {
+    const bool found = clear && clear_unbounded(v);
     bf16x8 pop[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -545,9 +617,13 @@ __device__ __forceinline__ bool second_product(State<D, NT>& st, const float (&s
     for (int n = 0; n < Shape<D>::kNV; ++n) {
         u32x4 vw;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-            vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1), v_word<D, F8>(v, 2 * x + 1, n >> 1),
-                                n & 1);
+        for (int x = 0; x < 4; ++x) {
+            if constexpr (Tr)
+                vw[x] = v.v[n][x];
+            else
+                vw[x] = pick_halves(v_word<D, F8>(v, 2 * x, n >> 1),
+                                    v_word<D, F8>(v, 2 * x + 1, n >> 1), n & 1);
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
             st.acc[t][n] = mfma16x16x32(__builtin_bit_cast(bf16x8, vw), pop[t], st.acc[t][n]);
@@ -586,10 +662,10 @@ __device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
         first_product<D, F8, NT>(sc, q, k);
         if constexpr (More) load_k(k, cache, after, h, lane);
         const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
-        follow_maximum<D, NT>(st, sc, scale_log2);
+        follow_maximum(st, sc, scale_log2);
         // (a chunk that is off was read from the pool's first block, whatever that holds)
         const bool found =
-            second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !cur.any());
+            second_product(st, sc, v, scale_log2, hidden || cur.on == 0);
         left_out |= found && hidden;
         if constexpr (More) {
             load_v(v, cache, after, h, lane);
@@ -605,7 +681,7 @@ __device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
 // The same through a tile in LDS of the wavefront's own, with few registers: K and V of the next
 // chunk are asked for as soon as this one's have been read from their place.
 template <int D, bool F8, bool Pad, int NT, class Next, class Seen>
-__device__ __forceinline__ bool attend_alone(State<D, NT>& st,
+__device__ __forceinline__ bool attend_alone(State<D, NT, !F8>& st,
                                              const bf16x8 (&q)[NT][Shape<D>::kSteps],
                                              const Cache<D, F8, Pad>& cache,
                                              const Tile<D, F8>& tile, const LdsCopy& copies,
@@ -634,18 +710,18 @@ __device__ __forceinline__ bool attend_alone(State<D, NT>& st,
             first_product<D, F8, NT>(sc, q, k);
         }
         const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
-        follow_maximum<D, NT>(st, sc, scale_log2);
+        follow_maximum(st, sc, scale_log2);
         if (more)
             wait_loads_but<kHalf>();  // V is there
         else
             wait_loads_but<0>();
-        VRegs<D, F8> v;
-        read_v<D, F8>(v, tile, lane);
+        VRegs<D, F8, !F8> v;
+        read_v(v, tile, lane);
         if (more) {
             wait_reads();
             copier.ask_half(after, true);
         }
-        const bool found = second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !cur.any());
+        const bool found = second_product(st, sc, v, scale_log2, hidden || cur.on == 0);
         left_out |= found && hidden;
         cur = after;
     }
@@ -659,7 +735,7 @@ __device__ __forceinline__ bool attend_alone(State<D, NT>& st,
 // steps; a tile is asked for Depth - Group steps before it is read, when all have left the steps
 // that read its place, one a step: requests are under way all the time.
 template <int Of, int Depth, int D, bool F8, bool Pad, int NT, class Next, class Seen>
-__device__ __forceinline__ bool attend_shared(State<D, NT>& st,
+__device__ __forceinline__ bool attend_shared(State<D, NT, !F8>& st,
                                               const bf16x8 (&q)[NT][Shape<D>::kSteps],
                                               const Cache<D, F8, Pad>& cache,
                                               const Tile<D, F8>* ring, const LdsCopy& copies,
@@ -675,7 +751,7 @@ __device__ __forceinline__ bool attend_shared(State<D, NT>& st,
     int asked = 0;    // how many those are
     auto ask = [&](int s) {
         const Pair p = next();
-        on |= (static_cast<uint32_t>(p.on[0]) | static_cast<uint32_t>(p.on[1]) << 1) << (2 * asked);
+        on |= p.on << (2 * asked);
         ++asked;
         copier.ask(s % Depth, p);
     };
@@ -691,7 +767,7 @@ __device__ __forceinline__ bool attend_shared(State<D, NT>& st,
         for (int x = 0; x < Group; ++x) {
             if (s + kAhead + x < steps) ask(s + kAhead + x);
             const int c = first + (s + x) * stride;
-            const Pair pair = next.read(c, (on & 1u) != 0, (on & 2u) != 0);
+            const Pair pair = next.read(c, on & 3u);
             on >>= 2;
             --asked;
             if (!busy || s + x >= steps || c >= last) continue;
@@ -702,12 +778,12 @@ __device__ __forceinline__ bool attend_shared(State<D, NT>& st,
                 read_k<D, F8>(k, tile, lane);
                 first_product<D, F8, NT>(sc, q, k);
             }
-            VRegs<D, F8> v;
-            read_v<D, F8>(v, tile, lane);
+            VRegs<D, F8, !F8> v;
+            read_v(v, tile, lane);
             const bool hidden = mask_scores<NT>(sc, pair, c, lane, seen);
-            follow_maximum<D, NT>(st, sc, scale_log2);
+            follow_maximum(st, sc, scale_log2);
             const bool found =
-                second_product<D, F8, NT>(st, sc, v, scale_log2, hidden || !pair.any());
+                second_product(st, sc, v, scale_log2, hidden || pair.on == 0);
             left_out |= found && hidden;
         }
     }
@@ -717,8 +793,8 @@ __device__ __forceinline__ bool attend_shared(State<D, NT>& st,
 // The infinities and NaN of V that attend left out, added to the rows that see their tokens (a
 // sum with one in it is one, whatever its weight). Rare, and written for few registers: element
 // by element.
-template <int D, bool F8, bool Pad, int NT, class Chunks, class Seen>
-__device__ __forceinline__ void add_unbounded(State<D, NT>& st, const Cache<D, F8, Pad>& cache,
+template <int D, bool F8, bool Pad, int NT, bool Tr, class Chunks, class Seen>
+__device__ __forceinline__ void add_unbounded(State<D, NT, Tr>& st, const Cache<D, F8, Pad>& cache,
                                               int h, int first, int last, int stride, int lane,
                                               Chunks chunk, Seen seen) {
     constexpr int NV = Shape<D>::kNV;
@@ -735,14 +811,14 @@ __device__ __forceinline__ void add_unbounded(State<D, NT>& st, const Cache<D, F
 #pragma unroll 1
         for (int key = 0; key < kChunk; ++key) {
             const int b = key >> 4;
-            if (!p.on[b] || (key & 15) >= p.lim[b]) continue;
+            if (!p.is_on(b) || (key & 15) >= p.lim[b]) continue;
             const int64_t slot = static_cast<int64_t>(p.pb[b]) * kBlock + (key & 15);
             const auto* row = cache.v + (slot * cache.hkv + h) * cache.dims();
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int n = 0; n < NV; ++n) {
-                    const int dim = NV * (4 * (lane >> 4) + r) + n;
+                    const int dim = st.dim(n, r, lane >> 4);
                     uint32_t f = 0;
                     if (!Pad || dim < cache.dr) {
                         if constexpr (F8)
@@ -794,8 +870,8 @@ struct Exchange {
 // Adds up the sums of the `parts` (a power of two) wavefronts that took different chunks of the
 // same rows into those of part 0: in each round the upper half hands its own over. A workgroup's
 // wavefronts are `part * groups + group`; all of them call it.
-template <int D, int NT, int Waves>
-__device__ __forceinline__ void add_parts(Exchange<D, NT, Waves>& x, State<D, NT>& st, int part,
+template <int D, int NT, bool Tr, int Waves>
+__device__ __forceinline__ void add_parts(Exchange<D, NT, Waves>& x, State<D, NT, Tr>& st, int part,
                                           int parts, int group, int groups, int lane) {
     constexpr int NV = Shape<D>::kNV;
     for (int half = parts / 2; half >= 1; half /= 2) {
@@ -832,34 +908,26 @@ __device__ __forceinline__ void add_parts(Exchange<D, NT, Waves>& x, State<D, NT
 }
 
 // Row j of tile t, finished, to `row` (bf16, dr elements).
-template <int D, bool Pad, int NT>
-__device__ __forceinline__ void store_row(const State<D, NT>& st, int t, float l, __bf16* row,
+template <int D, bool Pad, int NT, bool Tr>
+__device__ __forceinline__ void store_row(const State<D, NT, Tr>& st, int t, float l, __bf16* row,
                                           int dr, int lane) {
-    constexpr int NV = Shape<D>::kNV;
     const float inv = inverse_sum(l);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int n = 0; n < NV; n += 4) {
-            const int dim = NV * (4 * (lane >> 4) + r) + n;
-            const u32x2 w = {pack_bf16x2(st.acc[t][n][r] * inv, st.acc[t][n + 1][r] * inv),
-                             pack_bf16x2(st.acc[t][n + 2][r] * inv, st.acc[t][n + 3][r] * inv)};
-            if (!Pad || dim < dr) *reinterpret_cast<u32x2*>(row + dim) = w;
-        }
+    for (int x = 0; x < Shape<D>::kNV; ++x) {
+        const int dim = st.four_dim(x, lane >> 4);
+        const f32x4 f = st.four(t, x) * inv;
+        const u32x2 w = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+        if (!Pad || dim < dr) *reinterpret_cast<u32x2*>(row + dim) = w;
+    }
 }
 
 // The same as it is, to D floats.
-template <int D, int NT>
-__device__ __forceinline__ void store_part(const State<D, NT>& st, int t, float* row, int lane) {
-    constexpr int NV = Shape<D>::kNV;
+template <int D, int NT, bool Tr>
+__device__ __forceinline__ void store_part(const State<D, NT, Tr>& st, int t, float* row,
+                                           int lane) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int n = 0; n < NV; n += 4) {
-            const f32x4 w = {st.acc[t][n][r], st.acc[t][n + 1][r], st.acc[t][n + 2][r],
-                             st.acc[t][n + 3][r]};
-            *reinterpret_cast<f32x4*>(row + NV * (4 * (lane >> 4) + r) + n) = w;
-        }
+    for (int x = 0; x < Shape<D>::kNV; ++x)
+        *reinterpret_cast<f32x4*>(row + st.four_dim(x, lane >> 4)) = st.four(t, x);
 }
 
 // A merge's lane has D / 64 columns of a row next to one another.

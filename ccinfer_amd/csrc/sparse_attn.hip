@@ -92,11 +92,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 3 : 1) void sparse_decode_kern
     const float l = wave_sum_xor16_32(st.l[0]);
     if (row >= heads) return;
     if (a.splits == 1) {
-        store_row<D, Pad, 1>(st, 0, l, a.out + (static_cast<int64_t>(b) * a.hq + head0 + row) * dr,
+        store_row<D, Pad>(st, 0, l, a.out + (static_cast<int64_t>(b) * a.hq + head0 + row) * dr,
                              dr, lane);
     } else {
         const int64_t at = static_cast<int64_t>(blockIdx.x) * kTile + row;
-        store_part<D, 1>(st, 0, a.part_acc + at * D, lane);
+        store_part(st, 0, a.part_acc + at * D, lane);
         if (lane < 16) a.part_ml[at] = float2{st.m[0], l};
     }
 }

@@ -62,6 +62,7 @@ struct TreeArgs {
     __bf16* out;
     int batch, total, mbpr, hq, words;
     float scale_log2;
+    uint32_t by_group;  // 2^32 / (hq / hkv), rounded up: quotients by it are its high products
     int slots;      // of each kv head
     int min_units;  // of a slot
     int row_cap;    // rows of a workspace piece
@@ -103,6 +104,8 @@ __device__ __forceinline__ int row_groups(int rows) {
 // Cost of a chunk for a block. Its bytes take about as long as the products of all wavefronts;
 // fewer rows are bound by the bytes.
 constexpr int kFullUnits = 5;
+// Cost of an item's start and end: rows of q, the first chunks' way, sums joined and stored.
+constexpr int kStartUnits = 32;
 template <int D>
 __device__ __forceinline__ int chunk_units(int rows) {
     return 2 * rows <= kBlockRows<D> ? 4 : kFullUnits;
@@ -115,7 +118,8 @@ __device__ __forceinline__ int request_units(const Request& r, int G) {
     const int rows = r.nodes * G;
     const int full = (rows - 1) / kBlockRows<D>;
     const int chunks = (r.end + kChunk - 1) / kChunk;
-    return chunks * (kFullUnits * full + chunk_units<D>(rows - full * kBlockRows<D>));
+    return full * (kStartUnits + chunks * kFullUnits) + kStartUnits +
+           chunks * chunk_units<D>(rows - full * kBlockRows<D>);
 }
 
 // The blocks of chunks first, first + stride, ... below last of a table row, one chunk after the
@@ -158,21 +162,12 @@ struct BlockIds {
         }
         return p;
     }
-    // Of chunk c, whose blocks are there (on0, on1) or not: what its scores are masked by.
-    __device__ __forceinline__ Pair read(int c_, bool on0, bool on1) const {
+    // Of chunk c, whose blocks `on` are there: what its scores are masked by.
+    __device__ __forceinline__ Pair read(int c_, uint32_t on) const {
         const int left = end - c_ * kChunk;
-        return make_pair(on0 ? 0 : -1, left, on1 ? 0 : -1, left - kBlock);
+        return Pair{{0, 0}, {min(left, kBlock), min(left - kBlock, kBlock)}, on};
     }
 };
-
-// Workgroups go to the eight XCDs in turn. Here those of one XCD take neighbouring places: slots
-// next to one another, whose row blocks read the same chunks, with all heads of each, which lie
-// side by side in memory (an XCD with one head reads 256 bytes of every 2 KB, of which few of its
-// L2's channels hold anything: %TIME%).
-__device__ __forceinline__ int place_on_chip(int i, int n) {
-    const int xcd = i & 7, each = n >> 3, more = n & 7;
-    return xcd * each + min(xcd, more) + (i >> 3);
-}
 
 template <int D, bool F8, bool Pad>
 __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_kernel(
@@ -192,8 +187,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hkv = a.cache.hkv;
     const int G = a.hq / hkv, dr = a.cache.dims();
-    const int at_chip = place_on_chip(blockIdx.x, gridDim.x);
-    const int h = at_chip % hkv, slot = at_chip / hkv;
+    const int h = blockIdx.x % hkv, slot = blockIdx.x / hkv;
     SlotDesc* desc = a.desc + static_cast<int64_t>(h) * a.slots + slot;
 
     // Where each request's units start.
@@ -248,6 +242,10 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
         if (tid == 0) *desc = SlotDesc{0, 0, 0, 0};
         return;
     }
+    // (2^32 / 1 has no place in 32 bits)
+    auto node_of = [&](int r) {
+        return G == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.by_group));
+    };
     SlotDesc own{0, 0, 0, 0};
     int b = first_request;
     for (int u = __builtin_amdgcn_readfirstlane(u0); u < u1;) {
@@ -260,15 +258,17 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
         const int chunks = (req.end + kChunk - 1) / kChunk;
         const int full = (all_rows - 1) / kBlockRows<D>;
         const int local = u - __builtin_amdgcn_readfirstlane(starts[b]);
-        const int rb = min(local / (kFullUnits * chunks), full);
+        const int full_item = kStartUnits + kFullUnits * chunks;
+        const int rb = min(local / full_item, full);
         const int row0 = rb * kBlockRows<D>;
         const int block_rows = min(all_rows - row0, kBlockRows<D>);
         const int weight = chunk_units<D>(block_rows);
-        const int item = chunks * weight;
-        const int from = local - rb * kFullUnits * chunks;
+        const int item = kStartUnits + chunks * weight;
+        const int from = local - rb * full_item;
         const int to = min(item, from + (u1 - u));
         // a chunk belongs to the slot that its first unit lies in
-        const int c0 = (from + weight - 1) / weight, c1 = (to + weight - 1) / weight;
+        const int c0 = (max(from - kStartUnits, 0) + weight - 1) / weight;
+        const int c1 = (max(to - kStartUnits, 0) + weight - 1) / weight;
         const bool whole = from == 0 && to == item;
         const int which = from == 0 ? 1 : 0;  // piece of the slot: begins in it, or before it
         if (from == 0 && to < item)
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
         const int groups = row_groups<R>(block_rows);
         const int share = W / groups;
         const int group = wave % groups, part = wave / groups;
-        State<D, NT> st;
+        State<D, NT, !F8> st;
         st.clear();
         const bool busy = group * R < block_rows;
         bf16x8 q[NT][Shape<D>::kSteps];
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
             const int row = group * R + 16 * t + (lane & 15);
             const bool live = row < block_rows;
             const int r = row0 + (live ? row : 0);
-            const int node = r / G;
+            const int node = node_of(r);
             const int64_t token = req.first + node;
             load_q<D, F8, Pad>(q[t], a.q + (token * a.hq + h * G + (r - node * G)) * dr, live, dr,
                                lane);
@@ -355,12 +355,12 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
                 if (row >= block_rows) continue;
                 if (whole) {
                     const int r = row0 + row;
-                    const int node = r / G;
+                    const int node = node_of(r);
                     const int64_t token = req.first + node;
-                    store_row<D, Pad, NT>(
+                    store_row<D, Pad>(
                         st, t, l, a.out + (token * a.hq + h * G + (r - node * G)) * dr, dr, lane);
                 } else {
-                    store_part<D, NT>(st, t, pa + static_cast<int64_t>(row) * D, lane);
+                    store_part(st, t, pa + static_cast<int64_t>(row) * D, lane);
                     if (lane < 16) pm[row] = float2{st.m[t], l};
                 }
             }
@@ -460,6 +460,8 @@ hipError_t launch(const TreeAttention& t, void* workspace, hipStream_t stream) {
     a.hq = t.hq;
     a.words = t.words;
     a.scale_log2 = kLog2e / sqrtf(static_cast<float>(t.head_dim));
+    const uint64_t group = static_cast<uint64_t>(t.hq / t.hkv);
+    a.by_group = static_cast<uint32_t>(((uint64_t{1} << 32) + group - 1) / group);
     a.slots = slots_of(t.hkv);
     a.min_units = kMinUnits;
     a.row_cap = row_cap_of(t.total, t.hq, t.hkv, D);
@@ -482,10 +484,15 @@ bool tree_attention_supported(int batch, int total, int mbpr, int hq, int hkv, i
                               bool fp8) {
     if (batch > kTreeMaxBatch || head_dim > 256 || head_dim % 8 != 0) return false;
     if (fp8 && head_dim != 64 && head_dim != 128) return false;
-    // units: at most kFullUnits a chunk and row block
+    // units: at most kFullUnits a chunk and row block, and its start
     const int64_t block = head_dim <= 128 ? kBlockRows<128> : kBlockRows<256>;
     const int64_t blocks = static_cast<int64_t>(total) * (hq / hkv) / block + batch;
-    const int64_t units = kFullUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
+    const int64_t units = kStartUnits + kFullUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
+    // by_group: rows times the group below 2^32
+    const int64_t group = hq / hkv;
+    if (static_cast<int64_t>(total) * group >= (int64_t{1} << 32) / group) return false;
+    // a token's heads in bytes: products of 24 bits
+    if (static_cast<int64_t>(hkv) * head_dim * (fp8 ? 1 : 2) > rows::kMaxTokenBytes) return false;
     // below 2^28 row blocks the product keeps 64 bits; a request's and all requests' units, and
     // the ends of the slots, keep 32
     return blocks < (int64_t{1} << 28) && units * blocks < kMaxUnits &&
