@@ -930,6 +930,51 @@ __device__ __forceinline__ void store_part(const State<D, NT, Tr>& st, int t, fl
         *reinterpret_cast<f32x4*>(row + st.four_dim(x, lane >> 4)) = st.four(t, x);
 }
 
+// Pieces 0 .. n - 1 of a row, piece s in row at(s) of the parts, added up: a lane has D / 64
+// columns next to one another in x; returns the sum. Eight pieces are under way at once while there
+// are that many (one after the other waits for memory at each: %MERGE%).
+template <int D, class At>
+__device__ __forceinline__ float merge_row(float (&x)[D / 64], int n, const float* part_acc,
+                                           const float2* part_ml, int lane, At at) {
+    constexpr int P = D / 64;
+    float m = kNegInf, l = 0.f;
+#pragma unroll
+    for (int y = 0; y < P; ++y) x[y] = 0.f;
+    auto add = [&](int s0, auto count) {
+        constexpr int N = decltype(count)::value;
+        float2 ml[N];
+        float a[N][P];
+        float top = m;
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+            const int64_t row = at(s0 + z);
+            ml[z] = part_ml[row];
+#pragma unroll
+            for (int y = 0; y < P; ++y) a[z][y] = part_acc[row * D + lane * P + y];
+        }
+#pragma unroll
+        for (int z = 0; z < N; ++z) top = fmaxf(top, ml[z].x);
+        const float use = top == kNegInf ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - use);
+        l *= f;
+#pragma unroll
+        for (int y = 0; y < P; ++y) x[y] *= f;
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+            const float w = __builtin_amdgcn_exp2f(ml[z].x - use);
+            l += ml[z].y * w;
+#pragma unroll
+            for (int y = 0; y < P; ++y) x[y] += a[z][y] * w;
+        }
+        m = top;
+    };
+    int s = 0;
+    for (; s + 8 <= n; s += 8) add(s, std::integral_constant<int, 8>{});
+    for (; s + 2 <= n; s += 2) add(s, std::integral_constant<int, 2>{});
+    if (s < n) add(s, std::integral_constant<int, 1>{});
+    return l;
+}
+
 // A merge's lane has D / 64 columns of a row next to one another.
 template <int D>
 __device__ __forceinline__ void store_columns(__bf16* out, const float (&x)[D / 64], float inv,

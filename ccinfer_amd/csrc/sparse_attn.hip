@@ -107,7 +107,6 @@ __global__ __launch_bounds__(kThreads) void sparse_merge_kernel(const float* par
                                                                 const float2* part_ml, __bf16* out,
                                                                 int64_t rows, int hq, int hkv,
                                                                 int splits, int tiles, int dr) {
-    constexpr int P = D / 64;
     const int lane = threadIdx.x & 63;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves +
                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -117,21 +116,10 @@ __global__ __launch_bounds__(kThreads) void sparse_merge_kernel(const float* par
     const int G = hq / hkv;
     const int h = head / G, g = head - h * G;
     const int64_t item = (b * hkv + h) * tiles + g / kTile;
-    float m = kNegInf, l = 0.f, x[P];
-#pragma unroll
-    for (int y = 0; y < P; ++y) x[y] = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const int64_t at = (item * splits + s) * kTile + g % kTile;
-        const float2 ml = part_ml[at];
-        const float top = fmaxf(m, ml.x);
-        const float use = top == kNegInf ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f(m - use);
-        const float fs = __builtin_amdgcn_exp2f(ml.x - use);
-        l = l * f + ml.y * fs;
-#pragma unroll
-        for (int y = 0; y < P; ++y) x[y] = x[y] * f + part_acc[at * D + lane * P + y] * fs;
-        m = top;
-    }
+    float x[D / 64];
+    const float l = merge_row<D>(x, splits, part_acc, part_ml, lane, [&](int s) {
+        return (item * splits + s) * kTile + g % kTile;
+    });
     store_columns<D>(out + row * dr, x, inverse_sum(l), dr, lane);
 }
 
