@@ -317,6 +317,8 @@ bool drafts_ok(int batch_size, int total_tokens, int max_blocks_per_req, int cac
 bool heads_ok(int rows, int num_q_heads, int num_kv_heads, int head_dim) {
     return num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 &&
            head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256 &&
+           // of one token's heads, K or V: 24-bit products of rows and bytes
+           static_cast<int64_t>(num_kv_heads) * head_dim * 2 <= kMaxTokenBytes &&
            fits_int(static_cast<int64_t>(rows) * num_q_heads);
 }
 

@@ -26,7 +26,6 @@ namespace ccinfer::hipk::rows {
 
 constexpr int kBlock = 16;
 constexpr int kChunk = 32;
-constexpr int64_t kMaxTokenBytes = (1 << 24) - 1;  // of one token's heads, K or V
 
 template <int D>
 struct Shape {
@@ -134,7 +133,7 @@ __device__ __forceinline__ int q_dim(int kk, int g) {
 }
 
 // A block's first row of head h, wave-uniform: loads take it from scalar registers and an offset
-// in bytes a lane (rows are less than 2^24 bytes apart: kMaxTokenBytes).
+// in bytes a lane (rows are less than 2^24 bytes apart: the entries see to it).
 template <class Elem, class C>
 __device__ __forceinline__ const char* block_rows(const Elem* base, const C& c, int pb, int h) {
     return reinterpret_cast<const char*>(

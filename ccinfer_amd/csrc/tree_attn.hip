@@ -480,11 +480,9 @@ bool tree_attention_supported(int batch, int total, int mbpr, int hq, int hkv, i
     const int64_t block = head_dim <= 128 ? kBlockRows<128> : kBlockRows<256>;
     const int64_t blocks = static_cast<int64_t>(total) * (hq / hkv) / block + batch;
     const int64_t units = kStartUnits + kFullUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
-    // by_group: rows times the group below 2^32
+    // by_group gives the quotients of rows whose product with the group is below 2^32
     const int64_t group = hq / hkv;
     if (static_cast<int64_t>(total) * group >= (int64_t{1} << 32) / group) return false;
-    // a token's heads in bytes: products of 24 bits
-    if (static_cast<int64_t>(hkv) * head_dim * (fp8 ? 1 : 2) > rows::kMaxTokenBytes) return false;
     // below 2^28 row blocks the product keeps 64 bits; a request's and all requests' units, and
     // the ends of the slots, keep 32
     return blocks < (int64_t{1} << 28) && units * blocks < kMaxUnits &&

@@ -116,7 +116,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """prefill_attention of a request's new tokens with a mask among them in place of their order:
     each sees the committed context and the new tokens that its row of tree_mask names (written to
     the cache before the call, as in prefill). bf16 cache, or an fp8 one with k_scale and v_scale
-    (head dims 64 and 128); returns output.
+    (head dims 64 and 128); at most 1024 requests; returns output.
 
     Rows that see nothing become zeros. Rows of no request, and of requests with fewer context
     tokens than nodes, keep the contents of `output` (uninitialised when `output` is None). K and V

@@ -458,8 +458,8 @@ int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_cou
  * [b + 1] - query_start_loc[b] nodes; context_lens[b] counts them, as prefill does its new tokens:
  * node i lies at position context_lens[b] - n + i of the cache, whatever its depth in the tree.
  * parents[t] is the request's node from which node t goes on (lower than its own number), -1 for
- * one that goes on from the committed context. At most 2048 requests a call and 2048 nodes a
- * request. The reference decodes one token a request and step (src/backend/params.h:148-211). */
+ * one that goes on from the committed context. At most 2048 requests a call (1024 of the attention)
+ * and 2048 nodes a request. The reference decodes one token a request and step (src/backend/params.h:148-211). */
 
 /* From parents [total_tokens]: tree_mask [total_tokens][mask_words] (bit j of a row, bit j % 32 of
  * word j / 32: the node sees the request's node j; its ancestors and itself), positions
@@ -489,9 +489,9 @@ size_t ccinfer_tree_attention_workspace_size(int batch_size, int total_query_tok
  * context is shorter than their nodes, are left as they are. A node's K and V that a row does not
  * see do not reach it, infinities and NaN included. k_scale / v_scale NULL: a bf16 cache, head_dim
  * a multiple of 8 up to 256; else an fp8 cache (ccinfer_write_kv_cache_fp8), head_dim 64 or 128;
- * CCINFER_ERR_UNSUPPORTED for others, for more than 2048 requests or 64 mask words, and for batches
+ * CCINFER_ERR_UNSUPPORTED for others, for more than 1024 requests or 64 mask words, and for batches
  * whose rows and tables together pass 2^30 units of work. q, caches, scales and output 16-byte
- * aligned. The workspace needs no initialisation. */
+ * aligned; num_kv_heads * head_dim below 2^23. The workspace needs no initialisation. */
 int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cache,
                            const float* k_scale, const float* v_scale, const int32_t* block_table,
                            const int32_t* query_start_loc, const int32_t* context_lens,
@@ -532,9 +532,10 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
 /* The bounds of the blocks that hold the newest tokens of each row, query_start_loc[b + 1] -
  * query_start_loc[b] of them (query_start_loc NULL: one; no fewer than were written or moved since
  * the last call), over all their positions below context_lens[b]. A key that is NaN makes both
- * bounds of its element NaN. With k_scale: an fp8 cache; bounds are rounded to bf16 where a scale is no power of two. Blocks that
- * are shared by rows are whole (other sharings: the last one written stays). At most 2048 rows
- * (CCINFER_ERR_UNSUPPORTED). head_dim a multiple of 8 up to 256. */
+ * bounds of its element NaN. With k_scale: an fp8 cache; bounds are rounded to bf16 where a scale
+ * is no power of two. Blocks that are shared by rows are whole (other sharings: the last one
+ * written stays). At most 2048 rows (CCINFER_ERR_UNSUPPORTED). head_dim a multiple of 8 up to 256,
+ * num_kv_heads * head_dim below 2^23. */
 int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* key_bounds,
                               const int32_t* block_table, const int32_t* context_lens,
                               const int32_t* query_start_loc, int batch_size,
@@ -543,7 +544,8 @@ int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* k
 
 /* scores [batch_size][num_kv_heads][max_blocks_per_req] float: for block j of the row the largest,
  * over the query heads of the kv head, of sum_d max(q_d lo_d, q_d hi_d) / sqrt(head_dim): no key
- * of the block gives a larger logit. -infinity past the context, for negative table entries, and
+ * of the block gives a larger logit (but for float32's rounding, and that of the bounds of an fp8
+ * cache). -infinity past the context, for negative table entries, and
  * for rows whose context the table does not hold; NaN where a bound or q is NaN, NaN or an
  * infinity where a bound is infinite. */
 int ccinfer_score_kv_blocks(const void* q, const void* key_bounds, const int32_t* block_table,

@@ -56,6 +56,10 @@ def test_tree_attention_refusals(lib):
     refused(f, ok, 17, [8, 32])
     refused(f, ok, 18, [None, FAKE + 4])
     refused(f, ok, 19, [need - 1])
+    refused(f, ok, 10, [1025], UNSUPPORTED)
+    wide = list(ok)
+    wide[14] = wide[15] = 1 << 16                # heads of a token: 2^24 bytes
+    assert f(*wide) == INVALID
     for i in (0, 1, 2, 9):
         refused(f, ok, i, [FAKE + 8])
     refused(f, ok, 3, [FAKE])                    # one scale alone
