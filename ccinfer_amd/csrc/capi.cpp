@@ -327,6 +327,7 @@ bool blocks_ok(int batch_size, int max_blocks_per_req, int num_q_heads, int num_
                int head_dim, int cache_block_size) {
     return batch_size > 0 && drafts_ok(batch_size, 1, max_blocks_per_req, cache_block_size) &&
            heads_ok(batch_size, num_q_heads, num_kv_heads, head_dim) &&
+           fits_int(static_cast<int64_t>(batch_size) * max_blocks_per_req) &&
            fits_int(static_cast<int64_t>(batch_size) * num_kv_heads *
                     ((max_blocks_per_req + int64_t{255}) / 256));
 }

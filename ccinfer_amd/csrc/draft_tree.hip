@@ -28,7 +28,7 @@ __global__ __launch_bounds__(kThreads) void draft_tree_kernel(
     const int first = qsl[b], n = qsl[b + 1] - first, c = ctx[b];
     const int before = c - n;
     const bool range_ok = first >= 0 && n >= 0 && first <= total - n;
-    const bool ok = range_ok && before >= 0 && n <= max_nodes;
+    const bool ok = range_ok && c >= n && n <= max_nodes;  // (before may have passed 32 bits)
     if (!ok) {
         // rows that are there get no mask, position or slot
         const int from = max(first, 0);
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(AcceptDrafts a, KvLaye
     const int first = a.qsl[b], n = a.qsl[b + 1] - first, c = a.ctx[b];
     const int before = c - n;
     const bool range_ok = first >= 0 && n >= 0 && first <= a.total - n;
-    if (!range_ok || before < 0 || n <= 0 || n > kTreeMaxNodes) {
+    if (!range_ok || c < n || n <= 0 || n > kTreeMaxNodes) {
         if (part == 0) {
             const int from = max(first, 0);
             const int to = static_cast<int>(

@@ -266,6 +266,8 @@ __global__ __launch_bounds__(kThreads) void score_kernel(
             w[s] = load16(qrow + (dim < head_dim ? dim : 0));
             if (dim >= head_dim) w[s] = u32x4{0u, 0u, 0u, 0u};
         }
+        // the waits below count the copies as the newest loads
+        __builtin_amdgcn_sched_barrier(0);
         ask(0);
         if (there > 1) ask(1);
         bf16x8 qp[S], qn[S];

@@ -90,7 +90,8 @@ __device__ __forceinline__ Request request_of(int from, int to, int c, int total
     r.before = c - r.n;
     r.nodes = min(to, total) - r.first;
     r.end = min(c, mbpr * kBlock);
-    if (r.first < 0 || r.n <= 0 || r.before < 0 || r.nodes < 0) r.nodes = 0;
+    // (c, not `before`, which a broken context may have taken past 32 bits)
+    if (r.first < 0 || r.n <= 0 || c < r.n || r.nodes < 0) r.nodes = 0;
     return r;
 }
 
@@ -328,18 +329,18 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
                                     LdsCopy(lds_copy, shared.tiles + wave), h, c0 + part, c1,
                                     share, a.scale_log2, lane, ids, seen);
         else if (groups == 2)
-            left_out = attend_shared<2, 2>(st, q, a.cache, shared.tiles + 2 * part, LdsCopy(lds_copy, shared.tiles + 2 * part),
-                                           group, h,
-                                           c0 + part, c1, share, steps, busy, a.scale_log2, lane,
-                                           ids, seen);
+            left_out = attend_shared<2, 2>(
+                st, q, a.cache, shared.tiles + 2 * part,
+                LdsCopy(lds_copy, shared.tiles + 2 * part), group, h, c0 + part, c1, share, steps,
+                busy, a.scale_log2, lane, ids, seen);
         else if (groups == 4)
-            left_out = attend_shared<4, 4>(st, q, a.cache, shared.tiles + 4 * part, LdsCopy(lds_copy, shared.tiles + 4 * part),
-                                           group, h,
-                                           c0 + part, c1, share, steps, busy, a.scale_log2, lane,
-                                           ids, seen);
+            left_out = attend_shared<4, 4>(
+                st, q, a.cache, shared.tiles + 4 * part,
+                LdsCopy(lds_copy, shared.tiles + 4 * part), group, h, c0 + part, c1, share, steps,
+                busy, a.scale_log2, lane, ids, seen);
         else if constexpr (W == 8)
-            left_out = attend_shared<8, 8>(st, q, a.cache, shared.tiles, LdsCopy(lds_copy, shared.tiles),
-                                           group, h, c0, c1, 1,
+            left_out = attend_shared<8, 8>(st, q, a.cache, shared.tiles,
+                                           LdsCopy(lds_copy, shared.tiles), group, h, c0, c1, 1,
                                            steps, busy, a.scale_log2, lane, ids, seen);
         else
             left_out = false;

@@ -122,6 +122,9 @@ def test_bounds_scores_select_refusals(lib):
     refused(f, ok, 0, [FAKE + 8])
     refused(f, ok, 2, [FAKE + 8])
     refused(f, ok, 6, [2049], UNSUPPORTED)
+    long = list(ok)
+    long[6], long[7] = 2048, 1 << 20             # entries of the table: 2^31
+    assert f(*long) == INVALID
     fp8 = list(ok)
     fp8[1] = FAKE
     refused(f, fp8, 0, [FAKE + 4])

@@ -249,3 +249,29 @@ def test_the_largest_tree(gpu, nodes, before):
         assert np.array_equal(host(said["accepted"]), counts)
         assert np.array_equal(host(said["accepted_nodes"]), taken)
         assert np.array_equal(host(said["context_lens"]), lengths)
+
+
+def test_contexts_far_below_zero(gpu):
+    """A context whose difference with the nodes passes 32 bits is one of fewer tokens than nodes."""
+    say("drafted trees with contexts of -2^31")
+    low = -2 ** 31
+    ctx, qsl = i32([low, 20, low + 1], gpu), i32([0, 3, 5, 8], gpu)
+    table = i32([[0, 1], [2, 3], [4, 5]], gpu)
+    parents = i32([-1, 0, 1, -1, 0, -1, 0, 0], gpu)
+    plan = cc.build_draft_tree(parents, qsl, ctx, table, 4)
+    assert host(plan["status"]).tolist() == [6, 0, 6]
+    assert host(plan["slot_mapping"]).tolist() == [-1] * 3 + [34 + 16, 35 + 16] + [-1] * 3
+    k, v = torch.randn(2, 96, 1, 64, device=gpu).bfloat16()
+    q = torch.randn(8, 2, 64, device=gpu).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cc.tree_attention(q, k, v, table, qsl, ctx, plan["tree_mask"], output=out)
+    assert bool((out[:3] == 7).all()) and bool((out[5:] == 7).all())
+    assert bool((out[3:5] != 7).any())
+    bounds = torch.full((6, 1, 2, 64), 5.0, dtype=torch.bfloat16, device=gpu)
+    cc.update_key_bounds(k, bounds, table, ctx, qsl)
+    assert bool((bounds[[0, 1, 2, 4, 5]] == 5).all()) and bool((bounds[3] != 5).any())
+    keep = k.clone()
+    said = cc.accept_draft_tokens(parents, parents, parents, qsl, ctx, table, k, v)
+    assert host(said["accepted"]).tolist()[::2] == [0, 0]
+    assert host(said["context_lens"]).tolist()[::2] == [low, low + 1]
+    assert torch.equal(k[:48], keep[:48]) and torch.equal(k[64:], keep[64:])
