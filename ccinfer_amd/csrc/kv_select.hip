@@ -60,7 +60,8 @@ __device__ __forceinline__ Touched touched(const int32_t* ctx, const int32_t* qs
 
 // A thread takes eight dims of one block: 16 loads of 16 (fp8: 8) bytes in flight, whole rows of
 // all heads across the lanes. Tokens that the block does not hold are read as its last one.
-// Bound by the reads: 11 operations an element leave room at HBM's rate.
+// Bound by the reads: 11 operations an element leave room at HBM's rate (16 prompts, 287 MB: 64 us,
+// 4.5 TB/s; 48 rows' newest blocks: 4.6 us).
 template <bool F8>
 __global__ __launch_bounds__(kThreads) void key_bounds_kernel(
     const void* __restrict__ k_cache, const float* __restrict__ k_scale,
@@ -333,7 +334,10 @@ constexpr int kBins = 256;
 // wanted becomes the next range, until a bin fits exactly or holds one value; of that value the
 // lowest blocks are taken. Scores lie close together, so cutting the range that they fill takes
 // two or three rounds and spreads the counters, where their leading bits would meet in a few.
-// A thread holds `Per` blocks that lie next to one another: ranks come from one scan.
+// A thread holds `Per` blocks that lie next to one another: ranks come from one scan. A chain of
+// meetings: 9.0 us for one row of 1251 blocks, 11 for 48 rows of up to 2000 (256 threads of eight
+// blocks: 9.4 and 9.7; 1024 bins: 11.1 and 11.5; scores asked for before the context is there: 8.7
+// and 10.8, but spilled registers in the longest rows).
 template <int Threads, int Per>
 __global__ __launch_bounds__(Threads) void select_kernel(const float* __restrict__ scores,
                                                          const int32_t* __restrict__ ctx,
@@ -499,7 +503,8 @@ hipError_t update_key_bounds(const void* k, const float* k_scale, void* bounds,
 hipError_t score_kv_blocks(const void* q, const void* bounds, const int32_t* table,
                            const int32_t* ctx, float* scores, int batch, int mbpr, int hq, int hkv,
                            int head_dim, hipStream_t stream) {
-    // 64 blocks a wavefront, or 16 where that keeps fewer than two of them a SIMD busy
+    // 64 blocks a wavefront, or 16 where that keeps fewer than two of them a SIMD busy (one row of
+    // 1251 blocks: 6.4 us and 4.2)
     const int64_t waves = (static_cast<int64_t>(mbpr) + 63) / 64 * batch * hkv;
     const int tiles = waves < 2048 ? 1 : 4;
     const int each = kThreads / 4 * tiles;  // blocks of a workgroup

