@@ -111,27 +111,23 @@ __device__ __forceinline__ int row_groups(int rows) {
     return rows <= R ? 1 : (rows <= 2 * R ? 2 : (rows <= 4 * R ? 4 : 8));
 }
 
-// Cost of a chunk for a block. Its bytes take about as long as the products of all wavefronts;
-// fewer rows are bound by the bytes.
-constexpr int kFullUnits = 5;
+// Cost of a chunk, whatever the rows of its block (4 units in place of 5 for up to half the rows:
+// the same to 1 % slower). Several units, so that the ranges are nearly equal: with one, 8 requests
+// of 2048 tokens take 41 us in place of 36.6.
+constexpr int kChunkUnits = 4;
 // Cost of an item's start and end: rows of q, the first chunks' way, sums joined and stored, 20 to
 // 30 thousand cycles (left out, a slot may get many short requests: 248 of 64 tokens with 8 of
-// 8192 take 286 us in place of 156).
+// 8192 take 286 us in place of 154).
 constexpr int kStartUnits = 32;
-template <int D>
-__device__ __forceinline__ int chunk_units(int rows) {
-    return 2 * rows <= kBlockRows<D> ? 4 : kFullUnits;
-}
 
 // Units of a request's row blocks.
 template <int D>
 __device__ __forceinline__ int request_units(const Request& r, int G) {
     if (r.nodes <= 0) return 0;
     const int rows = r.nodes * G;
-    const int full = (rows - 1) / kBlockRows<D>;
+    const int blocks = (rows - 1) / kBlockRows<D> + 1;
     const int chunks = (r.end + kChunk - 1) / kChunk;
-    return full * (kStartUnits + chunks * kFullUnits) + kStartUnits +
-           chunks * chunk_units<D>(rows - full * kBlockRows<D>);
+    return blocks * (kStartUnits + chunks * kChunkUnits);
 }
 
 // The blocks of chunks first, first + stride, ... below last of a table row, one chunk after the
@@ -268,19 +264,16 @@ __global__ __launch_bounds__(kWaves<D> * 64, kWaves<D> / 4) void tree_attention_
                                        __builtin_amdgcn_readfirstlane(ctxs[b]), a.total, a.mbpr);
         const int all_rows = req.nodes * G;
         const int chunks = (req.end + kChunk - 1) / kChunk;
-        const int full = (all_rows - 1) / kBlockRows<D>;
+        const int item = kStartUnits + chunks * kChunkUnits;
         const int local = u - __builtin_amdgcn_readfirstlane(starts[b]);
-        const int full_item = kStartUnits + kFullUnits * chunks;
-        const int rb = min(local / full_item, full);
+        const int rb = local / item;
         const int row0 = rb * kBlockRows<D>;
         const int block_rows = min(all_rows - row0, kBlockRows<D>);
-        const int weight = chunk_units<D>(block_rows);
-        const int item = kStartUnits + chunks * weight;
-        const int from = local - rb * full_item;
+        const int from = local - rb * item;
         const int to = min(item, from + (u1 - u));
         // a chunk belongs to the slot that its first unit lies in
-        const int c0 = (max(from - kStartUnits, 0) + weight - 1) / weight;
-        const int c1 = (max(to - kStartUnits, 0) + weight - 1) / weight;
+        const int c0 = (max(from - kStartUnits, 0) + kChunkUnits - 1) / kChunkUnits;
+        const int c1 = (max(to - kStartUnits, 0) + kChunkUnits - 1) / kChunkUnits;
         const bool whole = from == 0 && to == item;
         const int which = from == 0 ? 1 : 0;  // piece of the slot: begins in it, or before it
         if (from == 0 && to < item)
@@ -412,8 +405,10 @@ __global__ __launch_bounds__(kMergeWaves * 64) void tree_merge_kernel(
 
 // Workgroups that the chip holds at once: one for each of 256 CUs.
 constexpr int kResident = 256;
-// Units of a slot at least: what two to sixteen chunks cost.
-constexpr int kMinUnits = 64;
+// Units of a slot at least: a start and eight chunks, one for each wavefront of a block of few rows
+// (twice as many: 8 requests of 2048 tokens 38.5 us in place of 36.6; half: one of 1000 21.3 in
+// place of 20.4).
+constexpr int kMinUnits = kStartUnits + 8 * kChunkUnits;
 
 int slots_of(int hkv) { return std::max(1, kResident / hkv); }
 
@@ -484,10 +479,10 @@ bool tree_attention_supported(int batch, int total, int mbpr, int hq, int hkv, i
                               bool fp8) {
     if (batch > kTreeMaxBatch || head_dim > 256 || head_dim % 8 != 0) return false;
     if (fp8 && head_dim != 64 && head_dim != 128) return false;
-    // units: at most kFullUnits a chunk and row block, and its start
+    // units: the chunks of a row block, and its start
     const int64_t block = head_dim <= 128 ? kBlockRows<128> : kBlockRows<256>;
     const int64_t blocks = static_cast<int64_t>(total) * (hq / hkv) / block + batch;
-    const int64_t units = kStartUnits + kFullUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
+    const int64_t units = kStartUnits + kChunkUnits * (static_cast<int64_t>(mbpr) / 2 + 1);
     // by_group gives the quotients of rows whose product with the group is below 2^32
     const int64_t group = hq / hkv;
     if (static_cast<int64_t>(total) * group >= (int64_t{1} << 32) / group) return false;
