@@ -1043,6 +1043,11 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
         !fits_int(static_cast<int64_t>(max_blocks_per_req) * cache_block_size))
         return CCINFER_ERR_INVALID_ARGUMENT;
     if (batch_size > kTreeMaxRequests) return CCINFER_ERR_UNSUPPORTED;
+    // the workgroups of a request read the inputs each by itself while one of them writes
+    for (const int32_t* out : {accepted, accepted_nodes, tokens, context_lens_out})
+        for (const int32_t* in : {draft_tokens, target_tokens, parents, query_start_loc,
+                                  context_lens, block_table})
+            if (out == in) return CCINFER_ERR_INVALID_ARGUMENT;
     AcceptDrafts a;
     a.draft = draft_tokens;
     a.target = target_tokens;

@@ -512,7 +512,8 @@ int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cac
  * same arguments for each layer moves them). Blocks that hold nodes belong to one request alone.
  * A row without a block in the pool is not moved. A request without nodes, with more than 2048,
  * with fewer context tokens than nodes or with nodes outside [0, total_tokens): accepted 0, its
- * context as it is. context_lens_out may not be context_lens where the call is made again. */
+ * context as it is. Outputs lie apart from the inputs (CCINFER_ERR_INVALID_ARGUMENT where one is
+ * an input). */
 int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
                                 const int32_t* parents, const int32_t* query_start_loc,
                                 const int32_t* context_lens, const int32_t* block_table,

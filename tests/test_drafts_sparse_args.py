@@ -100,7 +100,11 @@ def test_accept_refusals(lib):
         refused(f, ok, i, [None])
     for i in (6, 7, 8, 13, 16, 17, 18, 19):
         refused(f, ok, i, [0, -1])
+    ok = [FAKE + 64 * i if a == FAKE and i < 6 else a for i, a in enumerate(ok)]
+    ok[20:24] = [FAKE + 64 * i for i in range(20, 24)]
     refused(f, ok, 14, [8 * 16 * 2 * 64 * 2 - 2])  # layers that lie inside one another
+    for i in range(20, 24):
+        refused(f, ok, i, ok[:6])                  # an output that is an input
     refused(f, ok, 11, [FAKE])                     # one scale alone
     refused(f, ok, 6, [2049], UNSUPPORTED)
     bare = list(ok)
