@@ -316,8 +316,8 @@ hipError_t compact_kv_blocks(const int32_t* table, const int32_t* refs, int64_t 
                              hipStream_t stream);
 
 // ---- drafted tokens -------------------------------------------------------------
-// Requests of a call (of an attention call), and nodes (drafted tokens) of a request, at most.
 constexpr int64_t kMaxTokenBytes = (1 << 24) - 1;  // of one token's heads, K or V
+// Requests of a call (of an attention call), and nodes (drafted tokens) of a request, at most.
 constexpr int kTreeMaxRequests = 2048;
 constexpr int kTreeMaxBatch = 1024;
 constexpr int kTreeMaxNodes = 2048;
