@@ -34,8 +34,7 @@ __global__ __launch_bounds__(kThreads) void draft_tree_kernel(
     if (!ok) {
         // rows that are there get no mask, position or slot
         const int from = max(first, 0);
-        const int to = static_cast<int>(
-            min(static_cast<int64_t>(total), static_cast<int64_t>(first) + n));
+        const int to = min(total, qsl[b + 1]);  // (n may have passed 32 bits)
         for (int64_t t = from + threadIdx.x; t < to; t += kThreads) {
             for (int w = 0; w < words; ++w) mask[t * words + w] = 0u;
             positions[t] = -1;
@@ -103,8 +102,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(AcceptDrafts a, KvLaye
     if (!range_ok || c < n || n <= 0 || n > kTreeMaxNodes) {
         if (part == 0) {
             const int from = max(first, 0);
-            const int to = static_cast<int>(
-                min(static_cast<int64_t>(a.total), static_cast<int64_t>(first) + n));
+            const int to = min(a.total, a.qsl[b + 1]);  // (n may have passed 32 bits)
             for (int t = from + static_cast<int>(threadIdx.x); t < to; t += kThreads) {
                 a.nodes[t] = -1;
                 a.tokens[t] = -1;

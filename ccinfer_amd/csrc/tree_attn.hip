@@ -97,8 +97,8 @@ __device__ __forceinline__ Request request_of(int from, int to, int c, int total
     r.before = c - r.n;
     r.nodes = min(to, total) - r.first;
     r.end = min(c, mbpr * kBlock);
-    // (c, not `before`, which a broken context may have taken past 32 bits)
-    if (r.first < 0 || r.n <= 0 || c < r.n || r.nodes < 0) r.nodes = 0;
+    // (the inputs, not their differences, which broken ones may have taken past 32 bits)
+    if (from < 0 || to <= from || c < r.n || r.nodes < 0) r.nodes = 0;
     return r;
 }
 
