@@ -31,15 +31,20 @@ __global__ __launch_bounds__(kThreads) void draft_tree_kernel(
     const int before = c - n;
     const bool range_ok = first >= 0 && n >= 0 && first <= total - n;
     const bool ok = range_ok && c >= n && n <= max_nodes;  // (before may have passed 32 bits)
-    if (!ok) {
-        // rows that are there get no mask, position or slot
-        const int from = max(first, 0);
-        const int to = min(total, qsl[b + 1]);  // (n may have passed 32 bits)
-        for (int64_t t = from + threadIdx.x; t < to; t += kThreads) {
+    // Rows [from, to) that are there get no mask, position or slot.
+    auto leave_out = [&](int from, int to) {
+        for (int64_t t = max(from, 0) + threadIdx.x; t < min(to, total); t += kThreads) {
             for (int w = 0; w < words; ++w) mask[t * words + w] = 0u;
             positions[t] = -1;
             slots[t] = -1;
         }
+    };
+    // Those of no request too: left as they were, a captured step's cache write would go to the
+    // slots of an earlier replay with more nodes.
+    if (range_ok && b == 0) leave_out(0, first);
+    if (range_ok && b == static_cast<int>(gridDim.x) - 1) leave_out(first + n, total);
+    if (!ok) {
+        leave_out(first, qsl[b + 1]);  // (n may have passed 32 bits)
         if (threadIdx.x == 0) status[b] = kInvalid;
         return;
     }

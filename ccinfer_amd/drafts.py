@@ -64,8 +64,8 @@ def build_draft_tree(parents: torch.Tensor, query_start_loc: torch.Tensor,
     [total] (for rotary embeddings: committed tokens + depth), slot_mapping [total] (for the cache
     write) and status [requests]: 0, or 6 for a request with more than max_nodes nodes or fewer
     context tokens than nodes (its rows: no mask, -1, -1), with a parent that is no earlier node
-    (taken as -1) or without a block for a node (slot -1). At most 2048 nodes a request. `out`
-    reuses tensors of an earlier call."""
+    (taken as -1) or without a block for a node (slot -1). Rows of no request (a padded batch): no
+    mask, -1, -1. At most 2048 nodes a request. `out` reuses tensors of an earlier call."""
     op = "build_draft_tree"
     _require(parents.is_cuda, op)
     dev = current_device()

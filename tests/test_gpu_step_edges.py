@@ -80,3 +80,71 @@ def test_rows_whose_difference_passes_32_bits(gpu, qsl, ctx):
     cc.tree_attention(q, k, v, table, dq, dc, mask.view(total, 1), output=out)
     torch.cuda.synchronize()
     assert bool((out == 7).all())
+
+
+# ---- rows of no request --------------------------------------------------------------------
+
+def test_plan_of_a_padded_batch(gpu):
+    """Rows before the first request and behind the last one get no mask, position -1 and slot -1,
+    whatever an earlier call left there."""
+    say("plan of a padded batch")
+    qsl, total = np.array([2, 5, 5, 9]), 300
+    ctx, table = np.array([20, 7, 33]), np.array([[4, 1, -1], [2, -1, -1], [0, 3, 5]])
+    parents = np.zeros(total, np.int32)
+    parents[2:9] = [-1, 0, 0, -1, 0, 1, 2]
+    out = {"tree_mask": torch.full((total, 2), 7, dtype=torch.int32, device=gpu),
+           "positions": torch.full((total,), 7, dtype=torch.int32, device=gpu),
+           "slot_mapping": torch.full((total,), 7, dtype=torch.int32, device=gpu),
+           "status": torch.full((3,), 7, dtype=torch.int32, device=gpu)}
+    cc.build_draft_tree(i32(parents, gpu), i32(qsl, gpu), i32(ctx, gpu), i32(table, gpu), 40,
+                        out=out)
+    got = {n: host(x) for n, x in out.items()}
+    assert got["status"].tolist() == [0, 0, 0]
+    assert got["tree_mask"][2:9].tolist() == [[m, 0] for m in (1, 3, 5, 1, 3, 7, 15)]
+    assert got["positions"][2:9].tolist() == [17, 18, 18, 29, 30, 31, 32]
+    assert got["slot_mapping"][2:9].tolist() == [17, 18, 19, 3 * 16 + 13, 3 * 16 + 14,
+                                                 3 * 16 + 15, 5 * 16]
+    none = np.r_[0:2, 9:total]
+    assert not got["tree_mask"][none].any()
+    assert (got["positions"][none] == -1).all() and (got["slot_mapping"][none] == -1).all()
+
+
+def test_a_replayed_step_of_fewer_nodes_writes_no_old_slots(gpu):
+    """A captured step of up to 12 nodes: replays with fewer leave the slots of earlier replays."""
+    say("captured plan and cache write, fewer nodes in each replay")
+    total, table = 12, i32([[0, 1], [2, 3]], gpu)
+    parents = i32(np.tile([-1, 0, 1, 2, 3, 4], 2), gpu)
+    qsl, ctx = i32([0, 6, 12], gpu), i32([16, 16], gpu)
+    k, v = torch.zeros(2, 64, 1, 64, dtype=torch.bfloat16, device=gpu)
+    new = torch.randn(2, total, 1, 64, device=gpu).bfloat16()
+
+    def step():
+        plan = cc.build_draft_tree(parents, qsl, ctx, table, 6)
+        cc.write_kv_cache(new[0], new[1], k, v, plan["slot_mapping"])
+        return plan
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for nodes, lens in (((6, 6), (16, 16)), ((2, 3), (20, 18)), ((1, 0), (21, 18)),
+                        ((4, 2), (30, 20))):
+        qsl.copy_(i32(np.concatenate([[0], np.cumsum(nodes)]), gpu))
+        ctx.copy_(i32(lens, gpu))
+        new.copy_(torch.randn(new.shape, device=gpu))
+        want = k.clone(), v.clone()
+        at = 0
+        for b in range(2):
+            for i in range(nodes[b]):
+                p = lens[b] - nodes[b] + i
+                for x in range(2):
+                    want[x][(2 * b + p // 16) * 16 + p % 16] = new[x, at]
+                at += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1]), nodes
