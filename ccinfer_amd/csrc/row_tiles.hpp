@@ -487,6 +487,18 @@ __device__ __forceinline__ bool clear_unbounded(VRegs<D, F8, Tr>& r) {
     return found;
 }
 
+// Zeros in place of what this lane's V holds of tokens that are not there: copies of ones that are,
+// of whose infinities a probability of 0 would make NaN.
+template <int D, bool F8>
+__device__ __forceinline__ void clear_absent(VRegs<D, F8>& r, const Pair& p, int lane) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // token T(g, e)
+        const bool there = p.is_on(e >> 2) && 4 * (lane >> 4) + (e & 3) < p.lim[e >> 2];
+#pragma unroll
+        for (auto& w : r.v[e]) w = there ? w : 0u;
+    }
+}
+
 // Products of q with K: sc[t][e] of row j and token T(g, e), times the token's scale in an fp8
 // cache; the logits' factor follows in the exponent.
 template <int D, bool F8, int NT>
@@ -526,7 +538,7 @@ __device__ __forceinline__ void first_product(float (&sc)[NT][8],
 
 // Masks the scores of a chunk that some row does not see whole. seen(c, t, bits): false where
 // every row of tile t sees all that is there of the chunk, else bits has a bit for each of its 32
-// tokens that this lane's row sees. Returns whether `seen` hid any (wave-uniform).
+// tokens that this lane's row sees. Returns whether it masked any (wave-uniform).
 template <int NT, class Seen>
 __device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, int c, int lane,
                                             Seen seen) {
@@ -537,7 +549,8 @@ __device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, i
         bits[t] = 0xffffffffu;
         hidden |= seen(c, t, bits[t]);
     }
-    if (hidden || !p.whole()) {
+    const bool part = hidden || !p.whole();
+    if (part) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -548,7 +561,7 @@ __device__ __forceinline__ bool mask_scores(float (&sc)[NT][8], const Pair& p, i
                 sc[t][e] = ok ? sc[t][e] : kNegInf;
             }
     }
-    return hidden;
+    return part;
 }
 
 // The reference that the exponents are taken from follows the maximum only when a score passes it
@@ -632,17 +645,13 @@ __device__ __forceinline__ bool second_product(State<D, NT, Tr>& st, const float
 
 // Chunks first, first + stride, ... below last of the rows of one wavefront. next(): their Pairs,
 // one after the other (the last one again behind it), from ids that lie in the wavefront's lanes:
-// a scalar load a chunk would make every wait for LDS wait for it too. Chunks that `seen` hides a
-// part of (mask_scores) are multiplied without the infinities and NaN of V, which would reach rows
-// that do not see their token (0 x inf); true if there were any: add_unbounded then brings them
-// to the rows that do.
-template <int D, bool F8, bool Pad, int NT, class Next, class Seen>
-__device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
+// a scalar load a chunk would make every wait for LDS wait for it too. Every row sees all tokens
+// that are there.
+template <int D, bool F8, bool Pad, int NT, class Next>
+__device__ __forceinline__ void attend(State<D, NT>& st, const bf16x8 (&q)[NT][Shape<D>::kSteps],
                                        const Cache<D, F8, Pad>& cache, int h, int first, int last,
-                                       int stride, float scale_log2, int lane, Next& next,
-                                       Seen seen) {
-    if (first >= last) return false;
-    bool left_out = false;
+                                       int stride, float scale_log2, int lane, Next& next) {
+    if (first >= last) return;
     KRegs<D, F8> k;
     VRegs<D, F8> v;
     Pair cur = next();
@@ -660,12 +669,11 @@ __device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
         float sc[NT][8];
         first_product<D, F8, NT>(sc, q, k);
         if constexpr (More) load_k(k, cache, after, h, lane);
-        const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
+        const bool part =
+            mask_scores<NT>(sc, cur, c, lane, [](int, int, uint32_t&) { return false; });
         follow_maximum(st, sc, scale_log2);
-        // (a chunk that is off was read from the pool's first block, whatever that holds)
-        const bool found =
-            second_product(st, sc, v, scale_log2, hidden || cur.on == 0);
-        left_out |= found && hidden;
+        if (part) clear_absent(v, cur, lane);
+        second_product(st, sc, v, scale_log2, false);
         if constexpr (More) {
             load_v(v, cache, after, h, lane);
             cur = after;
@@ -674,11 +682,13 @@ __device__ __forceinline__ bool attend(State<D, NT>& st, const bf16x8 (&q)[NT][S
     };
     while (c + stride < last) step(std::true_type{});
     step(std::false_type{});
-    return left_out;
 }
 
 // The same through a tile in LDS of the wavefront's own, with few registers: K and V of the next
-// chunk are asked for as soon as this one's have been read from their place.
+// chunk are asked for as soon as this one's have been read from their place. Rows see what `seen`
+// says (mask_scores). Chunks of which some row does not see all, or of which not all is there, are
+// multiplied without the infinities and NaN of V, which would reach rows that do not see their token
+// (0 x inf); true if there were any: add_unbounded then brings them to the rows that do.
 template <int D, bool F8, bool Pad, int NT, class Next, class Seen>
 __device__ __forceinline__ bool attend_alone(State<D, NT, !F8>& st,
                                              const bf16x8 (&q)[NT][Shape<D>::kSteps],
@@ -708,7 +718,7 @@ __device__ __forceinline__ bool attend_alone(State<D, NT, !F8>& st,
             }
             first_product<D, F8, NT>(sc, q, k);
         }
-        const bool hidden = mask_scores<NT>(sc, cur, c, lane, seen);
+        const bool part = mask_scores<NT>(sc, cur, c, lane, seen);
         follow_maximum(st, sc, scale_log2);
         if (more)
             wait_loads_but<kHalf>();  // V is there
@@ -720,8 +730,7 @@ __device__ __forceinline__ bool attend_alone(State<D, NT, !F8>& st,
             wait_reads();
             copier.ask_half(after, true);
         }
-        const bool found = second_product(st, sc, v, scale_log2, hidden || cur.on == 0);
-        left_out |= found && hidden;
+        left_out |= second_product(st, sc, v, scale_log2, part);
         cur = after;
     }
     return left_out;
@@ -780,11 +789,9 @@ __device__ __forceinline__ bool attend_shared(State<D, NT, !F8>& st,
             }
             VRegs<D, F8, !F8> v;
             read_v(v, tile, lane);
-            const bool hidden = mask_scores<NT>(sc, pair, c, lane, seen);
+            const bool part = mask_scores<NT>(sc, pair, c, lane, seen);
             follow_maximum(st, sc, scale_log2);
-            const bool found =
-                second_product(st, sc, v, scale_log2, hidden || pair.on == 0);
-            left_out |= found && hidden;
+            left_out |= second_product(st, sc, v, scale_log2, part);
         }
     }
     return left_out;
@@ -803,11 +810,11 @@ __device__ __forceinline__ void add_unbounded(State<D, NT, Tr>& st, const Cache<
         bool some = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            bits[t] = 0;
+            bits[t] = 0xffffffffu;
             some |= seen(c, t, bits[t]);
         }
-        if (!some) continue;
         const Pair p = chunk(c);
+        if (!some && p.whole()) continue;
 #pragma unroll 1
         for (int key = 0; key < kChunk; ++key) {
             const int b = key >> 4;

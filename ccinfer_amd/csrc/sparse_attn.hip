@@ -87,8 +87,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 3 : 1) void sparse_decode_kern
         k = min(k + 2, last_k);
         return p;
     };
-    attend(st, q, a.cache, h, first, chunks, stride, a.scale_log2, lane, next,
-           [](int, int, uint32_t&) { return false; });
+    attend(st, q, a.cache, h, first, chunks, stride, a.scale_log2, lane, next);
     add_parts(sums, st, wave, kWaves, 0, 1, lane);
     if (wave != 0) return;
     const float l = wave_sum_xor16_32(st.l[0]);

@@ -148,3 +148,62 @@ def test_a_replayed_step_of_fewer_nodes_writes_no_old_slots(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(k, want[0]) and torch.equal(v, want[1]), nodes
+
+
+# ---- infinities beside tokens that are not there ---------------------------------------------
+
+def check_unbounded(got, want, tol):
+    """Infinite where the reference is (with its sign), else within its bound."""
+    got = host(got.double())
+    there = np.isfinite(want)
+    assert np.array_equal(got[~there], want[~there])
+    assert np.all(np.abs(got[there] - want[there]) <= tol[there])
+    assert np.any(~there)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (8, 2, 128), (4, 2, 80), (4, 1, 256)])
+def test_sparse_decode_of_an_infinite_value(gpu, hq, hkv, d):
+    """V of one token that a row sees is infinite: the row's result is, in that column alone, also
+    where the token's block is not full or has no other beside it in its list."""
+    say(f"sparse decode, an infinity in V, {hq}/{hkv} x {d}")
+    rng = np.random.default_rng(d)
+    ctx = np.array([37])
+    table, blocks = R.make_tables(rng, ctx, 4)
+    q = torch.randn(1, hq, d).bfloat16()
+    for token, lists in ((36, ([2], [0, 2], [2, -1], [-1, 2], [2, 9], [0, 1, 2], [2, 0])),
+                         (20, ([1], [1, -1], [-1, 1], [0, 2, 1], [1, 7], [3, 1]))):
+        cache = R.Cache(rng, blocks, hkv, d, False, R.held_slots(table, ctx, blocks))
+        slot = int(table[0, token // 16]) * 16 + token % 16
+        cache.t["v"][slot, 0, 3], cache.t["v"][slot, hkv - 1, d - 2] = np.inf, -np.inf
+        cache.t["v64"] = cache.t["v"].double().numpy()
+        t = cache.on(gpu)
+        for chosen in lists:
+            sel = np.broadcast_to(np.array(chosen), (1, hkv, len(chosen)))
+            out = cc.sparse_decode_attention(q.to(gpu), t["k"], t["v"], i32(table, gpu),
+                                             i32(ctx, gpu), i32(sel, gpu))
+            want, tol = R.sparse_decode(q.double().numpy(), cache, table, ctx, sel)
+            check_unbounded(out, want, tol)
+
+
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+@pytest.mark.parametrize("nodes", [3, 14, 30, 60])
+def test_tree_attention_of_an_infinite_value_beside_a_hole(gpu, nodes, d):
+    """The same in the committed context, beside a block that the table does not have: one, two,
+    four and eight wavefronts' rows."""
+    say(f"tree attention of {nodes} nodes, an infinity in V beside a hole, d {d}")
+    rng = np.random.default_rng(nodes + d)
+    hq, hkv, before = 8, 2, 150
+    ctx, qsl = np.array([before + nodes]), np.array([0, nodes])
+    table, blocks = R.make_tables(rng, ctx, 16)
+    table[0, 3] = table[0, 4] = -1
+    cache = R.Cache(rng, blocks, hkv, d, False, R.held_slots(table, ctx, blocks))
+    for token, column in ((2 * 16 + 5, 3), (5 * 16 + 15, d - 1)):
+        cache.t["v"][int(table[0, token // 16]) * 16 + token % 16, :, column] = np.inf
+    cache.t["v64"] = cache.t["v"].double().numpy()
+    t, see = cache.on(gpu), R.visible(R.random_tree(rng, nodes))
+    q = torch.randn(nodes, hq, d).bfloat16()
+    words = -(-nodes // 32)
+    out = cc.tree_attention(q.to(gpu), t["k"], t["v"], i32(table, gpu), i32(qsl, gpu),
+                            i32(ctx, gpu), i32(R.pack_mask(see, words), gpu))
+    want, tol = R.tree_attention(q.double().numpy(), cache, table, qsl, ctx, [see], 0.0)
+    check_unbounded(out, want, tol)
