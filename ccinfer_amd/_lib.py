@@ -91,6 +91,11 @@ SIGNATURES = {
         [_vp] * 6 + [_c_int] * 3 + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
         + [_vp] * 5,
     ),
+    "ccinfer_accept_planned_tokens": (
+        _c_int,
+        [_vp] * 7 + [_c_int] * 3 + [_vp] * 4 + [_c_int] + [_c_i64] * 2 + [_c_int] * 4
+        + [_vp] * 5,
+    ),
     "ccinfer_update_key_bounds": (_c_int, [_vp] * 6 + [_c_int] * 5 + [_vp]),
     "ccinfer_score_kv_blocks": (_c_int, [_vp] * 5 + [_c_int] * 6 + [_vp]),
     "ccinfer_select_kv_blocks": (_c_int, [_vp] * 2 + [_c_int] * 7 + [_vp, _vp]),

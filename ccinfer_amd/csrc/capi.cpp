@@ -1021,15 +1021,16 @@ int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cac
     return map_hip_error(tree_attention(t, workspace, as_stream(stream)));
 }
 
-int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
-                                const int32_t* parents, const int32_t* query_start_loc,
-                                const int32_t* context_lens, const int32_t* block_table,
-                                int batch_size, int total_tokens, int max_blocks_per_req,
-                                void* k_cache, void* v_cache, float* k_scale, float* v_scale,
-                                int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
-                                int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
-                                int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
-                                int32_t* context_lens_out, void* stream) {
+int ccinfer_accept_planned_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
+                                  const int32_t* parents, const int32_t* query_start_loc,
+                                  const int32_t* context_lens, const int32_t* block_table,
+                                  const int32_t* status, int batch_size, int total_tokens,
+                                  int max_blocks_per_req, void* k_cache, void* v_cache,
+                                  float* k_scale, float* v_scale, int num_layers,
+                                  int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                                  int n_kv_heads, int head_dim, int cache_block_size,
+                                  int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
+                                  int32_t* context_lens_out, void* stream) {
     if (!draft_tokens || !target_tokens || !parents || !query_start_loc || !context_lens ||
         !block_table || !accepted || !accepted_nodes || !tokens || !context_lens_out)
         return CCINFER_ERR_INVALID_ARGUMENT;
@@ -1046,7 +1047,7 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
     // the workgroups of a request read the inputs each by itself while one of them writes
     for (const int32_t* out : {accepted, accepted_nodes, tokens, context_lens_out})
         for (const int32_t* in : {draft_tokens, target_tokens, parents, query_start_loc,
-                                  context_lens, block_table})
+                                    context_lens, block_table, status})
             if (out == in) return CCINFER_ERR_INVALID_ARGUMENT;
     AcceptDrafts a;
     a.draft = draft_tokens;
@@ -1055,6 +1056,7 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
     a.qsl = query_start_loc;
     a.ctx = context_lens;
     a.table = block_table;
+    a.status = status;
     a.batch = batch_size;
     a.total = total_tokens;
     a.mbpr = max_blocks_per_req;
@@ -1063,6 +1065,22 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
     a.tokens = tokens;
     a.lengths = context_lens_out;
     return map_hip_error(accept_draft_tokens(a, kv, as_stream(stream)));
+}
+
+int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
+                                const int32_t* parents, const int32_t* query_start_loc,
+                                const int32_t* context_lens, const int32_t* block_table,
+                                int batch_size, int total_tokens, int max_blocks_per_req,
+                                void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                int num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                                int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
+                                int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
+                                int32_t* context_lens_out, void* stream) {
+    return ccinfer_accept_planned_tokens(
+        draft_tokens, target_tokens, parents, query_start_loc, context_lens, block_table, nullptr,
+        batch_size, total_tokens, max_blocks_per_req, k_cache, v_cache, k_scale, v_scale,
+        num_layers, layer_stride, scale_layer_stride, num_blocks, n_kv_heads, head_dim,
+        cache_block_size, accepted, accepted_nodes, tokens, context_lens_out, stream);
 }
 
 int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* key_bounds,

@@ -104,7 +104,9 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(AcceptDrafts a, KvLaye
     const int first = a.qsl[b], n = a.qsl[b + 1] - first, c = a.ctx[b];
     const int before = c - n;
     const bool range_ok = first >= 0 && n >= 0 && first <= a.total - n;
-    if (!range_ok || c < n || n <= 0 || n > kTreeMaxNodes) {
+    // What the plan refused was not written to the cache, or not all of it: nothing of it is taken.
+    const bool planned = a.status == nullptr || a.status[b] == 0;
+    if (!planned || !range_ok || c < n || n <= 0 || n > kTreeMaxNodes) {
         if (part == 0) {
             const int from = max(first, 0);
             const int to = min(a.total, a.qsl[b + 1]);  // (n may have passed 32 bits)
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(AcceptDrafts a, KvLaye
             }
             if (threadIdx.x == 0) {
                 a.accepted[b] = 0;
-                a.lengths[b] = c;
+                a.lengths[b] = !planned && range_ok && c >= n ? before : c;
             }
         }
         return;

@@ -353,6 +353,7 @@ struct AcceptDrafts {
     const int32_t* qsl = nullptr;
     const int32_t* ctx = nullptr;
     const int32_t* table = nullptr;
+    const int32_t* status = nullptr;  // of the plan, or none
     int batch = 0, total = 0, mbpr = 0;
     int32_t* accepted = nullptr;
     int32_t* nodes = nullptr;

@@ -159,7 +159,8 @@ def accept_draft_tokens(draft_tokens: torch.Tensor, target_tokens: torch.Tensor,
                         v_cache: Optional[torch.Tensor] = None,
                         k_scale: Optional[torch.Tensor] = None,
                         v_scale: Optional[torch.Tensor] = None, cache_block_size: int = 16,
-                        out: Optional[dict] = None) -> dict:
+                        out: Optional[dict] = None,
+                        status: Optional[torch.Tensor] = None) -> dict:
     """What the model confirms of the trees. draft_tokens [total]: the nodes' tokens; target_tokens
     [total]: what the model says after each node. A request's path starts at node 0 (the token that
     the last step ended with) and goes on to the lowest child whose drafted token is the target of
@@ -172,7 +173,12 @@ def accept_draft_tokens(draft_tokens: torch.Tensor, target_tokens: torch.Tensor,
     context_lens [requests], the contexts without the rejected nodes: `lengths` of
     update_block_tables, which gives back the blocks that they filled. A request without nodes, or
     with more than 2048, accepts 0. Layers held one by one: the same call for each of them, with
-    the context_lens that counts the nodes. `out` reuses tensors of an earlier call."""
+    the context_lens that counts the nodes. `out` reuses tensors of an earlier call (none of them an
+    input of this one); rows of no request keep what they hold there.
+
+    `status`: the plan's. A request that the plan refused (status not 0) was not written to the cache,
+    or not all of it, and what the model says after its nodes means nothing: it accepts 0, and its
+    context loses the nodes. Without `status` such a request is walked like any other."""
     op = "accept_draft_tokens"
     _require(draft_tokens.is_cuda, op)
     dev = current_device()
@@ -180,7 +186,8 @@ def accept_draft_tokens(draft_tokens: torch.Tensor, target_tokens: torch.Tensor,
     rows, width = _table(block_table, context_lens, dev, op)
     _require(_index(target_tokens, dev, op) == total and _index(parents, dev, op) == total
              and _index(query_start_loc, dev, op) == rows + 1 and total < 2 ** 31
-             and 0 < cache_block_size < 2 ** 31, op)
+             and 0 < cache_block_size < 2 ** 31
+             and (status is None or _index(status, dev, op) == rows), op)
     if k_cache is None:
         _require(v_cache is None and k_scale is None and v_scale is None, op)
         cache = (None, None, None, None, 0, 0, 0, 0, 0, 0, cache_block_size)
@@ -198,11 +205,12 @@ def accept_draft_tokens(draft_tokens: torch.Tensor, target_tokens: torch.Tensor,
              and _index(out["accepted_nodes"], dev, op) == total
              and _index(out["tokens"], dev, op) == total and _index(lengths, dev, op) == rows
              and (rows == 0 or lengths.data_ptr() != context_lens.data_ptr()), op)
-    code = _lib.load().ccinfer_accept_draft_tokens(
+    code = _lib.load().ccinfer_accept_planned_tokens(
         draft_tokens.data_ptr() or None, target_tokens.data_ptr() or None,
         parents.data_ptr() or None, query_start_loc.data_ptr(), context_lens.data_ptr() or None,
-        block_table.data_ptr() or None, rows, total, width, *cache, out["accepted"].data_ptr(),
-        out["accepted_nodes"].data_ptr(), out["tokens"].data_ptr(), lengths.data_ptr(), _stream())
+        block_table.data_ptr() or None, None if status is None else status.data_ptr(), rows, total,
+        width, *cache, out["accepted"].data_ptr(), out["accepted_nodes"].data_ptr(),
+        out["tokens"].data_ptr(), lengths.data_ptr(), _stream())
     if code:
         raise CcinferError(code, op)
     return out

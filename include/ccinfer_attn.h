@@ -513,8 +513,9 @@ int ccinfer_tree_attention(const void* q, const void* k_cache, const void* v_cac
  * same arguments for each layer moves them). Blocks that hold nodes belong to one request alone.
  * A row without a block in the pool is not moved. A request without nodes, with more than 2048,
  * with fewer context tokens than nodes or with nodes outside [0, total_tokens): accepted 0, its
- * context as it is. Outputs lie apart from the inputs (CCINFER_ERR_INVALID_ARGUMENT where one is
- * an input). */
+ * context as it is. Rows of no request keep what accepted_nodes and tokens hold. Outputs lie apart
+ * from the inputs (CCINFER_ERR_INVALID_ARGUMENT where one is an input). The plan's status is not
+ * looked at: see ccinfer_accept_planned_tokens. */
 int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
                                 const int32_t* parents, const int32_t* query_start_loc,
                                 const int32_t* context_lens, const int32_t* block_table,
@@ -524,6 +525,21 @@ int ccinfer_accept_draft_tokens(const int32_t* draft_tokens, const int32_t* targ
                                 int num_blocks, int n_kv_heads, int head_dim, int cache_block_size,
                                 int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
                                 int32_t* context_lens_out, void* stream);
+
+/* ccinfer_accept_draft_tokens after ccinfer_build_draft_tree's status [batch_size] (NULL: none). Nodes
+ * of a request whose status is not CCINFER_OK have no mask, slot or block, or not all of them, so that
+ * what the model says after them means nothing: it accepts 0, nothing of it moves, and its context
+ * loses the nodes (context_lens without them, where it has as many). */
+int ccinfer_accept_planned_tokens(const int32_t* draft_tokens, const int32_t* target_tokens,
+                                  const int32_t* parents, const int32_t* query_start_loc,
+                                  const int32_t* context_lens, const int32_t* block_table,
+                                  const int32_t* status, int batch_size, int total_tokens,
+                                  int max_blocks_per_req, void* k_cache, void* v_cache,
+                                  float* k_scale, float* v_scale, int num_layers,
+                                  int64_t layer_stride, int64_t scale_layer_stride, int num_blocks,
+                                  int n_kv_heads, int head_dim, int cache_block_size,
+                                  int32_t* accepted, int32_t* accepted_nodes, int32_t* tokens,
+                                  int32_t* context_lens_out, void* stream);
 
 /* ---- decode over selected blocks of the context ----------------------------------------
  * Decode that reads the blocks in which a query's weight can lie. Beside each layer's K lie

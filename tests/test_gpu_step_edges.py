@@ -207,3 +207,74 @@ def test_tree_attention_of_an_infinite_value_beside_a_hole(gpu, nodes, d):
                             i32(ctx, gpu), i32(R.pack_mask(see, words), gpu))
     want, tol = R.tree_attention(q.double().numpy(), cache, table, qsl, ctx, [see], 0.0)
     check_unbounded(out, want, tol)
+
+
+# ---- requests that the plan refused ------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_refused_plans_accept_nothing(gpu, fp8):
+    """More nodes than planned for, a parent that is no earlier node, a node without a block, fewer
+    context tokens than nodes: with the plan's status they accept 0, keep their K and V and lose the
+    nodes; the others go on as without it."""
+    say(f"acceptance of refused plans, fp8 {fp8}")
+    nodes, before = [4, 9, 5, 6, 3, 0, 7], np.array([20, 30, 5, 12, 40, 8, 33])
+    trees = [R.random_tree(np.random.default_rng(n), n) for n in nodes]
+    ctx, qsl = before + nodes, np.concatenate([[0], np.cumsum(nodes)])
+    ctx[4] = 2
+    rng = np.random.default_rng(1)
+    table, blocks = R.make_tables(rng, ctx, 4)
+    parents = np.concatenate([np.array(t, np.int32) for t in trees])
+    parents[qsl[2] + 3] = 4
+    table[3, (ctx[3] - 1) // 16] = -1
+    draft, target = np.zeros((2, int(qsl[-1])), np.int32)     # whole chains are confirmed
+    dq, dc, dt = i32(qsl, gpu), i32(ctx, gpu), i32(table, gpu)
+    plan = cc.build_draft_tree(i32(parents, gpu), dq, dc, dt, 8)
+    refused = [False, True, True, True, True, False, False]
+    assert (host(plan["status"]) != 0).tolist() == refused
+    start = R.Cache(rng, blocks, 2, 64, fp8).on(gpu)
+    args = (i32(draft, gpu), i32(target, gpu), i32(parents, gpu), dq, dc, dt)
+    runs = []
+    for status in (None, plan["status"]):
+        t = {n: None if x is None else x.clone() for n, x in start.items()}
+        out = cc.accept_draft_tokens(*args, t["k"], t["v"], k_scale=t["ks"], v_scale=t["vs"],
+                                     status=status)
+        runs.append({n: host(x) for n, x in out.items()})
+    plain, said = runs
+    good = ~np.array(refused)
+    for n in ("accepted", "context_lens"):
+        assert np.array_equal(said[n][good], plain[n][good])
+    assert not said["accepted"][~good].any() and plain["accepted"][1] > 0
+    assert said["context_lens"][~good].tolist() == [30, 5, 12, 2]
+    for b in range(7):
+        rows = slice(qsl[b], qsl[b + 1])
+        for n in ("accepted_nodes", "tokens"):
+            want = np.full(nodes[b], -1) if refused[b] else plain[n][rows]
+            assert np.array_equal(said[n][rows], want), (b, n)
+    # the refused requests' blocks hold what they held
+    for b in np.nonzero(~good)[0]:
+        for block in table[b][table[b] >= 0]:
+            s = slice(block * 16, block * 16 + 16)
+            for n in ("k", "v"):
+                assert torch.equal(t[n][s], start[n][s])
+
+
+def test_a_step_goes_on_after_a_refused_plan(gpu):
+    """Contexts of a refused request cut back by update_block_tables: the next step plans it again."""
+    say("a step after a refused plan")
+    table = torch.full((2, 6), -1, dtype=torch.int32, device=gpu)
+    ctx, refs = torch.zeros(2, dtype=torch.int32, device=gpu), \
+        torch.zeros(16, dtype=torch.int32, device=gpu)
+    rows, none = i32([0, 1], gpu), i32([-1, -1], gpu)
+    assert cc.update_block_tables(table, ctx, refs, rows, none, i32([30, 17], gpu)).item() == 0
+    qsl, parents = i32([0, 6, 9], gpu), i32([-1, 0, 1, 2, 3, 4, -1, 0, 1], gpu)
+    same = torch.zeros(9, dtype=torch.int32, device=gpu)
+    for most, want in ((4, [30, 20]), (8, [36, 23])):
+        before = host(ctx)
+        assert cc.update_block_tables(table, ctx, refs, rows, None,
+                                      i32(before + [6, 3], gpu)).item() == 0
+        plan = cc.build_draft_tree(parents, qsl, ctx, table, most)
+        said = cc.accept_draft_tokens(same, same, parents, qsl, ctx, table, status=plan["status"])
+        assert cc.update_block_tables(table, ctx, refs, rows, None,
+                                      said["context_lens"]).item() == 0
+        assert host(ctx).tolist() == want
+        assert int(refs.sum().item()) == sum(-(-c // 16) for c in want)
