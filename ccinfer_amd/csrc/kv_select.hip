@@ -59,7 +59,9 @@ __device__ __forceinline__ Touched touched(const int32_t* ctx, const int32_t* qs
 }
 
 // A thread takes eight dims of one block: 16 loads of 16 (fp8: 8) bytes in flight, whole rows of
-// all heads across the lanes. Tokens that the block does not hold are read as its last one.
+// all heads across the lanes. Tokens that the block does not hold are read as its last one. Rows
+// that share a block which one of them does not fill (query tokens of one request) all take the
+// tokens of the longest of them, so that it does not matter whose bounds are written last.
 // Bound by the reads: 11 operations an element leave room at HBM's rate (16 prompts, 287 MB: 64 us,
 // 4.5 TB/s; 48 rows' newest blocks: 4.6 us).
 template <bool F8>
@@ -99,8 +101,11 @@ __global__ __launch_bounds__(kThreads) void key_bounds_kernel(
         __syncthreads();
     }
     const int64_t work = static_cast<int64_t>(items) * pieces;
-    for (int64_t x = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; x < work;
-         x += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int lane = threadIdx.x & 63;
+    // whole wavefronts, the threads behind the last piece with it once more
+    for (int64_t x0 = static_cast<int64_t>(blockIdx.x) * kThreads; x0 < work;
+         x0 += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t x = min(x0 + threadIdx.x, work - 1);
         const int item = static_cast<int>(x / pieces);
         const int piece = static_cast<int>(x - static_cast<int64_t>(item) * pieces);
         int b = item;
@@ -114,10 +119,28 @@ __global__ __launch_bounds__(kThreads) void key_bounds_kernel(
         }
         const Touched t = touched(ctx, qsl, b, mbpr);
         const int blk = t.first + (qsl != nullptr ? item - starts[b] : 0);
-        if (blk >= t.last) continue;
-        const int pb = table[static_cast<int64_t>(b) * mbpr + blk];
+        const int pb = blk < t.last ? table[static_cast<int64_t>(b) * mbpr + blk] : -1;
+        int held = min(t.ctx - blk * kBlock, kBlock);
+        // the lanes' unfinished blocks, one after the other: every lane looks at other rows (48
+        // rows 3.6 -> 4.2 us, 1024 5.4 -> 9.0, 2048 9.6 -> 20.8: a line of the table for each pair
+        // of rows; only of longer contexts, asked for once those are there: 4.3, 10.0 and 22.5)
+        uint64_t open = __builtin_amdgcn_ballot_w64(pb >= 0 && held < kBlock);
+        while (open != 0) {
+            const int of = __builtin_ctzll(open);
+            const int pb0 = __builtin_amdgcn_readlane(pb, of);
+            const int blk0 = __builtin_amdgcn_readlane(blk, of);
+            int longest = 0;
+            for (int r = lane; r < batch; r += 64) {
+                const int c = ctx[r];
+                if (table[static_cast<int64_t>(r) * mbpr + blk0] == pb0) longest = max(longest, c);
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) longest = max(longest, __shfl_xor(longest, off));
+            const bool same = pb == pb0 && blk == blk0;
+            if (same) held = min(longest - blk * kBlock, kBlock);
+            open &= ~__builtin_amdgcn_ballot_w64(same);
+        }
         if (pb < 0) continue;
-        const int held = min(t.ctx - blk * kBlock, kBlock);
         const int h = piece / per_head;
         const int dim = (piece - h * per_head) * 8;
         const int64_t row = static_cast<int64_t>(hkv) * head_dim;

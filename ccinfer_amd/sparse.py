@@ -53,7 +53,8 @@ def update_key_bounds(k_cache: torch.Tensor, key_bounds: torch.Tensor, block_tab
     """Renews key_bounds of the blocks that hold each row's newest tokens: one token a row, or
     query_start_loc[b + 1] - query_start_loc[b] (as a prefill or a tree of drafts wrote; after
     accept_draft_tokens the tree's own query_start_loc with the shorter contexts), from all
-    their positions below the context length. A NaN key makes both bounds of its element NaN."""
+    their positions below the context length. Rows may share blocks (a row for each query token of a
+    request): the longest context counts. A NaN key makes both bounds of its element NaN."""
     op = "update_key_bounds"
     _require(k_cache.is_cuda, op)
     dev = current_device()

@@ -551,8 +551,8 @@ int ccinfer_accept_planned_tokens(const int32_t* draft_tokens, const int32_t* ta
  * query_start_loc[b] of them (query_start_loc NULL: one; no fewer than were written or moved since
  * the last call), over all their positions below context_lens[b]. A key that is NaN makes both
  * bounds of its element NaN. With k_scale: an fp8 cache; bounds are rounded to bf16 where a scale
- * is no power of two. Blocks that are shared by rows are whole (other sharings: the last one
- * written stays). At most 2048 rows (CCINFER_ERR_UNSUPPORTED). head_dim a multiple of 8 up to 256,
+ * is no power of two. Of rows that share a block (several query tokens of one request), the longest
+ * context counts. At most 2048 rows (CCINFER_ERR_UNSUPPORTED). head_dim a multiple of 8 up to 256,
  * num_kv_heads * head_dim below 2^23. */
 int ccinfer_update_key_bounds(const void* k_cache, const float* k_scale, void* key_bounds,
                               const int32_t* block_table, const int32_t* context_lens,

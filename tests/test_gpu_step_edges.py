@@ -278,3 +278,90 @@ def test_a_step_goes_on_after_a_refused_plan(gpu):
                                       said["context_lens"]).item() == 0
         assert host(ctx).tolist() == want
         assert int(refs.sum().item()) == sum(-(-c // 16) for c in want)
+
+
+# ---- rows that share a block -------------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hkv,d", [(8, 128), (1, 64), (3, 24), (2, 256)])
+def test_bounds_of_several_rows_of_a_request(gpu, fp8, hkv, d):
+    """A row for each new token, all with the request's table row: the bounds are of the keys below
+    the longest context, in whatever order the rows come."""
+    say(f"bounds of rows that share blocks, {hkv} x {d} fp8 {fp8}")
+    rng = np.random.default_rng(hkv + d)
+    whole = np.array([37, 100, 16, 1, 64, 200])       # contexts after the new tokens
+    tokens = np.array([5, 20, 3, 1, 1, 33])
+    table, blocks = R.make_tables(rng, whole, 14)
+    cache = R.Cache(rng, blocks, hkv, d, fp8, R.held_slots(table, whole, blocks))
+    t = cache.on(gpu)
+    row = np.repeat(np.arange(6), tokens)
+    ctx = np.concatenate([np.arange(c - n + 1, c + 1) for c, n in zip(whole, tokens)])
+    start = torch.randn(blocks, hkv, 2, d).bfloat16()
+    want = R.key_bounds(cache, table, whole, tokens, start.double().numpy())
+    for order in (np.arange(len(row)), np.arange(len(row))[::-1], rng.permutation(len(row))):
+        bounds = start.to(gpu)
+        cc.update_key_bounds(t["k"], bounds, i32(table[row[order]], gpu), i32(ctx[order], gpu),
+                             k_scale=t["ks"])
+        assert np.array_equal(host(bounds.double()), want)
+    # the same as ranges of new tokens: two rows a request, the first without its last tokens
+    both = np.repeat(np.arange(6), 2)
+    short = np.maximum(whole - 3, 0)
+    ctx = np.stack([short, whole], 1).reshape(-1)
+    new = np.stack([np.maximum(tokens - 3, 0), np.minimum(tokens, 3)], 1).reshape(-1)
+    bounds = start.to(gpu)
+    cc.update_key_bounds(t["k"], bounds, i32(table[both], gpu), i32(ctx, gpu),
+                         i32(np.concatenate([[0], np.cumsum(new)]), gpu), k_scale=t["ks"])
+    assert np.array_equal(host(bounds.double()), want)
+
+
+def test_bounds_of_many_rows_that_share_blocks(gpu):
+    """More rows than two wavefronts look at together: 300 requests of 2 to 4 rows."""
+    say("bounds of 900 rows that share blocks")
+    rng = np.random.default_rng(4)
+    tokens, whole = rng.integers(2, 5, 300), rng.integers(4, 70, 300)
+    table, blocks = R.make_tables(rng, whole, 5)
+    cache = R.Cache(rng, blocks, 1, 64, False, R.held_slots(table, whole, blocks))
+    row = rng.permutation(np.repeat(np.arange(300), tokens))
+    seen, ctx = np.zeros(300, int), np.zeros(len(row), int)
+    for x, b in enumerate(row):
+        ctx[x] = whole[b] - seen[b]
+        seen[b] += 1
+    start = torch.zeros(blocks, 1, 2, 64).bfloat16()
+    bounds = start.to(gpu)
+    cc.update_key_bounds(cache.on(gpu)["k"], bounds, i32(table[row], gpu), i32(ctx, gpu))
+    want = R.key_bounds(cache, table, whole, tokens, start.double().numpy())
+    assert np.array_equal(host(bounds.double()), want)
+
+
+def test_a_step_of_several_tokens_a_request(gpu):
+    """The whole chain with a row for each of four new tokens of two requests."""
+    say("selected blocks, four query rows a request")
+    rng = np.random.default_rng(6)
+    hkv, hq, d, m = 2, 8, 128, 4
+    whole = np.array([503, 81])
+    table, blocks = R.make_tables(rng, whole, 34)
+    cache = R.Cache(rng, blocks, hkv, d, False, R.held_slots(table, whole, blocks))
+    t = cache.on(gpu)
+    bounds = torch.full((blocks, hkv, 2, d), float("nan"), dtype=torch.bfloat16, device=gpu)
+    before = whole - m
+    cc.update_key_bounds(t["k"], bounds, i32(table, gpu), i32(before, gpu),
+                         i32(np.concatenate([[0], np.cumsum(before)]), gpu))
+    row = np.repeat(np.arange(2), m)
+    ctx = np.concatenate([np.arange(c - m + 1, c + 1) for c in whole])
+    rows = i32(table[row], gpu), i32(ctx, gpu)
+    cc.update_key_bounds(t["k"], bounds, *rows)
+    q = torch.randn(2 * m, hq, d).bfloat16()
+    sc = cc.score_kv_blocks(q.to(gpu), bounds, *rows)
+    got = host(sc.double())
+    _, tol = R.scores(q.double().numpy(), host(bounds.double()), table[row], ctx)
+    for b in range(2 * m):
+        for p in range(ctx[b]):
+            s = int(table[row[b], p // 16]) * 16 + p % 16
+            for h in range(hkv):
+                top = (q[b, 4 * h:4 * h + 4].double().numpy() @ cache.t["k64"][s, h]).max()
+                assert top / np.sqrt(d) <= got[b, h, p // 16] + tol[b, h, p // 16]
+    chosen = cc.select_kv_blocks(sc, rows[1], 6)
+    assert np.array_equal(host(chosen), R.select(host(sc), ctx, 6, 1, 1))
+    out = cc.sparse_decode_attention(q.to(gpu), t["k"], t["v"], *rows, chosen)
+    want, tol = R.sparse_decode(q.double().numpy(), cache, table[row], ctx, host(chosen))
+    check(out, want, tol)
