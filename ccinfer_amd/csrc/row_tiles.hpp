@@ -402,10 +402,13 @@ __device__ __forceinline__ void wait_loads_but() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Until this wavefront's LDS reads have arrived: what they read may be written again.
+// Until this wavefront's LDS reads have arrived: what they read may be written again. (The copies
+// that write it are hidden from the compiler, see LdsCopy: a read stays before them by the clobber.)
 __device__ __forceinline__ void wait_reads() {
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
 

@@ -365,3 +365,53 @@ def test_a_step_of_several_tokens_a_request(gpu):
     out = cc.sparse_decode_attention(q.to(gpu), t["k"], t["v"], *rows, chosen)
     want, tol = R.sparse_decode(q.double().numpy(), cache, table[row], ctx, host(chosen))
     check(out, want, tol)
+
+
+# ---- scores of large batches -------------------------------------------------------------------
+
+def scores_ref(q, bounds, table, ctx):
+    """_steps_ref.scores, a row and head at a time."""
+    rows, hq, d = q.shape
+    hkv, width = bounds.shape[1], table.shape[1]
+    out, tol = np.full((rows, hkv, width), -np.inf), np.zeros((rows, hkv, width))
+    for b in range(rows):
+        n = -(-int(ctx[b]) // 16) if ctx[b] > 0 else 0
+        if n > width:
+            continue
+        for h in range(hkv):
+            g = q[b].reshape(hkv, -1, 1, d)[h]
+            both = bounds[np.maximum(table[b, :n], 0), h]
+            terms = np.maximum(g * both[:, 0], g * both[:, 1])
+            there = table[b, :n] >= 0
+            out[b, h, :n] = np.where(there, terms.sum(-1).max(0) / np.sqrt(d), -np.inf)
+            tol[b, h, :n] = np.abs(terms).sum(-1).max(0) / np.sqrt(d) * (2 * d + 4) * 2.0 ** -24
+    return out, tol
+
+
+@pytest.mark.parametrize("rows,hq,hkv,d,width", [
+    (64, 16, 8, 128, 270), (64, 16, 8, 64, 270), (64, 8, 8, 256, 270), (64, 16, 8, 120, 270),
+    (64, 16, 8, 80, 257), (205, 40, 2, 64, 270), (256, 17, 1, 128, 500), (300, 34, 2, 40, 255)])
+def test_scores_of_large_batches(gpu, rows, hq, hkv, d, width):
+    """From 2048 wavefronts on each takes up to four tiles of 16 blocks, copied two ahead: contexts
+    that end in each of the tiles, holes, more than 16 query heads a kv head (two rounds)."""
+    say(f"scores of {rows} rows, {hq}/{hkv} x {d}, {width} blocks")
+    assert -(-width // 64) * rows * hkv >= 2048
+    rng = np.random.default_rng(rows + d)
+    n = rng.integers(0, width + 1, rows)
+    n[:12] = [0, 1, 15, 16, 17, 32, 33, 48, 49, 64, 65, width]
+    ctx = np.maximum(n * 16 - rng.integers(0, 16, rows), 0)
+    ctx[12] = width * 16 + 1                       # more than the table holds
+    blocks = 97
+    table = rng.integers(0, blocks, (rows, width))
+    table[rng.random(table.shape) < 0.1] = -1
+    bounds = torch.randn(blocks, hkv, 2, d).bfloat16().sort(dim=2).values.contiguous()
+    q = torch.randn(rows, hq, d).bfloat16()
+    out = torch.full((rows, hkv, width), float("nan"), device=gpu)
+    want, tol = scores_ref(q.double().numpy(), bounds.double().numpy(), table, ctx)
+    for _ in range(3):
+        cc.score_kv_blocks(q.to(gpu), bounds.to(gpu), i32(table, gpu), i32(ctx, gpu), out=out)
+        got = host(out.double())
+        inside = np.isfinite(want)
+        assert np.array_equal(np.isneginf(got), ~inside)
+        assert np.all(np.abs(got[inside] - want[inside]) <= tol[inside])
+        out.fill_(float("nan"))
