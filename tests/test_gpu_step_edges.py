@@ -415,3 +415,77 @@ def test_scores_of_large_batches(gpu, rows, hq, hkv, d, width):
         assert np.array_equal(np.isneginf(got), ~inside)
         assert np.all(np.abs(got[inside] - want[inside]) <= tol[inside])
         out.fill_(float("nan"))
+
+
+# ---- fp8 caches with scales that are no powers of two ------------------------------------------
+
+def odd_scales(cache, rng):
+    """The cache's scales times numbers in [1, 2), float32."""
+    gen = torch.Generator().manual_seed(int(rng.integers(1 << 31)))
+    for n in ("k", "v"):
+        s = cache.t[n + "s"] * (1 + torch.rand(cache.t[n + "s"].shape, generator=gen))
+        cache.t[n + "s"] = s
+        rows = s.view(cache.blocks, cache.hkv, 16).permute(0, 2, 1).reshape(-1, cache.hkv)
+        values = cache.t[n].view(R.E4M3).double()
+        cache.t[n + "64"] = (values * rows.double()[..., None]).numpy()
+    return cache
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_with_any_scales(gpu, d):
+    """Trees and selected blocks. The references' bound holds: a probability times its scale is one
+    more float32 rounding, of the 64 that the bound counts beside the sums."""
+    say(f"fp8 attention with any scales, d {d}")
+    rng = np.random.default_rng(d)
+    nodes, before = [26, 3, 64], np.array([300, 0, 95])
+    trees = [R.random_tree(rng, n) for n in nodes]
+    ctx, qsl = before + nodes, np.concatenate([[0], np.cumsum(nodes)])
+    table, blocks = R.make_tables(rng, ctx, 24)
+    cache = odd_scales(R.Cache(rng, blocks, 2, d, True, R.held_slots(table, ctx, blocks)), rng)
+    t, sees = cache.on(gpu), [R.visible(p) for p in trees]
+    q = torch.randn(int(qsl[-1]), 8, d).bfloat16()
+    mask = np.concatenate([R.pack_mask(s, 2) for s in sees])
+    out = cc.tree_attention(q.to(gpu), t["k"], t["v"], i32(table, gpu), i32(qsl, gpu),
+                            i32(ctx, gpu), i32(mask, gpu), k_scale=t["ks"], v_scale=t["vs"])
+    want, tol = R.tree_attention(q.double().numpy(), cache, table, qsl, ctx, sees, 0.0)
+    check(out, want, tol)
+    for take in (3, 20):
+        sel = np.stack([[rng.permutation(24)[:take] for _ in range(2)] for _ in ctx])
+        out = cc.sparse_decode_attention(q[:3].to(gpu), t["k"], t["v"], i32(table, gpu),
+                                         i32(ctx, gpu), i32(sel, gpu), k_scale=t["ks"],
+                                         v_scale=t["vs"])
+        want, tol = R.sparse_decode(q[:3].double().numpy(), cache, table, ctx, sel)
+        check(out, want, tol)
+
+
+@pytest.mark.parametrize("hkv,d", [(8, 128), (3, 24)])
+def test_bounds_and_scores_with_any_scales(gpu, hkv, d):
+    """A bound is the product in float32 (2^-24 of it) rounded to bf16 (2^-8 of that): no key passes
+    it by more, and no logit its block's score by more than such parts of |q| |bound|."""
+    say(f"fp8 bounds with any scales, {hkv} x {d}")
+    rng = np.random.default_rng(d)
+    ctx = np.array([333, 64, 17])
+    table, blocks = R.make_tables(rng, ctx, 22)
+    cache = odd_scales(R.Cache(rng, blocks, hkv, d, True, R.held_slots(table, ctx, blocks)), rng)
+    t = cache.on(gpu)
+    bounds = torch.zeros(blocks, hkv, 2, d, dtype=torch.bfloat16, device=gpu)
+    dt, dc = i32(table, gpu), i32(ctx, gpu)
+    cc.update_key_bounds(t["k"], bounds, dt, dc, i32(np.cumsum([0, *ctx]), gpu), k_scale=t["ks"])
+    want = R.key_bounds(cache, table, ctx, ctx, np.zeros(bounds.shape))
+    got = host(bounds.double())
+    assert np.all(np.abs(got - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -23))
+    assert not np.array_equal(got, want)               # (some are rounded)
+    q = torch.randn(3, 2 * hkv, d).bfloat16()
+    sc = host(cc.score_kv_blocks(q.to(gpu), bounds, dt, dc).double())
+    exact, tol = R.scores(q.double().numpy(), got, table, ctx)
+    there = np.isfinite(exact)
+    assert np.all(np.abs(sc[there] - exact[there]) <= tol[there])
+    q = q.double().numpy()
+    for b in range(3):
+        for p in range(ctx[b]):
+            s, j = int(table[b, p // 16]) * 16 + p % 16, p // 16
+            for h in range(hkv):
+                g = q[b, 2 * h:2 * h + 2]
+                top = (g @ cache.t["k64"][s, h]).max() / np.sqrt(d)
+                slack = (np.abs(g) @ np.abs(want[table[b, j], h]).max(0)).max() / np.sqrt(d)
+                assert top <= sc[b, h, j] + tol[b, h, j] + slack * (2.0 ** -8 + 2.0 ** -23)
