@@ -34,13 +34,6 @@ struct Shape {
     static constexpr int kVWords = D / 32;  // the same in 32-bit words of bf16
 };
 
-// A pointer to what no kernel writes while this one runs: wave-uniform loads through it go to the
-// scalar unit, whose waits do not wait for the vector loads in flight.
-__device__ __forceinline__ const __attribute__((address_space(4))) int32_t* unwritten(
-    const int32_t* p) {
-    return (const __attribute__((address_space(4))) int32_t*)(reinterpret_cast<uintptr_t>(p));
-}
-
 // One layer's cache of rows of D dims, or, padded, of dr < D, a multiple of 8 (the rest of D counts
 // as zeros).
 template <int D, bool F8, bool Pad>
