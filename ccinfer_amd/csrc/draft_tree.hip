@@ -3,8 +3,10 @@
 //
 // Both are chains of dependent reads over a few integers: latency. A workgroup stages its
 // request's arrays in LDS once, so that every step of a walk is an LDS read. Plan of 26 nodes 2.4 us,
-// of 192 requests of 4 to 64 nodes 4.3; acceptance of one request over 24 layers 5.0, of 96 with
-// 34 MB of K and V to move 18 (1.9 TB/s: each workgroup walks before it moves).
+// of 192 requests of 4 to 64 nodes 4.2; acceptance of one request over 24 layers 4.9 (under a tracer,
+// which adds to each). 96 requests with 34 MB of K and V to move: 16.8 us a call, 2.0 TB/s. Each of the
+// 1152 workgroups walks before it moves, and their LDS (41 KB, for 2048 nodes) lets three run on a CU
+// at once: they come in two rounds.
 #include <algorithm>
 
 #include "attn_common.hpp"
@@ -248,7 +250,7 @@ hipError_t accept_draft_tokens(const AcceptDrafts& a, const KvLayers& kv, hipStr
     const bool wide = kv.token_bytes % 16 == 0 && kv.layer_stride % 16 == 0 &&
                       (reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v)) % 16 == 0;
     const int64_t columns = kv.layers * 2 * (kv.token_bytes / (wide ? 16 : 1));
-    // a column a thread, up to about eight workgroups a CU in all
+    // a column a thread, up to 2048 workgroups in all (three run on a CU at once, by their LDS)
     const int64_t most = std::max<int64_t>(1, 2048 / a.batch);
     const int parts = static_cast<int>(
         std::clamp<int64_t>((columns + kThreads - 1) / kThreads, 1, most));

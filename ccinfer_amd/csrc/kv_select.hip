@@ -2,8 +2,10 @@
 // the cache, the most that a query can make of a block by them, and the best blocks by that.
 //
 // bounds: bf16 [blocks][kv heads][2][head_dim], the smallest and the largest of the block's keys
-// element by element: 1/16 of the bytes of the block's K and V. A score by them costs an eighth of
-// reading K, and is never below the block's largest logit (but for float32's rounding).
+// element by element: 1/16 of the bytes of the block's K and V in a bf16 cache, about 1/8 in an fp8
+// one. A score by them costs an eighth of reading K (fp8: a quarter). It is never below the block's
+// largest logit but for float32's rounding and, over an fp8 cache with scales that are no powers of two,
+// that of the bounds to the nearest bf16.
 #include <algorithm>
 #include <cmath>
 
@@ -63,7 +65,7 @@ __device__ __forceinline__ Touched touched(const int32_t* ctx, const int32_t* qs
 // that share a block which one of them does not fill (query tokens of one request) all take the
 // tokens of the longest of them, so that it does not matter whose bounds are written last.
 // Bound by the reads: 11 operations an element leave room at HBM's rate (16 prompts, 287 MB: 64 us,
-// 4.5 TB/s; 48 rows' newest blocks: 4.6 us).
+// 4.5 TB/s; 48 rows' newest blocks: 4.2 us).
 template <bool F8>
 __global__ __launch_bounds__(kThreads) void key_bounds_kernel(
     const void* __restrict__ k_cache, const float* __restrict__ k_scale,
@@ -359,8 +361,9 @@ constexpr int kBins = 256;
 // two or three rounds and spreads the counters, where their leading bits would meet in a few.
 // A thread holds `Per` blocks that lie next to one another: ranks come from one scan. A chain of
 // meetings: 9.0 us for one row of 1251 blocks, 11 for 48 rows of up to 2000 (256 threads of eight
-// blocks: 9.4 and 9.7; 1024 bins: 11.1 and 11.5; scores asked for before the context is there: 8.7
-// and 10.8, but spilled registers in the longest rows).
+// blocks: 9.4 and 9.7, a loss for one row and a gain for many; 1024 bins: 11.1 and 11.5; scores asked
+// for before the context is there: 8.7 and 10.8, but for registers that the longest rows do not have:
+// with 64 blocks a thread 40 of them are spilled as it is).
 template <int Threads, int Per>
 __global__ __launch_bounds__(Threads) void select_kernel(const float* __restrict__ scores,
                                                          const int32_t* __restrict__ ctx,
@@ -544,7 +547,8 @@ hipError_t score_kv_blocks(const void* q, const void* bounds, const int32_t* tab
 
 hipError_t select_kv_blocks(const float* scores, const int32_t* ctx, int32_t* selected, int batch,
                             int mbpr, int hkv, int take, int first, int last, hipStream_t stream) {
-    // the fewest blocks a thread that cover the table row
+    // the fewest blocks a thread that cover the table row, whatever the number of rows (the figures of
+    // eight a thread stand at the kernel)
     if (mbpr <= 256 * 4)
         return launch_select<256, 4>(scores, ctx, selected, batch, mbpr, hkv, take, first, last,
                                      stream);

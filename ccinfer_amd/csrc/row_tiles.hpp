@@ -14,8 +14,8 @@
 // chunks (attend_shared) copy each chunk once into a ring in LDS: the first product wants 16 rows
 // of K in 16 neighbouring lanes, in memory a read of 16 lines at once, of which the address unit
 // takes one a cycle, and every wavefront by itself would ask for them again (48 trees of 8 to 64
-// nodes, 735 MB: 383 us, the address unit busy for all of it; through the ring 255, and 236 to 245
-// with V out of LDS transposed, which saves 32 of 170 vector instructions a chunk).
+// nodes, 735 MB, the kernel under a tracer: 383 us, the address unit busy for all of it; through the
+// ring 255, and 238 with V out of LDS transposed, which saves 32 of 170 vector instructions a chunk).
 #pragma once
 
 #include <type_traits>

@@ -20,12 +20,17 @@
 // straight to the output; the pieces of one that is cut go to the workspace, and the workgroups
 // of a second launch, one set for each slot in which a cut item begins, add them up.
 //
-// What bounds it: with few rows the reads of K and V; with all 256 rows of a block (256
-// operations a byte) the two wavefronts of each SIMD, whose 140 vector and 100 scalar instructions
-// a chunk, and the waits between the products, leave the matrix unit busy for 22 % of the time. 48
-// trees of 8 to 64 nodes over 735 MB of K and V, 32 / 8 heads of 128: 236 to 245 us (3.0 TB/s,
-// 0.43 PFLOP/s) and 15 for the merge. One tree of 26 nodes over 1187 tokens, 16 / 8 heads: 17.5 us,
-// of which the scan of the requests takes 2, the start 5 and the chunks 7, and 3.9 for the merge.
+// What bounds it: with few rows an item's start and end, in which nothing else is under way (8
+// requests of 2048 tokens and 8 nodes, 32 / 8 heads of 128: 36.5 us, 1.9 TB/s; 248 of 64 tokens and 8 of
+// 8192: 153 us, 2.4 TB/s); with all 256 rows of a block (256 operations a byte) the two wavefronts
+// of each SIMD, which meet and then do the same phase at once: 140 vector and 95 scalar instructions a
+// chunk, LDS reads and the waits between the products leave the matrix unit busy for 22 % of the
+// time. 48 trees of 8 to 64 nodes over 735 MB of K and V: 238 us a call, the merge with it (3.1 TB/s,
+// 0.44 PFLOP/s); over an fp8 cache (394 MB) 329, whose conversions come on top. One tree of 26 nodes
+// over 1187 tokens, 16 / 8 heads: 22 us a call; under a tracer 17.5, of which the scan of the requests
+// takes 2, the start 5 and the chunks 7, and 3.9 for the merge. Head dims of 72 to 120 spill 27
+// registers (120: 259 us, 689 MB), those over 128 have half the wavefronts and a quarter of the rows a
+// block (256: 1129 us, 1470 MB).
 #include <algorithm>
 
 #include "kernels.hpp"

@@ -11,8 +11,8 @@ attends:
     o = sparse_decode_attention(q, k, v, table, ctx, selected)
 
 Conventions are those of `ops`; blocks of 16 tokens, head dims in multiples of 8 up to 256 (64 and
-128 over an fp8 cache). Several query tokens of one request are rows of their own, with the same
-table row and the context length that each sees.
+128 over an fp8 cache). Several query tokens of one request are rows of their own in all of these
+calls, with the same table row and the context length that each sees.
 """
 from __future__ import annotations
 

@@ -486,7 +486,8 @@ size_t ccinfer_tree_attention_workspace_size(int batch_size, int total_query_tok
 /* ccinfer_prefill_attention with a mask among the new tokens in place of their order: row i of
  * request b sees the positions before its request's nodes and node j where bit j of tree_mask
  * [query_start_loc[b] + i] is set (any mask, also one without itself; a node past the mask's words
- * is seen by none). Rows that see nothing become zeros; rows of no request, and of requests whose
+ * is seen by none). Sums are held times up to 2^8: of V from 2^119 on they may pass float32, and a
+ * row of an fp8 cache that holds an infinity may make NaN of its other elements. Rows that see nothing become zeros; rows of no request, and of requests whose
  * context is shorter than their nodes, are left as they are. A node's K and V that a row does not
  * see do not reach it, infinities and NaN included. k_scale / v_scale NULL: a bf16 cache, head_dim
  * a multiple of 8 up to 256; else an fp8 cache (ccinfer_write_kv_cache_fp8), head_dim 64 or 128;
@@ -544,8 +545,9 @@ int ccinfer_accept_planned_tokens(const int32_t* draft_tokens, const int32_t* ta
 /* ---- decode over selected blocks of the context ----------------------------------------
  * Decode that reads the blocks in which a query's weight can lie. Beside each layer's K lie
  * key_bounds, bf16 [num_blocks][num_kv_heads][2][head_dim]: the smallest and the largest of each
- * block's keys, element by element (1/16 of the cache's bytes). Blocks of 16 tokens. Several
- * query tokens of one request are rows of their own, with the same table row. */
+ * block's keys, element by element (1/16 of a bf16 cache's bytes, about 1/8 of an fp8 one's). Blocks
+ * of 16 tokens. Several query tokens of one request are rows of their own, with the same table row,
+ * in all of these calls. */
 
 /* The bounds of the blocks that hold the newest tokens of each row, query_start_loc[b + 1] -
  * query_start_loc[b] of them (query_start_loc NULL: one; no fewer than were written or moved since
@@ -589,7 +591,7 @@ size_t ccinfer_sparse_decode_workspace_size(int batch_size, int num_q_heads, int
  * blocks selected [batch_size][num_kv_heads][num_selected] (numbers within the row; ones outside
  * the context, and of negative table entries, are passed over; one that is named twice counts
  * twice). Zeros for a row that sees nothing or whose context the table does not hold. Caches, head
- * dims and alignment as in ccinfer_tree_attention. */
+ * dims, alignment and the range of V as in ccinfer_tree_attention. */
 int ccinfer_sparse_decode_attention(const void* q, const void* k_cache, const void* v_cache,
                                     const float* k_scale, const float* v_scale,
                                     const int32_t* block_table, const int32_t* context_lens,
