@@ -8,6 +8,7 @@
 // 1152 workgroups walks before it moves, and their LDS (41 KB, for 2048 nodes) lets three run on a CU
 // at once: they come in two rounds.
 #include <algorithm>
+#include <cstdint>
 
 #include "attn_common.hpp"
 #include "kernels.hpp"
@@ -61,7 +62,8 @@ __global__ __launch_bounds__(kThreads) void draft_tree_kernel(
     const int32_t* row = table + static_cast<int64_t>(b) * mbpr;
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const int pos = before + i;
-        const int blk = pos / 16 < mbpr ? row[pos / 16] : -1;
+        int blk = pos / 16 < mbpr ? row[pos / 16] : -1;
+        if (blk > INT32_MAX / 16) blk = -1;  // a slot past 32 bits would be another block's
         bad |= blk < 0;
         uint32_t* m = mask + static_cast<int64_t>(first + i) * words;
         int at = words - 1;

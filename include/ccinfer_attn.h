@@ -468,8 +468,8 @@ int ccinfer_compact_kv_blocks(const int32_t* block_table, const int32_t* ref_cou
  * status [batch_size]: CCINFER_OK, or CCINFER_ERR_INVALID_ARGUMENT for a request with more than
  * max_nodes nodes, fewer context tokens than nodes, or nodes outside [0, total_tokens) (its rows
  * then get no mask, position -1 and slot -1), with a parent out of range (taken as -1) or without
- * a block for a node (slot -1). Rows of no request, before the first one's nodes or behind the last
- * one's (a padded batch), get no mask, position -1 and slot -1. */
+ * a block for a node, or one whose slots pass 32 bits (slot -1). Rows of no request, before the first
+ * one's nodes or behind the last one's (a padded batch), get no mask, position -1 and slot -1. */
 int ccinfer_build_draft_tree(const int32_t* parents, const int32_t* query_start_loc,
                              const int32_t* context_lens, const int32_t* block_table,
                              int batch_size, int total_tokens, int max_blocks_per_req,

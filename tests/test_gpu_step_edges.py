@@ -489,3 +489,13 @@ def test_bounds_and_scores_with_any_scales(gpu, hkv, d):
                 top = (g @ cache.t["k64"][s, h]).max() / np.sqrt(d)
                 slack = (np.abs(g) @ np.abs(want[table[b, j], h]).max(0)).max() / np.sqrt(d)
                 assert top <= sc[b, h, j] + tol[b, h, j] + slack * (2.0 ** -8 + 2.0 ** -23)
+
+
+def test_plan_of_blocks_whose_slots_pass_32_bits(gpu):
+    """Such a table entry is no block: its slots would come out as those of another one."""
+    say("plan of blocks of 2^27 and more")
+    table = i32([[1 << 27, 3], [1 << 28, 2], [(1 << 27) - 1, 1], [2 ** 31 - 1, 0]], gpu)
+    plan = cc.build_draft_tree(i32([-1, 0] * 4, gpu), i32([0, 2, 4, 6, 8], gpu),
+                               i32([17] * 4, gpu), table, 2)
+    assert host(plan["status"]).tolist() == [6, 6, 0, 6]
+    assert host(plan["slot_mapping"]).tolist() == [-1, 48, -1, 32, 2 ** 31 - 1, 16, -1, 0]
